@@ -158,6 +158,7 @@ std::vector<int64_t> gemm_plan(int64_t M, int64_t N, int64_t K) {
 void register_kernel_ops(pybind11::module& m);  // defined in ops_bindings.cpp
 void register_runtime(pybind11::module& m);     // defined in runtime.cpp
 void register_symm(pybind11::module& m);        // defined in symm.cpp
+void register_ffn(pybind11::module& m);         // defined in ffn_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "arc_forge_2026_b200 native kernels (sm_100a)";
@@ -172,4 +173,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_kernel_ops(m);
   register_runtime(m);
   register_symm(m);
+  register_ffn(m);
 }

@@ -1,0 +1,233 @@
+// Bindings of the gated feed-forward block, the norms with trainable weights and dropout: argument checks,
+// allocation of results and scratch on the tensors' own device, launch on that device's current stream.
+#include "binding_utils.h"
+#include "ffn.h"
+
+using namespace afb_bind;
+
+namespace {
+
+using OptT = c10::optional<at::Tensor>;
+
+int elem_type(const at::Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return afb::ELEM_BF16;
+    case at::kHalf: return afb::ELEM_FP16;
+    case at::kFloat: return afb::ELEM_FP32;
+    default: TORCH_CHECK(false, what, ": bf16, fp16 or fp32 expected, got ", t.scalar_type());
+  }
+}
+
+// rows a TMA tensor map can walk: unit inner stride, row stride a multiple of 16 bytes, 16-byte aligned base; copied
+// into that form when they are not
+at::Tensor tma_rows(const at::Tensor& t) {
+  const int64_t e = t.element_size();
+  const bool ok = t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) * e % 16 == 0)) &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  if (ok) return t;
+  at::Tensor c = at::empty(t.sizes(), t.options());
+  c.copy_(t);
+  return c;
+}
+int64_t ld(const at::Tensor& t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+afb::FfnShape ffn_shape(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, int64_t act) {
+  AFB_CHECK_CUDA(x);
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "gated_ffn: bf16 or fp16 x");
+  TORCH_CHECK(x.dim() == 2 && w13.dim() == 2 && w2.dim() == 2, "gated_ffn: x [T, H], w13 [2F, H], w2 [N, F]");
+  TORCH_CHECK(w13.size(1) == x.size(1) && w13.size(0) == 2 * w2.size(1), "gated_ffn: x [T, H], w13 [2F, H], w2 [N, F]");
+  TORCH_CHECK(x.size(1) > 0 && w2.size(1) > 0 && w2.size(0) > 0 && x.size(1) % 8 == 0 && w2.size(1) % 8 == 0 &&
+                  w2.size(0) % 8 == 0,
+              "gated_ffn: H, F and N are multiples of 8");
+  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 1024 && x.size(1) < (1 << 24) && w13.size(0) < (1 << 24) &&
+                  w2.size(0) < (1 << 24),
+              "gated_ffn: size out of range");
+  TORCH_CHECK(act >= 0 && act <= 2, "gated_ffn: act is 0 (silu), 1 (tanh-GELU) or 2 (erf-GELU)");
+  for (const at::Tensor* t : {&w13, &w2})
+    TORCH_CHECK(t->device() == x.device() && t->scalar_type() == x.scalar_type(),
+                "gated_ffn: weights are on x's device, in its type");
+  afb::FfnShape s;
+  s.T = x.size(0), s.H = (int)x.size(1), s.F = (int)w2.size(1), s.N = (int)w2.size(0);
+  s.act = (int)act, s.fp16 = x.scalar_type() == at::kHalf;
+  return s;
+}
+
+at::Tensor scratch_of(size_t n, const at::Tensor& like) {
+  return at::empty({(int64_t)n}, like.options().dtype(at::kFloat));
+}
+
+// (y, h, gu): h and gu are what ffn_bwd reads; gu is kept only when `save`
+std::tuple<at::Tensor, at::Tensor, OptT> gated_ffn_fwd(const at::Tensor& x_, const at::Tensor& w13_,
+                                                       const at::Tensor& w2_, OptT residual, int64_t act, bool save) {
+  const afb::FfnShape s = ffn_shape(x_, w13_, w2_, act);
+  c10::cuda::CUDAGuard g(x_.device());
+  const at::Tensor x = tma_rows(x_), w13 = tma_rows(w13_.contiguous()), w2 = tma_rows(w2_.contiguous());
+  at::Tensor r;
+  if (residual.has_value()) {
+    TORCH_CHECK(residual->dim() == 2 && residual->size(0) == s.T && residual->size(1) == s.N &&
+                    residual->scalar_type() == x.scalar_type() && residual->device() == x.device(),
+                "gated_ffn: residual is [T, N] in x's type on its device");
+    r = tma_rows(*residual);
+  }
+  at::Tensor y = at::empty({s.T, s.N}, x.options()), h = at::empty({s.T, s.F}, x.options());
+  OptT gu;
+  if (save) gu = at::empty({s.T, 2 * (int64_t)s.F}, x.options().dtype(at::kFloat));
+  const at::Tensor scr = scratch_of(afb::ffn_fwd_scratch(s, num_sms()), x);
+  check_rc(afb::ffn_fwd(s, x.data_ptr(), ld(x), w13.data_ptr(), w2.data_ptr(), r.defined() ? r.data_ptr() : nullptr,
+                        r.defined() ? ld(r) : 0, h.data_ptr(), optr<float>(gu), y.data_ptr(), ptr<float>(scr), num_sms(), status_ptr(x.get_device()), stream()),
+           "gated_ffn_fwd");
+  return {y, h, gu};
+}
+
+// (dx, dw13, dw2), each None unless asked for
+std::tuple<OptT, OptT, OptT> gated_ffn_bwd(const at::Tensor& dy_, const at::Tensor& x_, const at::Tensor& w13_,
+                                           const at::Tensor& w2_, OptT h, OptT gu, int64_t act, bool need_dx,
+                                           bool need_dw13, bool need_dw2) {
+  const afb::FfnShape s = ffn_shape(x_, w13_, w2_, act);
+  TORCH_CHECK(dy_.dim() == 2 && dy_.size(0) == s.T && dy_.size(1) == s.N && dy_.scalar_type() == x_.scalar_type() &&
+                  dy_.device() == x_.device(),
+              "gated_ffn: dy is [T, N] in x's type on its device");
+  if (need_dw2)
+    TORCH_CHECK(h.has_value() && h->is_contiguous() && h->scalar_type() == x_.scalar_type() && h->dim() == 2 &&
+                    h->size(0) == s.T && h->size(1) == s.F && h->device() == x_.device(),
+                "gated_ffn: h of the forward pass");
+  if (need_dx || need_dw13)
+    TORCH_CHECK(gu.has_value() && gu->is_contiguous() && gu->scalar_type() == at::kFloat && gu->dim() == 2 &&
+                    gu->size(0) == s.T && gu->size(1) == 2 * (int64_t)s.F && gu->device() == x_.device(),
+                "gated_ffn: gu of the forward pass");
+  c10::cuda::CUDAGuard g(x_.device());
+  const at::Tensor x = tma_rows(x_), w13 = tma_rows(w13_.contiguous()), w2 = tma_rows(w2_.contiguous()),
+                   dy = tma_rows(dy_);
+  OptT dx, dw13, dw2;
+  at::Tensor dgu;
+  if (need_dx || need_dw13) dgu = at::empty({s.T, 2 * (int64_t)s.F}, x.options());
+  if (need_dx) dx = at::empty({s.T, s.H}, x.options());
+  if (need_dw13) dw13 = at::empty({2 * (int64_t)s.F, s.H}, x.options());
+  if (need_dw2) dw2 = at::empty({s.N, s.F}, x.options());
+  if (s.T == 0) {
+    if (dw13) dw13->zero_();
+    if (dw2) dw2->zero_();
+    return {dx, dw13, dw2};
+  }
+  const at::Tensor scr = scratch_of(afb::ffn_bwd_scratch(s, num_sms()), x);
+  check_rc(afb::ffn_bwd(s, dy.data_ptr(), ld(dy), x.data_ptr(), ld(x), w13.data_ptr(), w2.data_ptr(), optr<void>(h),
+                        optr<float>(gu), dgu.defined() ? dgu.data_ptr() : nullptr, optr<void>(dx), optr<void>(dw13),
+                        optr<void>(dw2), ptr<float>(scr), num_sms(), status_ptr(x.get_device()), stream()),
+           "gated_ffn_bwd");
+  return {dx, dw13, dw2};
+}
+
+afb::NormArgs norm_args(const at::Tensor& x, const at::Tensor& w, bool rms, double eps) {
+  AFB_CHECK_CUDA(x);
+  TORCH_CHECK(x.dim() == 2 && (x.stride(1) == 1 || x.size(1) == 1), "norm: x is [rows, width] with unit inner stride");
+  afb::NormArgs a;
+  a.rows = x.size(0), a.width = (int)x.size(1), a.rms = rms, a.eps = (float)eps;
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= afb::NORM_MAX_WIDTH, "norm: rows of 1 to ", afb::NORM_MAX_WIDTH);
+  a.dtype = elem_type(x, "norm x");
+  a.wtype = elem_type(w, "norm w");
+  TORCH_CHECK(a.wtype == a.dtype || a.wtype == afb::ELEM_FP32, "norm: weights in x's type or fp32");
+  TORCH_CHECK(w.device() == x.device() && w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous(),
+              "norm: w is contiguous [width] on x's device");
+  a.x = x.data_ptr(), a.ldx = x.stride(0), a.w = w.data_ptr();
+  return a;
+}
+
+// (y, mean, rstd); mean and rstd only when `save` (mean not for rms)
+std::tuple<at::Tensor, OptT, OptT> norm_train_fwd(const at::Tensor& x, const at::Tensor& w, OptT b, double eps,
+                                                  bool rms, bool save) {
+  afb::NormArgs a = norm_args(x, w, rms, eps);
+  if (b.has_value()) {
+    TORCH_CHECK(!rms, "norm: rms has no bias");
+    TORCH_CHECK(b->device() == x.device() && b->sizes() == w.sizes() && b->scalar_type() == w.scalar_type() &&
+                    b->is_contiguous(),
+                "norm: b is like w");
+    a.b = b->data_ptr();
+  }
+  c10::cuda::CUDAGuard g(x.device());
+  at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  OptT mean, rstd;
+  if (save) {
+    rstd = at::empty({a.rows}, x.options().dtype(at::kFloat));
+    if (!rms) mean = at::empty({a.rows}, x.options().dtype(at::kFloat));
+  }
+  a.y = y.data_ptr(), a.mean = optr<float>(mean), a.rstd = optr<float>(rstd);
+  check_rc(afb::norm_fwd(a, num_sms(), stream()), "norm_train_fwd");
+  return {y, mean, rstd};
+}
+
+// (dx, dw, db), each None unless asked for
+std::tuple<OptT, OptT, OptT> norm_train_bwd(const at::Tensor& dy_, const at::Tensor& x, const at::Tensor& w, OptT mean,
+                                            const at::Tensor& rstd, bool rms, bool need_dx, bool need_dw,
+                                            bool need_db) {
+  afb::NormArgs a = norm_args(x, w, rms, 0.);
+  TORCH_CHECK(dy_.sizes() == x.sizes() && dy_.scalar_type() == x.scalar_type() && dy_.device() == x.device(),
+              "norm: dy is like x");
+  TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.is_contiguous() && rstd.numel() == a.rows &&
+                  rstd.device() == x.device(),
+              "norm: rstd of the forward pass");
+  TORCH_CHECK(rms || (mean.has_value() && mean->scalar_type() == at::kFloat && mean->is_contiguous() &&
+                      mean->numel() == a.rows && mean->device() == x.device()),
+              "norm: mean of the forward pass");
+  c10::cuda::CUDAGuard g(x.device());
+  const at::Tensor dy = dy_.contiguous();
+  OptT dx, dw, db;
+  if (need_dx) dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  if (need_dw) dw = at::empty(w.sizes(), w.options());
+  if (need_db) db = at::empty(w.sizes(), w.options());
+  if (a.rows == 0) {
+    if (dw) dw->zero_();
+    if (db) db->zero_();
+    return {dx, dw, db};
+  }
+  a.dy = dy.data_ptr(), a.mean = optr<float>(mean), a.rstd = ptr<float>(rstd);
+  a.dx = optr<void>(dx), a.dw = optr<void>(dw), a.db = optr<void>(db);
+  at::Tensor part;
+  if (need_dw || need_db) {
+    part = scratch_of((size_t)afb::norm_bwd_partials(a, num_sms()) * 2 * a.width, x);
+    a.partial = ptr<float>(part);
+  }
+  check_rc(afb::norm_bwd(a, num_sms(), stream()), "norm_train_bwd");
+  return {dx, dw, db};
+}
+
+at::Tensor dropout_op(const at::Tensor& x_, OptT residual, int64_t threshold, int64_t seed, int64_t offset, OptT rng) {
+  AFB_CHECK_CUDA(x_);
+  const int dt = elem_type(x_, "dropout x");
+  TORCH_CHECK(threshold >= 0 && threshold <= 65536, "dropout: threshold out of range");
+  c10::cuda::CUDAGuard g(x_.device());
+  const at::Tensor x = x_.contiguous();
+  at::Tensor r;
+  if (residual.has_value()) {
+    TORCH_CHECK(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() &&
+                    residual->device() == x.device(),
+                "dropout: residual is like x");
+    r = residual->contiguous();
+  }
+  const int64_t* rp = nullptr;
+  if (rng.has_value()) {
+    TORCH_CHECK(rng->scalar_type() == at::kLong && rng->dim() == 1 && rng->numel() == 2 && rng->is_contiguous() &&
+                    rng->device() == x.device(),
+                "dropout: the seed tensor is int64 [2] (seed, offset) on x's device");
+    rp = rng->data_ptr<int64_t>();
+  }
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  check_rc(afb::dropout(x.data_ptr(), r.defined() ? r.data_ptr() : nullptr, y.data_ptr(), x.numel(), dt,
+                        (uint32_t)threshold, (uint64_t)seed, (uint64_t)offset, rp, num_sms(), stream()),
+           "dropout");
+  return y;
+}
+
+}  // namespace
+
+void register_ffn(pybind11::module& m) {
+  m.def("gated_ffn_fwd", &gated_ffn_fwd, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("residual"),
+        py::arg("act"), py::arg("save"));
+  m.def("gated_ffn_bwd", &gated_ffn_bwd, py::arg("dy"), py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("h"),
+        py::arg("gu"), py::arg("act"), py::arg("need_dx"), py::arg("need_dw13"), py::arg("need_dw2"));
+  m.def("norm_train_fwd", &norm_train_fwd, py::arg("x"), py::arg("w"), py::arg("b"), py::arg("eps"), py::arg("rms"),
+        py::arg("save"));
+  m.def("norm_train_bwd", &norm_train_bwd, py::arg("dy"), py::arg("x"), py::arg("w"), py::arg("mean"),
+        py::arg("rstd"), py::arg("rms"), py::arg("need_dx"), py::arg("need_dw"), py::arg("need_db"));
+  m.def("dropout", &dropout_op, py::arg("x"), py::arg("residual"), py::arg("threshold"), py::arg("seed"),
+        py::arg("offset"), py::arg("rng"));
+}

@@ -33,7 +33,9 @@ from torch import nn
 
 from ..config import DrafterConfig
 from ..models.reference import HyperConnection, apply_rope, hc_inject, rms_norm, rope_cos_sin
+from . import kernels
 from .drafter_objective import CandidateSelector, Objective, acceptance_terms, combine, dpace_terms, opd_terms
+from .ffn import gated_ffn, native_ok
 
 
 class DrafterTrain(nn.Module):
@@ -102,17 +104,25 @@ class DrafterTrain(nn.Module):
             probe(site, x, y, gate)
         return y, gate
 
+    @staticmethod
+    def _gated(y, w13, w2):
+        """The SwiGLU feed-forward of y: fp32 products, or (registry name ``gated_ffn``, opt-in, on a GPU) the fused
+        block in bf16 over the fp32 masters."""
+        if y.is_cuda and kernels.use("gated_ffn"):
+            yb, w13b, w2b = (t.to(torch.bfloat16) for t in (y, w13, w2))
+            kernels.hit("gated_ffn", native_ok(yb, w13b, w2b))
+            return gated_ffn(yb, w13b, w2b).to(y.dtype)
+        I = w2.shape[1]
+        gu = y @ w13.t()
+        return (F.silu(gu[..., :I]) * gu[..., I:]) @ w2.t()
+
     def _ffn(self, m, y, i: int, probe):
-        I = self.cfg.intermediate_size
-        gu = y @ m.w13.t()
-        out = (F.silu(gu[..., :I]) * gu[..., I:]) @ m.w2.t()
+        out = self._gated(y, m.w13, m.w2)
         if self.cfg.ffn == "dense_shared":
-            Is = self.cfg.shared_intermediate_size
             logit = y @ m.shared_gate.t()
             if probe is not None:
                 probe(f"shared{i}", None, logit, None)
-            sg = y @ m.sw13.t()
-            out = out + torch.sigmoid(logit) * ((F.silu(sg[..., :Is]) * sg[..., Is:]) @ m.sw2.t())
+            out = out + torch.sigmoid(logit) * self._gated(y, m.sw13, m.sw2)
         return out
 
     def block_logits(self, tokens: torch.Tensor, hidden: torch.Tensor, anchors: torch.Tensor, probe=None,

@@ -1,0 +1,99 @@
+"""Gated feed-forward block ``y = (act(x Wg^T) * (x Wu^T)) W2^T (+ residual)`` with its gradients
+(``csrc/ffn.cu``): both input projections, the activation and the product are one tcgen05 kernel, the activation's
+gradient is the epilogue of the down projection's backward product, and every product reads its operands where they
+lie (no transposed copies).
+
+    y = gated_ffn(x, w13, w2)                         # x [..., H], w13 = [Wg; Wu] [2F, H], w2 [N, F]
+    y = gated_ffn(x, w13, w2, act="gelu_tanh", residual=r)
+
+Types: bf16 or fp16, weights in x's type. Sums are fp32; ``h`` and the gradients of the two pre-activations are
+rounded once to x's type (they are tensor-core operands), the pre-activations themselves are kept in fp32 for the
+backward pass (8 F bytes a row; not kept when no gradient is asked for). Results do not depend on timing or on other
+work on the GPU: every sum has a fixed order.
+
+Off the GPU, in fp32, or when H, F or N is no multiple of 8 the plain-torch form runs. The student's shared experts
+and the drafter trainer's feed-forward use it when the registry name ``gated_ffn`` is enabled
+(``--fast-kernels all`` leaves it off, so their results stay what they were).
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+ACTS = {"silu": 0, "gelu_tanh": 1, "gelu": 2}
+
+
+def _ext():
+    from ..ops import C
+    return C()
+
+
+def gated_ffn_reference(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, act: str = "silu",
+                        residual: torch.Tensor | None = None) -> torch.Tensor:
+    """The block in plain torch, in fp32 (fp64 for fp64 inputs), rounded once to x's type."""
+    ct = torch.promote_types(x.dtype, torch.float32)
+    I = w2.shape[1]
+    gu = x.to(ct) @ w13.to(ct).t()
+    g, u = gu[..., :I], gu[..., I:]
+    a = F.silu(g) if act == "silu" else F.gelu(g, approximate="tanh" if act == "gelu_tanh" else "none")
+    y = (a * u) @ w2.to(ct).t()
+    if residual is not None:
+        y = y + residual.to(ct)
+    return y.to(x.dtype)
+
+
+class _GatedFFN(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w13, w2, residual, act):
+        need_x, need_w13, need_w2 = ctx.needs_input_grad[:3]
+        y, h, gu = _ext().gated_ffn_fwd(x, w13, w2, residual, act, need_x or need_w13)
+        ctx.save_for_backward(x, w13, w2, h if need_w2 else None, gu)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w13, w2, h, gu = ctx.saved_tensors
+        need_x, need_w13, need_w2, need_r, _ = ctx.needs_input_grad
+        dx = dw13 = dw2 = None
+        if need_x or need_w13 or need_w2:
+            dx, dw13, dw2 = _ext().gated_ffn_bwd(dy, x, w13, w2, h, gu, ctx.act, need_x, need_w13, need_w2)
+        return dx, dw13, dw2, dy if need_r else None, None
+
+
+def native_ok(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> bool:
+    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and w13.dtype == x.dtype and w2.dtype == x.dtype
+            and x.shape[-1] % 8 == 0 and w2.shape[0] % 8 == 0 and w2.shape[1] % 8 == 0)
+
+
+def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, act: str = "silu",
+              residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``(act(g) * u) @ w2.T (+ residual)`` with ``[g | u] = x @ w13.T``; x [..., H], w13 [2F, H] (gate rows, then up
+    rows), w2 [N, F], residual [..., N]; ``act``: ``silu``, ``gelu_tanh`` or ``gelu``. Differentiable (once) in x,
+    w13, w2 and residual."""
+    if act not in ACTS:
+        raise ValueError(f"gated_ffn: unknown act {act!r}; known: {', '.join(ACTS)}")
+    if w13.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w13.shape[1] != x.shape[-1] \
+            or w13.shape[0] != 2 * w2.shape[1]:
+        raise ValueError(f"gated_ffn: x [..., H], w13 [2F, H], w2 [N, F]; got {tuple(x.shape)}, {tuple(w13.shape)}, "
+                         f"{tuple(w2.shape)}")
+    if 0 in (x.shape[-1], *w2.shape):
+        raise ValueError("gated_ffn: empty feature dimension")
+    for name, t in (("w13", w13), ("w2", w2), ("residual", residual)):
+        if t is not None and (t.device != x.device or t.dtype != x.dtype):
+            raise ValueError(f"gated_ffn: {name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
+    out_shape = (*x.shape[:-1], w2.shape[0])
+    if residual is not None and residual.shape != out_shape:
+        raise ValueError(f"gated_ffn: residual {tuple(residual.shape)}, result {out_shape}")
+    if not native_ok(x, w13, w2):
+        return gated_ffn_reference(x, w13, w2, act, residual)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, w2.shape[0])
+    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad
+                                    or (r2 is not None and r2.requires_grad)):
+        y = _GatedFFN.apply(x2, w13, w2, r2, ACTS[act])
+    else:
+        y = _ext().gated_ffn_fwd(x2, w13, w2, r2, ACTS[act], False)[0]
+    return y if x.dim() == 2 else y.view(out_shape)

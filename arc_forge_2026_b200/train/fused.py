@@ -6,11 +6,15 @@ math of ``models.reference`` off the GPU, or when a shape is outside what the ke
 oracles the GPU tests compare against. The reference's counterparts are its fused Triton training kernels
 (``training/work/qwen38fn_lora/trainer_kernels.py:234-290`` GatedRMSNormFLA, ``int3_moe.py:108-152,376-430``
 SwiGLU and token aggregation, ``fp8_moe.py`` _swiglu_backward / _routing_backward).
+
+Beside them, with trainable weights: :func:`layer_norm` and :func:`rms_norm` (``csrc/norm_train.cu``) and
+:func:`dropout` from a counter-based generator (``csrc/dropout.cu``); the gated feed-forward block is ``train/ffn.py``.
 """
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ..models import reference as R
 from . import kernels
@@ -99,14 +103,181 @@ def _norm_ok(x, w) -> bool:
     return _gpu_bf16(x) and x.shape[-1] in _NORM_H and x.dim() >= 2 and not w.requires_grad
 
 
+class _TrainNorm(torch.autograd.Function):
+    """LayerNorm / zero-centred RMSNorm with gradients of x, w and b (``csrc/norm_train.cu``); x [rows, width]."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, eps, rms):
+        save = any(ctx.needs_input_grad[:3])
+        y, mean, rstd = _ext().norm_train_fwd(x, w, b, eps, rms, save)
+        ctx.save_for_backward(x, w, mean, rstd)
+        ctx.rms = rms
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, mean, rstd = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx, dw, db = _ext().norm_train_bwd(dy, x, w, mean, rstd, ctx.rms, need_x, need_w, need_b)
+        return dx, dw, db, None, None
+
+
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+_NORM_MAX_WIDTH = 16384
+
+
+def _train_norm_ok(x, w) -> bool:
+    return (x.is_cuda and w.device == x.device and x.dtype in _FLOATS and w.dtype in (x.dtype, torch.float32)
+            and 1 <= x.shape[-1] <= _NORM_MAX_WIDTH)
+
+
+def _train_norm(x, w, b, eps, rms):
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x2.stride(-1) != 1:
+        x2 = x2.contiguous()
+    w = w.contiguous()
+    b = None if b is None else b.contiguous()
+    if torch.is_grad_enabled() and (x2.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
+        y = _TrainNorm.apply(x2, w, b, eps, rms)
+    else:
+        y = _ext().norm_train_fwd(x2, w, b, eps, rms, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
+
+
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
-    """Zero-centred RMSNorm ``x / rms(x) * (1 + w)`` (frozen w) of ``models.reference.rms_norm``."""
+    """Zero-centred RMSNorm ``x / rms(x) * (1 + w)`` of ``models.reference.rms_norm``: a frozen w at the model's widths
+    in bf16 on the student's kernel, a trainable w (gradient of w in w's type), any other width up to 16,384, fp16
+    and fp32 on the trainable norm's."""
     if kernels.use("rms_norm") and _norm_ok(x, w):
         kernels.hit("rms_norm", True)
         return _RMSNorm.apply(x, w.float().contiguous(), eps, None)
+    if kernels.use("rms_norm") and w.shape == x.shape[-1:] and _train_norm_ok(x, w):
+        kernels.hit("rms_norm", True)
+        return _train_norm(x, w, None, eps, True)
     if x.is_cuda:
         kernels.hit("rms_norm", False)
     return R.rms_norm(x, w, eps)
+
+
+def layer_norm_reference(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None, eps: float) -> torch.Tensor:
+    """LayerNorm over the last dim in fp32 (fp64 for fp64 inputs), rounded once to x's type."""
+    ct = torch.promote_types(x.dtype, torch.float32)
+    z = x.to(ct)
+    z = z - z.mean(-1, keepdim=True)
+    y = z * torch.rsqrt(z.square().mean(-1, keepdim=True) + eps) * w.to(ct)
+    return (y if b is None else y + b.to(ct)).to(x.dtype)
+
+
+def layer_norm(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """LayerNorm ``(x - mean) / sqrt(var + eps) * w (+ b)`` over the last dim (1 to 16,384 wide), differentiable (once)
+    in x, w and b; x bf16, fp16 or fp32, w and b in x's type or fp32 (their gradients come in their own type).
+    Statistics and sums are fp32 and of fixed order."""
+    if x.dim() < 1 or w.shape != x.shape[-1:] or (b is not None and b.shape != w.shape):
+        raise ValueError(f"layer_norm: x {tuple(x.shape)}, w {tuple(w.shape)}"
+                         + ("" if b is None else f", b {tuple(b.shape)}"))
+    if w.device != x.device or (b is not None and (b.device != w.device or b.dtype != w.dtype)):
+        raise ValueError("layer_norm: w and b on x's device, b in w's type")
+    if kernels.use("layer_norm") and _train_norm_ok(x, w):
+        kernels.hit("layer_norm", True)
+        return _train_norm(x, w, b, eps, False)
+    if x.is_cuda:
+        kernels.hit("layer_norm", False)
+    return layer_norm_reference(x, w, b, eps)
+
+
+def _i64(v: int) -> int:
+    """v mod 2^64 as a signed 64-bit integer."""
+    v &= (1 << 64) - 1
+    return v - (1 << 64) if v >> 63 else v
+
+
+def dropout_threshold(p: float) -> int:
+    """An element stays when its 16 random bits are below this: (1 - p) in 2^-16 steps."""
+    return int((1.0 - p) * 65536 + 0.5)
+
+
+def dropout_keep_reference(n: int, p: float, seed: int, offset: int = 0, device=None) -> torch.Tensor:
+    """Which of n elements :func:`dropout` keeps: element i takes bits 16 (i % 8) .. of the 128-bit output of
+    Philox4x32-10 with key ``seed`` and counter ``offset + i // 8``."""
+    m32 = 0xFFFFFFFF
+    ctr = torch.arange((n + 7) // 8, dtype=torch.int64, device=device) + _i64(offset)
+    s = [ctr & m32, (ctr >> 32) & m32, torch.zeros_like(ctr), torch.zeros_like(ctr)]
+    k0, k1 = seed & m32, (seed >> 32) & m32
+
+    def mul(a, m):  # 32 x 32 -> (high, low) without leaving int64
+        lo = a * (m & 0xFFFF)
+        mid = a * (m >> 16) + (lo >> 16)
+        return mid >> 16, ((mid & 0xFFFF) << 16) | (lo & 0xFFFF)
+    for _ in range(10):
+        ah, al = mul(s[0], 0xD2511F53)
+        bh, bl = mul(s[2], 0xCD9E8D57)
+        s = [bh ^ s[1] ^ k0, bl, ah ^ s[3] ^ k1, al]
+        k0, k1 = (k0 + 0x9E3779B9) & m32, (k1 + 0xBB67AE85) & m32
+    bits = torch.stack([(v >> sh) & 0xFFFF for v in s for sh in (0, 16)], 1).reshape(-1)[:n]
+    return bits < dropout_threshold(p)
+
+
+def _dropout_plain(x, residual, p, seed, offset, rng):
+    if rng is not None:
+        seed, offset = seed + int(rng[0]), offset + int(rng[1])
+    keep = dropout_keep_reference(x.numel(), p, seed, offset, x.device).view(x.shape)
+    t = dropout_threshold(p)
+    ct = torch.promote_types(x.dtype, torch.float32)
+    y = torch.where(keep, x.to(ct) * (65536.0 / t if t else 0.0), torch.zeros((), dtype=ct, device=x.device))
+    return (y if residual is None else y + residual.to(ct)).to(x.dtype)
+
+
+def _dropout_any(x, residual, p, seed, offset, rng, native):
+    if native:
+        return _ext().dropout(x, residual, dropout_threshold(p), _i64(seed), _i64(offset), rng)
+    return _dropout_plain(x, residual, p, seed, offset, rng)
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset, rng, native):
+        ctx.save_for_backward(rng)
+        ctx.args = (p, seed, offset, native)
+        return _dropout_any(x, residual, p, seed, offset, rng, native)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (rng,) = ctx.saved_tensors
+        p, seed, offset, native = ctx.args
+        dx = _dropout_any(dy, None, p, seed, offset, rng, native) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``x`` with elements dropped with probability ``p`` and the rest scaled by 1 / (1 - p), plus ``residual`` if given
+    (``csrc/dropout.cu``). The mask is a pure function of (seed, offset) and the element's index in x's row-major
+    order; it is never stored, the backward pass makes it again, and CPU and GPU agree on it. A call uses the counters
+    ``offset .. offset + ceil(numel / 8) - 1`` of ``seed``: calls whose ranges do not meet are independent.
+
+    p in [0, 1] is taken in steps of 2^-16 (the scale is that of the rounded p, so the expectation is exact); a dropped
+    element is 0 whatever it held. ``seed``: an int, or an int64 tensor [2] = (seed, offset) on x's device, read when
+    the kernel runs (a captured graph draws anew when the tensor is updated between replays; not between a forward and
+    its backward); ``offset`` is added to the tensor's."""
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout: p = {p} is not in [0, 1]")
+    rng = None
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.shape != (2,) or seed.device != x.device:
+            raise ValueError("dropout: the seed tensor is int64 [2] (seed, offset) on x's device")
+        rng, seed = seed.contiguous(), 0
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype
+                                 or residual.device != x.device):
+        raise ValueError("dropout: residual has x's shape, type and device")
+    if not x.is_floating_point():
+        raise ValueError(f"dropout: x is {x.dtype}")
+    native = x.is_cuda and x.dtype in _FLOATS and kernels.use("dropout")
+    if x.is_cuda:
+        kernels.hit("dropout", native)
+    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        return _Dropout.apply(x, residual, float(p), int(seed), int(offset), rng, native)
+    return _dropout_any(x, residual, float(p), int(seed), int(offset), rng, native)
 
 
 def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:

@@ -21,11 +21,12 @@ import threading
 
 NAMES = ("gdn_chunk", "conv_silu", "rms_norm", "gated_rms_norm", "swiglu", "moe_combine", "moe_dispatch",
          "int3_weight", "fp8_weight", "topk_tail_kl", "hc", "ple", "lora_grad",
-         "grouped_gemm", "attention")
+         "grouped_gemm", "attention", "layer_norm", "dropout", "gated_ffn")
 
-# opt-in kernels: correct and tested, but slower than the path they replace at the QAD shapes (measured), so "all"
-# leaves them off; name them explicitly to run them
-OPT_IN = {"grouped_gemm"}
+# opt-in kernels, left off by "all" (name them explicitly to run them): grouped_gemm is slower than the path it
+# replaces at the QAD shapes (measured); gated_ffn rounds the shared experts' feed-forward at other places than the
+# separate products do, so runs that do not ask for it keep their results
+OPT_IN = {"grouped_gemm", "gated_ffn"}
 
 _lock = threading.Lock()
 _enabled: set[str] = set(NAMES) - OPT_IN

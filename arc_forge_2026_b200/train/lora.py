@@ -76,14 +76,25 @@ class _LoRANative(torch.autograd.Function):
 
 
 class LoRAAdapter(nn.Module):
-    def __init__(self, in_features: int, out_features: int, r: int, alpha: float, device, generator=None):
+    """``dropout`` > 0: in training mode the adapter reads its input through ``fused.dropout`` with the generator
+    (``dropout_seed``, ``dropout_step``), so a recomputed forward (activation checkpointing) and a resumed run draw
+    the same masks; the trainer sets the step before each forward (:func:`set_dropout_step`)."""
+
+    def __init__(self, in_features: int, out_features: int, r: int, alpha: float, device, generator=None,
+                 dropout: float = 0.0, dropout_seed: int = 0):
         super().__init__()
+        if not 0.0 <= dropout < 1.0:
+            raise ValueError(f"LoRA dropout {dropout} is not in [0, 1)")
         self.r, self.alpha, self.scale = r, alpha, alpha / r
+        self.dropout, self.dropout_seed, self.dropout_step = dropout, dropout_seed, 0
         self.A = nn.Parameter(torch.randn(r, in_features, generator=generator, device=device) / math.sqrt(in_features))
         self.B = nn.Parameter(torch.zeros(out_features, r, device=device))
 
     def forward(self, x):
-        from . import kernels
+        from . import fused, kernels
+        if self.dropout and self.training:
+            # a step's counters: 2^36 blocks of eight elements, more than one call takes
+            x = fused.dropout(x, self.dropout, self.dropout_seed, self.dropout_step << 36)
         if (x.is_cuda and kernels.use("lora_grad") and self.r in (8, 16, 32, 64) and x.shape[-1] % 8 == 0
                 and self.B.shape[0] % 8 == 0):
             return _LoRANative.apply(x, self.A, self.B, self.scale)
@@ -95,8 +106,10 @@ class LoRAAdapter(nn.Module):
         return (self.B.float() @ self.A.float()) * self.scale
 
 
-def attach_lora(student, r: int = 16, alpha: float = 32.0, targets=DEFAULT_TARGETS, seed: int = 0):
-    """Freeze every student parameter and attach adapters to the ``targets`` projections of every layer.
+def attach_lora(student, r: int = 16, alpha: float = 32.0, targets=DEFAULT_TARGETS, seed: int = 0,
+                dropout: float = 0.0):
+    """Freeze every student parameter and attach adapters to the ``targets`` projections of every layer (``dropout``:
+    probability of an input element of an adapter being dropped in training; each adapter has its own masks).
     Returns the adapter parameters (the only trainable ones)."""
     for p in student.parameters():
         p.requires_grad_(False)
@@ -107,10 +120,19 @@ def attach_lora(student, r: int = 16, alpha: float = 32.0, targets=DEFAULT_TARGE
             w = getattr(layer, name, None)
             if w is None:
                 continue
-            ad = LoRAAdapter(w.shape[1], w.shape[0], r, alpha, w.device, g)
+            ad = LoRAAdapter(w.shape[1], w.shape[0], r, alpha, w.device, g, dropout, (seed << 32) + len(params))
             layer.lora[name] = ad
             params += [ad.A, ad.B]
     return params
+
+
+def set_dropout_step(student, step: int):
+    """Number (0 .. 2^27 - 1) of the forward that follows: another number draws other masks in every adapter."""
+    if not 0 <= step < 1 << 27:
+        raise ValueError(f"dropout step {step} is not in [0, 2^27)")
+    for layer in student.layers:
+        for ad in layer.lora.values():
+            ad.dropout_step = step
 
 
 def lora_state(student) -> dict[str, torch.Tensor]:

@@ -17,7 +17,8 @@ as the reference's image rows do (``training/work/qwen38fn_lora/multimodal.py:10
 parallel run takes bins r, r + world, ... Each optimizer step runs ``--bins-per-step`` bins per rank; the loss is the
 token mean of -log p(label) over the step's trained tokens on all ranks; adapter gradients are averaged over ranks
 (replicated LoRA, one fp32 all-reduce), clipped by global norm, AdamW with bf16 moments. ``--offload-checkpoints``
-keeps the layer checkpoints in pinned host memory (``train/offload.py``). At the end (and with ``--save-every``)
+keeps the layer checkpoints in pinned host memory (``train/offload.py``). ``--lora-dropout`` drops elements of the
+adapters' inputs; the masks are a function of (seed, adapter, step, rank, bin), so a resumed run draws the same ones. At the end (and with ``--save-every``)
 the adapters and optimizer state are saved, and ``--export`` writes the merged model (``fn-lora-merged-v2``).
 """
 from __future__ import annotations
@@ -85,12 +86,16 @@ def media_inputs(tower, images, ids: torch.Tensor, image_token_id: int, merge: i
 
 
 def step_loss(student, bins, total_tokens: int, temperature: float = 1.0, offload: bool = False, media=None,
-              tower=None, image_token_id: int = -1):
+              tower=None, image_token_id: int = -1, dropout_step: int | None = None):
     """Backward of sum(-log p) / total_tokens over ``bins``; returns the summed loss (float). ``media[i]``: the image
-    list of bin i's one sequence (None for text bins)."""
+    list of bin i's one sequence (None for text bins). ``dropout_step``: the number of the first bin's forward for the
+    adapters' dropout (bin i takes the i-th after it)."""
+    from .lora import set_dropout_step
     from .losses import selective_logprob
     tot = 0.0
     for i, b in enumerate(bins):
+        if dropout_step is not None:
+            set_dropout_step(student, dropout_step + i)
         ctx = contextlib.nullcontext()
         if offload and b.ids.is_cuda:
             from .offload import CheckpointOffload
@@ -129,6 +134,8 @@ def main(argv=None):
     ap.add_argument("--lr", type=float, default=1e-4)
     ap.add_argument("--lora-r", dest="lora_r", type=int, default=16)
     ap.add_argument("--lora-alpha", dest="lora_alpha", type=float, default=32.0)
+    ap.add_argument("--lora-dropout", dest="lora_dropout", type=float, default=0.0,
+                    help="probability of dropping an input element of an adapter in training")
     ap.add_argument("--max-norm", dest="max_norm", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--offload-checkpoints", dest="offload", action="store_true")
@@ -166,7 +173,7 @@ def main(argv=None):
         from .optim import AdamWBF16 as _Opt
         groups = [{"params": [p for p in student.parameters() if p.requires_grad], "lr": 0.0}]
         load_dcp(args.init, student, _Opt(groups))  # masters only matter here
-    params = attach_lora(student, args.lora_r, args.lora_alpha, seed=args.seed)
+    params = attach_lora(student, args.lora_r, args.lora_alpha, seed=args.seed, dropout=args.lora_dropout)
     opt = AdamWBF16([{"params": params, "lr": args.lr}])
     media_ex: list = []
     seqs, masks = load_examples(args.data, media_ex)
@@ -223,7 +230,8 @@ def main(argv=None):
         t0 = time.perf_counter()
         opt.zero_grad(set_to_none=True)
         loss_sum = step_loss(student, mine, int(total.item()), offload=args.offload, media=mine_media, tower=tower,
-                             image_token_id=args.image_token_id)
+                             image_token_id=args.image_token_id,
+                             dropout_step=(step * world + rank) * args.bins_per_step if args.lora_dropout else None)
         ls = torch.tensor([loss_sum], device=dev, dtype=torch.float64)
         if world > 1:
             from ..parallel.shard_optim import average_gradients

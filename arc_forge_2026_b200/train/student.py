@@ -22,8 +22,9 @@ from ..config import FULL, ModelConfig
 from ..models import reference as R
 from ..models.ple import PLELayer
 from ..quant.int3_tiles import codes_to_tiles
-from . import fused
+from . import fused, kernels
 from .fakequant import fp8_weight, int3_weight
+from .ffn import gated_ffn, native_ok
 from .hc import hc_inject, hc_read
 from .gdn_chunk import chunk_gated_delta_rule
 
@@ -141,8 +142,12 @@ class StudentMoE(nn.Module):
         y = grouped_linear(h, W2, counts)
         # back to (token, k) order, weighted by the router and summed over k
         out = fused.moe_combine(y, inv, w)
-        gu = x @ self.shared_w13.to(x.dtype).t()
-        sh = fused.swiglu(gu) @ self.shared_down.to(x.dtype).t()
+        w13, w2 = self.shared_w13.to(x.dtype), self.shared_down.to(x.dtype)
+        if x.is_cuda and kernels.use("gated_ffn"):  # opt-in: one kernel per direction for both input projections
+            kernels.hit("gated_ffn", native_ok(x, w13, w2))
+            sh = gated_ffn(x, w13, w2)
+        else:
+            sh = fused.swiglu(x @ w13.t()) @ w2.t()
         sg = torch.sigmoid(x.float() @ self.shared_expert_gate.t()).to(x.dtype)
         return out + sg * sh
 

@@ -1,0 +1,489 @@
+"""The trainers' feed-forward operators on the GPU (gated feed-forward block, trainable norms, counter-based dropout)
+against their formulas in fp64.
+
+Tolerances are elementwise bounds. With u the relative half step of the element type and e = 2^-23 the largest
+relative error of one fp32 addition (rounded or truncated), a sum of K products computed in any order is off by at most
+K e sum |a b|; a value rounded to the element type by u |v|. The bounds below add those up through each formula.
+"""
+import math
+
+import pytest
+import torch
+
+from arc_forge_2026_b200.ops import check_status
+from arc_forge_2026_b200.train import fused, kernels
+from arc_forge_2026_b200.train.ffn import gated_ffn
+
+pytestmark = pytest.mark.gpu
+dev = "cuda"
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+E = 2.0 ** -23
+
+
+def u_of(dt):
+    return torch.finfo(dt).eps / 2
+
+
+def ffn_inputs(T, H, F, N, dt, seed=0, residual=True):
+    g = torch.Generator().manual_seed(seed)
+
+    def rn(*s, k=1.0):
+        return (torch.randn(*s, generator=g) * k).to(dt).to(dev)
+    return (rn(T, H), rn(2 * F, H, k=H ** -0.5), rn(N, F, k=F ** -0.5), rn(T, N) if residual else None, rn(T, N))
+
+
+def act64(name, g):
+    if name == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    if name == "gelu":
+        c = 0.5 * (1 + torch.erf(g / math.sqrt(2)))
+        return g * c, c + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    k = math.sqrt(2 / math.pi)
+    t = torch.tanh(k * (g + 0.044715 * g ** 3))
+    return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * k * (1 + 3 * 0.044715 * g * g)
+
+
+def ffn_oracle(x, w13, w2, res, dy, act):
+    """{name: (value, bound)} in fp64."""
+    u = u_of(x.dtype)
+    x, w13, w2, dy = (t.double() for t in (x, w13, w2, dy))
+    r = torch.zeros_like(dy) if res is None else res.double()
+    F, H, T, N = w2.shape[1], x.shape[1], x.shape[0], w2.shape[0]
+    gu, gua = x @ w13.T, x.abs() @ w13.abs().T
+    g, up = gu[:, :F], gu[:, F:]
+    eg, eu = H * E * gua[:, :F], H * E * gua[:, F:]
+    a, da = act64(act, g)
+    # the activation itself in fp32: exp / tanh / erf to a few units in 2^-22 of its size or of |g|; |act'|, |act''| <= 1.2
+    ea, eda = 1.2 * eg + 16 * E * (a.abs() + g.abs()), 1.2 * eg + 16 * E * (1 + g.abs())
+    h = a * up
+    eh = u * h.abs() + (ea * (up.abs() + eu) + (a.abs() + ea) * eu) + 4 * E * h.abs()
+    y = h @ w2.T + r
+    ey = eh @ w2.abs().T + F * E * ((h.abs() + eh) @ w2.abs().T) + 2 * E * r.abs()
+    dh = dy @ w2
+    edh = N * E * (dy.abs() @ w2.abs())
+    dg, du = dh * up * da, dh * a
+    edg = edh * (up.abs() + eu) * (da.abs() + eda) + dh.abs() * (eu * (da.abs() + eda) + up.abs() * eda)
+    edu = edh * (a.abs() + ea) + dh.abs() * ea
+    dgu = torch.cat([dg, du], 1)
+    edgu = torch.cat([edg, edu], 1)
+    edgu = edgu + (u + 8 * E) * (dgu.abs() + edgu)
+    A = dgu.abs() + edgu
+    out = {"y": (y, ey), "dx": (dgu @ w13, edgu @ w13.abs() + 2 * F * E * (A @ w13.abs())),
+           "dw13": (dgu.T @ x, edgu.T @ x.abs() + T * E * (A.T @ x.abs())),
+           "dw2": (dy.T @ h, dy.abs().T @ eh + T * E * (dy.abs().T @ (h.abs() + eh)))}
+    tiny = torch.finfo(torch.float16).tiny * 2 if u == u_of(HF) else 0.0  # fp16 results below its normal range
+    return {k: (v, e + u * (v.abs() + e) + tiny) for k, (v, e) in out.items()}
+
+
+def check(got, value, bound, what):
+    assert got.shape == value.shape, what
+    d = (got.double() - value).abs()
+    bad = ~(d <= bound)
+    assert not bad.any(), (what, int(bad.sum()), float((d / bound.clamp_min(1e-300)).max()))
+
+
+def run_ffn(x, w13, w2, res, dy, act):
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, w13, w2)]
+    r = None if res is None else res.detach().clone().requires_grad_(True)
+    y = gated_ffn(*leaves, act=act, residual=r)
+    grads = torch.autograd.grad(y, leaves + ([r] if r is not None else []), dy)
+    out = {"y": y.detach(), "dx": grads[0], "dw13": grads[1], "dw2": grads[2]}
+    if r is not None:
+        assert torch.equal(grads[3], dy)
+    return out
+
+
+# rows, hidden, intermediate, outputs: one element of everything, ragged tiles, one past a tile, K tails, wide and thin
+FFN_SIZES = [(1, 8, 8, 8), (3, 64, 40, 72), (5, 8, 264, 8), (17, 200, 24, 520), (128, 256, 128, 256),
+             (129, 136, 264, 200), (257, 512, 384, 512), (64, 640, 512, 64), (1001, 72, 136, 264), (300, 264, 1032, 16)]
+
+
+@pytest.mark.parametrize("size", FFN_SIZES)
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_gated_ffn_forward_and_gradients(size, dt):
+    for i, act in enumerate(("silu", "gelu_tanh", "gelu")):
+        t = ffn_inputs(*size, dt, seed=i, residual=i != 1)
+        got = run_ffn(*t, act)
+        ref = ffn_oracle(*t, act)
+        with torch.no_grad():
+            y = gated_ffn(*t[:3], act=act, residual=t[3])
+        check_status()
+        check(y, *ref["y"], ("y without gradients", act))
+        for k in got:
+            check(got[k], *ref[k], (k, act))
+
+
+@pytest.mark.parametrize("T", [1, 2, 7, 8, 15, 16, 17, 31, 33, 64, 65, 100, 128, 129, 192, 255, 256, 257])
+def test_gated_ffn_row_counts_of_serving(T):
+    t = ffn_inputs(T, 1024, 640, 1024, BF, seed=T)
+    ref = ffn_oracle(*t, "silu")
+    with torch.no_grad():
+        y = gated_ffn(*t[:3], residual=t[3])
+    check_status()
+    check(y, *ref["y"], T)
+
+
+def test_gated_ffn_gradient_against_differences():
+    """<gradient, direction> of the kernels against the central difference of the fp64 block along the direction."""
+    x, w13, w2, res, dy = ffn_inputs(96, 128, 200, 64, BF, seed=3)
+    got = run_ffn(x, w13, w2, res, dy, "silu")
+    ref = ffn_oracle(x, w13, w2, res, dy, "silu")
+    g = torch.Generator().manual_seed(9)
+
+    def loss(x, w13, w2):
+        gu = x @ w13.T
+        a, _ = act64("silu", gu[:, :200])
+        return ((a * gu[:, 200:]) @ w2.T * dy.double()).sum()
+    base = [t.double() for t in (x, w13, w2)]
+    for i, name in enumerate(("dx", "dw13", "dw2")):
+        v = torch.randn(base[i].shape, generator=g, dtype=torch.float64).to(dev)
+        eps = 1e-5
+        lo, hi = list(base), list(base)
+        lo[i], hi[i] = base[i] - eps * v, base[i] + eps * v
+        num = (loss(*hi) - loss(*lo)) / (2 * eps)
+        bound = (ref[name][1] * v.abs()).sum() + 1e-6 * num.abs() + 1e-6 * (ref[name][0].abs() * v.abs()).sum()
+        assert (num - (got[name].double() * v).sum()).abs() <= bound, name
+
+
+def test_gated_ffn_strides_and_gradient_subsets():
+    T, H, F, N = 70, 136, 72, 40
+    x, w13, w2, res, dy = ffn_inputs(T, H, F, N, BF, seed=4)
+    ref = ffn_oracle(x, w13, w2, res, dy, "silu")
+    wide = torch.zeros(T, H + 24, dtype=BF, device=dev)
+    wide[:, 8:8 + H] = x                                    # a strided view with an aligned base
+    odd = torch.zeros(T * H + 3, dtype=BF, device=dev)
+    odd[3:] = x.reshape(-1)                                 # a base no tensor map can start at
+    tr = x.t().contiguous().t()                             # column-major rows
+    for xv in (wide[:, 8:8 + H], odd[3:].view(T, H), tr):
+        leaf = xv.detach().requires_grad_(True)
+        w13t = w13.t().contiguous().t().requires_grad_(True)
+        y = gated_ffn(leaf, w13t, w2, residual=res.t().contiguous().t())
+        dx, dw13 = torch.autograd.grad(y, [leaf, w13t], dy.t().contiguous().t())
+        check(y.detach(), *ref["y"], "y")
+        check(dx, *ref["dx"], "dx")
+        check(dw13, *ref["dw13"], "dw13")
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (0, 1, 1), (1, 0, 1)):
+        ls = [t.detach().clone().requires_grad_(bool(n)) for t, n in zip((x, w13, w2), need)]
+        y = gated_ffn(*ls, residual=res)
+        gs = torch.autograd.grad(y, [t for t in ls if t.requires_grad], dy)
+        for name, gr in zip([n for n, k in zip(("dx", "dw13", "dw2"), need) if k], gs):
+            check(gr, *ref[name], (need, name))
+    # leading dimensions, and a gradient broadcast from a scalar
+    x3 = x.view(7, 10, H).clone().requires_grad_(True)
+    gated_ffn(x3, w13, w2).sum().backward()
+    one = ffn_oracle(x, w13, w2, None, torch.ones_like(dy), "silu")
+    check(x3.grad.view(T, H), *one["dx"], "dx of a sum")
+    check_status()
+
+
+def test_gated_ffn_no_rows_and_bad_values():
+    x, w13, w2, res, dy = ffn_inputs(0, 64, 32, 48, BF)
+    leaves = [t.requires_grad_(True) for t in (x, w13, w2)]
+    y = gated_ffn(*leaves)
+    assert y.shape == (0, 48)
+    dx, dw13, dw2 = torch.autograd.grad(y, leaves, torch.empty(0, 48, dtype=BF, device=dev))
+    assert dx.shape == (0, 64) and not dw13.any() and not dw2.any()
+    # a NaN or an infinity stays in its row of y and dx
+    x, w13, w2, res, dy = ffn_inputs(200, 64, 32, 48, BF, seed=5)
+    x[3, 5], x[150, 0] = float("nan"), float("inf")
+    got = run_ffn(x, w13, w2, None, dy, "silu")
+    rest = torch.ones(200, dtype=torch.bool)
+    rest[3] = rest[150] = False
+    assert torch.isfinite(got["y"][rest]).all() and torch.isfinite(got["dx"][rest]).all()
+    assert torch.isnan(got["y"][3]).all()
+    check_status()
+
+
+def test_gated_ffn_repeats_bitwise_and_on_other_streams():
+    t = ffn_inputs(333, 256, 136, 256, BF, seed=6)
+    a = run_ffn(*t, "silu")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = run_ffn(*t, "silu")
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    for k in a:
+        assert torch.equal(a[k], b[k]), k
+
+
+def test_feed_forward_half_layer_captured_and_replayed():
+    """norm -> gated block -> dropout + residual, forward and backward, in two graphs that are replayed in turn with
+    new inputs and new random offsets; each replay equals the eager call."""
+    T, H, F = 130, 256, 136
+    _, w13, w2, _, _ = ffn_inputs(T, H, F, H, BF, seed=7)
+    g = torch.Generator().manual_seed(8)
+    nw = (1 + 0.1 * torch.randn(H, generator=g)).to(dev)
+    nb = (0.1 * torch.randn(H, generator=g)).to(dev)
+
+    def step(x, params, dy, rng):
+        y = fused.layer_norm(x, params[2], params[3], 1e-6)
+        y = gated_ffn(y, params[0], params[1])
+        y = fused.dropout(y, 0.25, rng, residual=x)
+        return [y] + list(torch.autograd.grad(y, [x, *params], dy))
+    data = [[(torch.randn(T, H, generator=g).to(BF).to(dev), torch.randn(T, H, generator=g).to(BF).to(dev),
+              torch.tensor([5 + i, 1000 * i], device=dev)) for i in range(3)] for _ in range(2)]
+    graphs = []
+    for _ in range(2):
+        x = torch.zeros(T, H, dtype=BF, device=dev).requires_grad_(True)
+        dy, rng = torch.zeros(T, H, dtype=BF, device=dev), torch.zeros(2, dtype=torch.int64, device=dev)
+        params = [t.detach().clone().requires_grad_(True) for t in (w13, w2, nw, nb)]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step(x, params, dy, rng)
+        torch.cuda.current_stream().wait_stream(s)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step(x, params, dy, rng)
+        graphs.append((gr, x, dy, rng, out))
+    for i in range(3):
+        for k, (gr, x, dy, rng, out) in enumerate(graphs):
+            with torch.no_grad():
+                x.copy_(data[k][i][0])
+                dy.copy_(data[k][i][1])
+                rng.copy_(data[k][i][2])
+            gr.replay()
+        torch.cuda.synchronize()
+        for k, (gr, x, dy, rng, out) in enumerate(graphs):
+            params = [t.detach().clone().requires_grad_(True) for t in (w13, w2, nw, nb)]
+            ref = step(data[k][i][0].clone().requires_grad_(True), params, data[k][i][1], data[k][i][2])
+            for a, b in zip(out, ref):
+                assert torch.equal(a, b), (i, k)
+    check_status()
+
+
+# ------------------------------------------------------------------------------------------------------------- norms
+def norm_oracle(x, w, b, dy, eps, rms):
+    u, uw = u_of(x.dtype), u_of(w.dtype)
+    W, T = x.shape[-1], x.shape[0]
+    x, w, dy = x.double(), w.double(), dy.double()
+    depth = 64  # additions an element goes through in a row sum: 32 of its lane, 5 of the warp, 16 of the row's warps
+    mean = torch.zeros_like(x[:, :1]) if rms else x.mean(-1, keepdim=True)
+    xc = x - mean
+    rstd = (xc.square().mean(-1, keepdim=True) + eps).rsqrt()
+    ec = 0 * x if rms else E * (x.abs() + 2 * depth * x.abs().mean(-1, keepdim=True))
+    # relative error of rstd: half that of the mean square (its sum, and the errors of xc in it), and rsqrtf
+    er = depth * E + (ec * xc.abs()).mean(-1, keepdim=True) * rstd.square() + (ec * ec).mean(-1, keepdim=True) * rstd.square()
+    xh = xc * rstd
+    eh = ec * rstd + xh.abs() * (er + 4 * E)
+    m = 1 + w if rms else w
+    bb = torch.zeros_like(w) if b is None else b.double()
+    y = xh * m + bb
+    ey = eh * m.abs() + 4 * E * ((xh * m).abs() + bb.abs())
+    v = dy * m
+    ev = 2 * E * v.abs()
+    m1 = (v * xh).mean(-1, keepdim=True)
+    em1 = (depth * E * (v * xh).abs() + ev * xh.abs() + v.abs() * eh).mean(-1, keepdim=True)
+    m0 = torch.zeros_like(m1) if rms else v.mean(-1, keepdim=True)
+    em0 = (depth * E * v.abs() + ev).mean(-1, keepdim=True)
+    dx = rstd * (v - m0 - xh * m1)
+    edx = rstd * (ev + em0 + eh * m1.abs() + xh.abs() * em1 + 4 * E * (v.abs() + m0.abs() + (xh * m1).abs())) \
+        + dx.abs() * (er + 4 * E)
+    dw, edw = (dy * xh).sum(0), (dy.abs() * eh).sum(0) + (T + 8) * E * (dy * xh).abs().sum(0)
+    db, edb = dy.sum(0), (T + 8) * E * dy.abs().sum(0)
+    tiny = torch.finfo(HF).tiny
+    return {"y": (y, ey + u * (y.abs() + ey) + tiny), "dx": (dx, edx + u * (dx.abs() + edx) + tiny),
+            "dw": (dw, edw + uw * (dw.abs() + edw) + tiny), "db": (db, edb + uw * (db.abs() + edb) + tiny)}
+
+
+def norm_inputs(T, W, dt, wdt, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = (torch.randn(T, W, generator=g) + 0.5) * torch.exp(torch.randn(T, 1, generator=g))
+    return (x.to(dt).to(dev), (1 + 0.2 * torch.randn(W, generator=g)).to(wdt).to(dev),
+            (0.2 * torch.randn(W, generator=g)).to(wdt).to(dev), torch.randn(T, W, generator=g).to(dt).to(dev))
+
+
+def run_norm(x, w, b, dy, eps, rms):
+    ls = [t.detach().requires_grad_(True) for t in ([x, w] if rms or b is None else [x, w, b])]
+    y = fused.rms_norm(ls[0], ls[1], eps) if rms else fused.layer_norm(ls[0], ls[1], ls[2] if b is not None else None, eps)
+    gs = torch.autograd.grad(y, ls, dy)
+    return dict(zip(("y", "dx", "dw", "db"), (y.detach(), *gs)))
+
+
+@pytest.mark.parametrize("W", [1, 7, 8, 33, 128, 256, 264, 768, 1001, 1024, 1152, 1160, 2048, 2056, 2560, 4095, 4608,
+                               5000, 8192, 8200, 16384])
+@pytest.mark.parametrize("rms", [False, True])
+def test_trainable_norms(W, rms):
+    for i, (dt, wdt, T) in enumerate([(BF, FP, 37), (BF, BF, 700), (HF, HF, 5), (HF, FP, 1), (FP, FP, 300)]):
+        x, w, b, dy = norm_inputs(T, W, dt, wdt, seed=i)
+        b = None if i == 2 else b
+        got = run_norm(x, w, b, dy, 1e-6, rms)
+        ref = norm_oracle(x, w, None if rms else b, dy, 1e-6, rms)
+        for k in got:
+            check(got[k], *ref[k], (k, dt, wdt, T))
+
+
+def test_norm_strides_empty_frozen_and_constant_rows():
+    x, w, b, dy = norm_inputs(50, 264, BF, FP, seed=11)
+    ref = norm_oracle(x, w, b, dy, 1e-6, False)
+    wide = torch.zeros(50, 300, dtype=BF, device=dev)
+    for off in (8, 3):  # an aligned view and one that is not
+        wide[:, off:off + 264] = x
+        got = run_norm(wide[:, off:off + 264], w, b, dy.t().contiguous().t(), 1e-6, False)
+        for k in got:
+            check(got[k], *ref[k], (k, off))
+    x0 = torch.empty(0, 264, dtype=BF, device=dev)
+    got = run_norm(x0, w, b, x0, 1e-6, False)
+    assert got["dx"].shape == (0, 264) and not got["dw"].any() and not got["db"].any()
+    # only x, only w, only b
+    for i, k in enumerate(("dx", "dw", "db")):
+        ls = [t.detach().clone().requires_grad_(j == i) for j, t in enumerate((x, w, b))]
+        (gr,) = torch.autograd.grad(fused.layer_norm(*ls, 1e-6), [ls[i]], dy)
+        check(gr, *ref[k], k)
+    # constant rows: the variance is 0 and y is the bias
+    c = torch.full((3, 264), 7.0, dtype=BF, device=dev)
+    assert torch.equal(fused.layer_norm(c, w, b, 1e-6), b.to(BF).expand(3, -1))
+    # leading dimensions
+    y = fused.layer_norm(x.view(5, 10, 264), w, b, 1e-6)
+    assert torch.equal(y.view(50, 264), fused.layer_norm(x, w, b, 1e-6))
+    # a frozen weight at the model's widths stays on the student's kernel, bit for bit
+    xs = norm_inputs(9, 2048, BF, FP, seed=12)[0]
+    ws = torch.randn(2048, device=dev) * 0.1
+    y = torch.empty_like(xs)
+    from arc_forge_2026_b200.ops import C
+    C().rmsnorm_train(xs, None, ws, 1e-6, y, torch.empty(9, device=dev), None, None, None)
+    assert torch.equal(y, fused.rms_norm(xs, ws, 1e-6))
+
+
+def test_norm_repeats_bitwise():
+    x, w, b, dy = norm_inputs(3001, 1152, BF, FP, seed=13)
+    a, c = run_norm(x, w, b, dy, 1e-6, False), run_norm(x, w, b, dy, 1e-6, False)
+    for k in a:
+        assert torch.equal(a[k], c[k]), k
+
+
+def test_many_rows_pass_32_bit_offsets():
+    """More than 2^31 elements: the last rows equal those of a small call."""
+    rows, W = (1 << 31) // 1024 + 9, 1024
+    x = torch.zeros(rows, W, dtype=BF, device=dev)
+    tail = norm_inputs(9, W, BF, FP, seed=14)
+    x[-9:] = tail[0]
+    y = fused.layer_norm(x, tail[1], tail[2], 1e-6)
+    assert torch.equal(y[-9:], fused.layer_norm(tail[0], tail[1], tail[2], 1e-6))
+    del y
+    z = fused.dropout(x, 0.5, 3, 0)
+    off = (rows - 9) * W // 8
+    assert torch.equal(z[-9:], fused.dropout(tail[0], 0.5, 3, off))
+
+
+# ----------------------------------------------------------------------------------------------------------- dropout
+@pytest.mark.parametrize("shape", [(1,), (7,), (8,), (9,), (37, 1001), (64, 256), (2, 3, 40)])
+@pytest.mark.parametrize("dt", [BF, HF, FP])
+def test_dropout_equals_its_definition(shape, dt):
+    g = torch.Generator().manual_seed(1)
+    x, r, dy = (torch.randn(*shape, generator=g).to(dt) for _ in range(3))
+    for p, seed, off in ((0.0, 1, 0), (0.1, 2 ** 63 + 17, 2 ** 32 - 2), (0.5, -5, 2 ** 40), (0.999, 7, 1), (1.0, 7, 1)):
+        for res in (None, r):
+            lx = x.to(dev).requires_grad_(True)
+            lr = None if res is None else r.to(dev).requires_grad_(True)
+            y = fused.dropout(lx, p, seed, off, residual=lr)
+            gs = torch.autograd.grad(y, [lx] + ([] if lr is None else [lr]), dy.to(dev))
+            # the scale is one fp32 number on both sides, one product and one sum are rounded once each
+            assert torch.equal(y.cpu(), fused.dropout(x, p, seed, off, residual=res)), (p, seed)
+            assert torch.equal(gs[0].cpu(), fused.dropout(dy, p, seed, off))
+            assert lr is None or torch.equal(gs[1].cpu(), dy)
+
+
+def test_dropout_views_bad_values_seed_tensors_and_streams():
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(40, 50, generator=g).to(BF).to(dev)
+    want = fused.dropout(x, 0.3, 11, 5)
+    buf = torch.zeros(2001, dtype=BF, device=dev)
+    buf[1:] = x.reshape(-1)
+    assert torch.equal(fused.dropout(buf[1:].view(40, 50), 0.3, 11, 5), want)          # unaligned base
+    assert torch.equal(fused.dropout(x.t().contiguous().t(), 0.3, 11, 5), want)        # logical order, not memory's
+    assert torch.equal(fused.dropout(x, 0.3, torch.tensor([11, 5], device=dev)), want)
+    assert torch.equal(fused.dropout(x, 0.3, torch.tensor([11, 2], device=dev), 3), want)
+    assert not torch.equal(fused.dropout(x, 0.3, 11, 6), want)
+    bad = x.clone()
+    dropped = want == 0
+    bad[dropped] = float("nan")
+    assert torch.equal(fused.dropout(bad, 0.3, 11, 5), want)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = fused.dropout(x, 0.3, 11, 5)
+    s.synchronize()
+    assert torch.equal(other, want)
+    # a seed tensor changed between forward and backward is refused, not silently another mask
+    rng = torch.tensor([1, 2], device=dev)
+    y = fused.dropout(x.clone().requires_grad_(True), 0.3, rng)
+    rng.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    assert fused.dropout(torch.empty(0, 4, dtype=BF, device=dev), 0.3, 1).shape == (0, 4)
+
+
+def test_registry_counts_the_native_calls():
+    kernels.reset()
+    x, w, b, dy = norm_inputs(4, 64, BF, FP)
+    fused.layer_norm(x, w, b)
+    fused.rms_norm(x, w.requires_grad_(True), 1e-6)
+    fused.dropout(x, 0.1, 1)
+    c = kernels.counts()
+    assert c["native"] == {"layer_norm": 1, "rms_norm": 1, "dropout": 1} and not c["fallback"]
+
+
+def _with_opt_in(fn):
+    old = {n for n in kernels.NAMES if kernels.enabled(n)}
+    try:
+        kernels.enable(sorted(old | {"gated_ffn"}))
+        kernels.reset()
+        return fn(), kernels.counts()
+    finally:
+        kernels.enable(sorted(old))
+
+
+def test_student_and_drafter_take_the_block_when_asked():
+    """The opt-in path against the default one: the same products with other roundings. Each side rounds the
+    intermediate values of one layer's shared expert a few times, so the results agree to a few bf16 half steps."""
+    from arc_forge_2026_b200.config import drafter_preset, preset
+    from arc_forge_2026_b200.train.drafter_train import DrafterTrain
+    from arc_forge_2026_b200.train.student import random_student
+    st = random_student(preset("tiny_gpu"), dev, seed=0, checkpoint_layers=False)
+    moe = st.layers[0].moe
+    x = torch.randn(130, st.cfg.hidden_size, generator=torch.Generator().manual_seed(1)).to(BF).to(dev)
+
+    def step():
+        lx = x.clone().requires_grad_(True)
+        y = moe(lx)
+        return [y.detach(), *torch.autograd.grad(y.float().square().sum(), [lx, moe.shared_w13, moe.shared_down])]
+    base = step()
+    got, counts = _with_opt_in(step)
+    assert counts["native"]["gated_ffn"] == 1 and not counts["fallback"].get("gated_ffn")
+    for a, b in zip(got, base):
+        assert a.dtype == b.dtype and ((a - b).float().norm() / b.float().norm()) < 4 * u_of(BF)
+    cfg = drafter_preset("tiny")
+    dt = DrafterTrain(cfg, 256, 512, torch.arange(128), device=dev)
+    m, y = dt.layers[0], torch.randn(6, cfg.k, cfg.hidden_size, device=dev)
+
+    def dstep():
+        o = dt._ffn(m, y, 0, None)
+        return [o.detach(), *torch.autograd.grad(o.square().sum(), [m.w13, m.w2])]
+    base = dstep()
+    got, counts = _with_opt_in(dstep)
+    assert counts["native"]["gated_ffn"] == 1
+    for a, b in zip(got, base):  # fp32 products against bf16 operands: three rounded factors a product
+        assert a.dtype == FP and ((a - b).norm() / b.norm()) < 6 * u_of(BF)
+    check_status()
+
+
+def test_lora_dropout_on_the_native_products():
+    """An adapter's output and gradients with dropout equal those of the adapter without it on the dropped input."""
+    from arc_forge_2026_b200.train.lora import LoRAAdapter
+    g = torch.Generator(device=dev).manual_seed(2)
+    ad = LoRAAdapter(256, 128, 16, 32.0, dev, g, dropout=0.2, dropout_seed=9)
+    with torch.no_grad():
+        ad.B.normal_(generator=g)
+    ad.dropout_step = 3
+    x = torch.randn(200, 256, generator=g, device=dev).to(BF).requires_grad_(True)
+    y = ad(x)
+    dx, dA, dB = torch.autograd.grad(y.square().sum(), [x, ad.A, ad.B])
+    ad.eval()
+    xd = fused.dropout(x.detach(), 0.2, 9, 3 << 36).requires_grad_(True)
+    y2 = ad(xd)
+    dx2, dA2, dB2 = torch.autograd.grad(y2.square().sum(), [xd, ad.A, ad.B])
+    assert torch.equal(y, y2) and torch.equal(dA, dA2) and torch.equal(dB, dB2)
+    assert torch.equal(dx, fused.dropout(dx2, 0.2, 9, 3 << 36))
