@@ -1,7 +1,7 @@
 // Gated feed-forward block of the trainers, forward and backward, on tcgen05:
 //
-//   g = x Wg^T, u = x Wu^T, h = act(g) u      one kernel: a 128 x 256 accumulator tile is 128 gate columns beside the
-//                                             same 128 up columns, so a thread of the epilogue holds both of a pair
+//   g = x Wg^T, u = x Wu^T, h = act(g) u      one kernel: a 256-column accumulator tile is 128 gate columns beside
+//                                             the same 128 up columns, so an epilogue thread holds both of a pair
 //   y = h W2^T (+ residual)
 //   dh = dy W2, dg = dh u act'(g), du = dh act(g)   one kernel, the activation's gradient in the epilogue
 //   dx = [dg | du] [Wg; Wu]
@@ -15,32 +15,46 @@
 // result is bitwise reproducible.
 #include <algorithm>
 
-#include "common.cuh"
 #include "ffn.h"
 #include "gemm.h"
+#include "tc_pair.cuh"
 
 namespace afb {
 namespace ffn {
 
-constexpr int BM = 128, BN = 256, BK = 64, STAGES = 4;
-constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
-constexpr uint32_t BAR_OFF = STAGES * (A_BYTES + B_BYTES);
-constexpr uint32_t SMEM = BAR_OFF + (2 * STAGES + 1) * 8 + 16 + 1024;
+// A pair of CTAs computes a 256 x 256 accumulator tile: each holds 128 rows of A and 128 of the 256 rows of B
+constexpr int BM = 256, BN = 256, BK = 64;
+constexpr uint32_t OP_BYTES = 128 * BK * 2;  // one operand of one CTA and stage
+constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
 
 enum Epi { STORE = 0, PARTIAL = 1, DUAL = 2, DACT = 3 };
 enum Layout { NT = 0, NN = 1, TN = 2 };  // A K-major B K-major | A K-major B MN-major | both MN-major
+
+template <int EPI>
+struct Smem {
+  // epilogue staging of a warp: two 4 KB buffers (a 32-row box of 128-byte rows each); DACT two more of 2 KB
+  static constexpr uint32_t EPI_BYTES = EPI == DACT ? 12288 : 8192;
+  static constexpr int STAGES = EPI == DACT ? 4 : 5;
+  static constexpr uint32_t EPI_OFF = STAGES * 2 * OP_BYTES, BAR_OFF = EPI_OFF + EPI_WARPS * EPI_BYTES;
+  static constexpr uint32_t TOTAL = BAR_OFF + (2 * STAGES + 4 + EPI_WARPS) * 8 + 16 + 1024;
+};
 
 struct Args {
   int64_t M = 0;  // rows of the result
   int N = 0;      // columns of the result (DUAL: F)
   int64_t K = 0;
-  int F = 0;      // DUAL / DACT: columns of one half of w13
+  int F = 0;      // DUAL: columns of one half of w13
   int act = 0;
-  void* out = nullptr;  // STORE: result; DUAL: h; DACT: dgu
-  int64_t ldo = 0;
-  const void* residual = nullptr;  // STORE
-  int64_t ldr = 0;
-  float* f32 = nullptr;  // PARTIAL: [splits, M, N]; DUAL: gu or null; DACT: gu
+  int splits = 1;  // PARTIAL
+  int flag = 0;    // STORE: a residual is added; DUAL: g and u are kept
+};
+// tensor maps: operands, results and what the epilogue reads
+struct Maps {
+  CUtensorMap a, b;
+  CUtensorMap out;         // STORE result, PARTIAL sums, DUAL h, DACT dg
+  CUtensorMap out2;        // DACT du
+  CUtensorMap in0, in1;    // STORE residual | DACT g, u
+  CUtensorMap gate, up;    // DUAL g, u
 };
 
 template <bool F16>
@@ -53,15 +67,17 @@ AFB_DEV float2 unpack2(uint32_t v) {
   return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v));
 }
 
-// act(x) and its derivative
+// act(x) and its derivative. The quotients are __fdividef (2 units in the last place; 0 for a divisor past 2^126, where
+// the quotient is below the smallest normal number); tanh(z) = 1 - 2 / (exp(2 z) + 1) is used as 1 + t and 1 - t^2,
+// where its absolute error of some 1e-7 is what counts.
 AFB_DEV void act_grad(float x, int act, float& a, float& d) {
   if (act == 0) {
-    const float s = 1.f / (1.f + __expf(-x));
+    const float s = __fdividef(1.f, 1.f + __expf(-x));
     a = x * s;
     d = s * (1.f + x * (1.f - s));
   } else if (act == 1) {
     const float c = 0.7978845608028654f, x2 = x * x;
-    const float t = tanhf(c * x * (1.f + 0.044715f * x2));
+    const float t = 1.f - __fdividef(2.f, 1.f + __expf(2.f * c * x * (1.f + 0.044715f * x2)));
     a = 0.5f * x * (1.f + t);
     d = 0.5f * (1.f + t) + 0.5f * x * (1.f - t * t) * c * (1.f + 0.134145f * x2);
   } else {
@@ -76,40 +92,89 @@ AFB_DEV float act_only(float x, int act) {
   return a;
 }
 
+struct Tile {
+  int64_t m0;
+  int n0, split;
+};
+// tile order: bands of 8 row tiles, down the band first, so that the tiles in flight share both operands in L2
+AFB_DEV Tile tile_at(int64_t t, int mt, int nt, int tn) {
+  Tile r;
+  const int64_t per = (int64_t)mt * nt;
+  r.split = (int)(t / per);
+  t -= r.split * per;
+  const int64_t band = t / (8ll * nt);
+  const int rows = (int)min((int64_t)8, mt - band * 8);
+  const int64_t in = t - band * 8ll * nt;
+  r.m0 = (band * 8 + in % rows) * BM;
+  r.n0 = (int)(in / rows) * tn;
+  return r;
+}
+
+// fp32 row of 32 columns / 16-bit row of 64 columns <-> a 128-byte swizzled staging row
+AFB_DEV void put_row(uint8_t* buf, int row, const uint32_t* w) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<uint4*>(buf + sw128_offset(row, j)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+AFB_DEV void get_row(const uint8_t* buf, int row, uint32_t* w) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint4 q = *reinterpret_cast<const uint4*>(buf + sw128_offset(row, j));
+    w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
+  }
+}
+// 16-bit row of 32 columns -> a 64-byte swizzled staging row
+AFB_DEV void put_half_row(uint8_t* buf, int row, const uint32_t* w) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4)) =
+        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+}
+
+// Persistent: pair p of the grid takes tiles p, p + pairs, ... Each CTA: warp 0 loads its halves of the operands by
+// TMA into a STAGES-deep ring, one thread of the leader's warp 1 issues the MMAs of both CTAs into one of two TMEM
+// accumulators, and 8 epilogue warps drain the other one (two warps a lane quadrant, half of the columns each) through
+// swizzled staging rows and TMA stores, so the tensor cores work through the next tile meanwhile.
 template <int LAYOUT, int EPI, bool F16>
-__global__ void __launch_bounds__(192, 1)
-    ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, Args g,
-                    uint32_t* status) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    ffn_gemm_kernel(const __grid_constant__ Maps maps, Args g, uint32_t* status) {
+  using S = Smem<EPI>;
+  constexpr int STAGES = S::STAGES;
   constexpr bool A_MN = LAYOUT == TN, B_MN = LAYOUT != NT;
   constexpr int TN_COLS = EPI == DUAL ? BN / 2 : BN;  // result columns per tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sA = smem;
-  uint8_t* sB = smem + STAGES * A_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);
-  uint64_t* empty = full + STAGES;
-  uint64_t* done = empty + STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);  // leader's: both CTAs' operands have landed
+  uint64_t* empty = full + STAGES;                                  // the pair's MMAs of the stage are done
+  uint64_t* acc_full = empty + STAGES;                              // [2] accumulator complete
+  uint64_t* acc_empty = acc_full + 2;                               // [2] leader's: drained by both CTAs' epilogues
+  uint64_t* ld_bar = acc_empty + 2;                                 // [EPI_WARPS] a warp's epilogue loads
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ld_bar + EPI_WARPS);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t m0 = (int64_t)blockIdx.x * BM;
-  const int n0 = blockIdx.y * TN_COLS;
+  const uint32_t rank = cluster_cta_rank();
+  const int mt = (int)((g.M + BM - 1) / BM), nt = (g.N + TN_COLS - 1) / TN_COLS;
+  const int64_t tiles = (int64_t)mt * nt * g.splits;
+  const int64_t t0 = blockIdx.x >> 1, step = gridDim.x >> 1;
   const int kb_total = (int)((g.K + BK - 1) / BK);
-  const int kb_per = (kb_total + gridDim.z - 1) / gridDim.z;
-  const int kb0 = blockIdx.z * kb_per;
-  const int num_kb = max(0, min(kb_total, kb0 + kb_per) - kb0);
+  auto kb_lo = [&](int split) { return (int)((int64_t)kb_total * split / g.splits); };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(done, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_empty[s], 2 * EPI_WARPS);
+    }
+    for (int s = 0; s < EPI_WARPS; ++s) mbar_init(&ld_bar[s], 1);
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, BN);
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   grid_dep_wait();
@@ -117,248 +182,392 @@ __global__ void __launch_bounds__(192, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      prefetch_tmap(&tmA);
-      prefetch_tmap(&tmB);
-      int issued = 0;
-      for (int i = 0; i < num_kb; ++i) {
-        const int s = i % STAGES;
-        if (i >= STAGES && !mbar_wait(&empty[s], ((i / STAGES) & 1) ^ 1, status)) break;
-        mbar_arrive_expect_tx(&full[s], A_BYTES + B_BYTES);
-        uint8_t* a = sA + s * A_BYTES;
-        uint8_t* b = sB + s * B_BYTES;
-        const int k = (kb0 + i) * BK;
-        if constexpr (A_MN) {
-#pragma unroll
-          for (int j = 0; j < BM / 64; ++j) tma_load_2d(a + j * 8192, &tmA, &full[s], (int)m0 + j * 64, k);
-        } else {
-          tma_load_2d(a, &tmA, &full[s], k, (int)m0);
+      prefetch_tmap(&maps.a);
+      prefetch_tmap(&maps.b);
+      int64_t i = 0;  // stages issued
+      bool ok = true;
+      for (int64_t t = t0; t < tiles && ok; t += step) {
+        const Tile tl = tile_at(t, mt, nt, TN_COLS);
+        const int kb1 = kb_lo(tl.split + 1);
+        const int ma = (int)tl.m0 + (int)rank * 128;
+        const int nb = EPI == DUAL ? (int)rank * g.F + tl.n0 : tl.n0 + (int)rank * 128;
+        for (int kb = kb_lo(tl.split); kb < kb1; ++kb, ++i) {
+          const int s = (int)(i % STAGES);
+          if (i >= STAGES && !mbar_wait(&empty[s], ((i / STAGES) & 1) ^ 1, status)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 4 * OP_BYTES);
+          const uint32_t bar = cluster_addr(&full[s], 0);
+          uint8_t* a = smem + s * 2 * OP_BYTES;
+          uint8_t* b = a + OP_BYTES;
+          const int k = kb * BK;
+          if constexpr (A_MN) {
+            tma_load_2d_pair(a, &maps.a, bar, ma, k);
+            tma_load_2d_pair(a + 8192, &maps.a, bar, ma + 64, k);
+          } else {
+            tma_load_2d_pair(a, &maps.a, bar, k, ma);
+          }
+          if constexpr (B_MN) {
+            tma_load_2d_pair(b, &maps.b, bar, nb, k);
+            tma_load_2d_pair(b + 8192, &maps.b, bar, nb + 64, k);
+          } else {
+            tma_load_2d_pair(b, &maps.b, bar, k, nb);
+          }
         }
-        if constexpr (B_MN) {
-#pragma unroll
-          for (int j = 0; j < BN / 64; ++j) tma_load_2d(b + j * 8192, &tmB, &full[s], n0 + j * 64, k);
-        } else {  // two boxes of 128 rows: gate and up rows of w13 (DUAL), or consecutive rows
-          tma_load_2d(b, &tmB, &full[s], k, n0);
-          tma_load_2d(b + B_BYTES / 2, &tmB, &full[s], k, EPI == DUAL ? g.F + n0 : n0 + 128);
-        }
-        ++issued;
       }
-      for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, status);
+      // every stage issued has been read (so its copies have landed) before the CTA may leave
+      for (int64_t j = max((int64_t)0, i - STAGES); j < i; ++j)
+        mbar_wait(&empty[j % STAGES], (j / STAGES) & 1, status);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc =
-          idesc_f16(128, BN, F16 ? 0 : 1) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16);
-      for (int i = 0; i < num_kb; ++i) {
-        const int s = i % STAGES;
-        if (!mbar_wait(&full[s], (i / STAGES) & 1, status)) break;
+          idesc_f16(BM, BN, F16 ? 0 : 1) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16);
+      int64_t i = 0;
+      int n = 0;  // tiles of this pair
+      bool ok = true;
+      for (int64_t t = t0; t < tiles && ok; t += step, ++n) {
+        const int split = (int)(t / ((int64_t)mt * nt)), kb0 = kb_lo(split), kb1 = kb_lo(split + 1);
+        const uint32_t acc = tmem + (n & 1) * BN;
+        if (!mbar_wait(&acc_empty[n & 1], ((n >> 1) & 1) ^ 1, status)) break;
         tc_fence_after();
-        const uint32_t a = smem_u32(sA + s * A_BYTES), b = smem_u32(sB + s * B_BYTES);
+        for (int kb = kb0; kb < kb1; ++kb, ++i) {
+          const int s = (int)(i % STAGES);
+          if (!mbar_wait(&full[s], (i / STAGES) & 1, status)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = smem_u32(smem + s * 2 * OP_BYTES), b = a + OP_BYTES;
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-          const uint64_t da = A_MN ? sw128_desc_mn(a + kk * 2048, 8192, 1024) : sw128_desc(a) + 2 * kk;
-          const uint64_t db = B_MN ? sw128_desc_mn(b + kk * 2048, 8192, 1024) : sw128_desc(b) + 2 * kk;
-          umma_f16(tmem, da, db, idesc, (i | kk) != 0);
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            const uint64_t da = A_MN ? sw128_desc_mn(a + kk * 2048, 8192, 1024) : sw128_desc(a) + 2 * kk;
+            const uint64_t db = B_MN ? sw128_desc_mn(b + kk * 2048, 8192, 1024) : sw128_desc(b) + 2 * kk;
+            umma_f16_pair(acc, da, db, idesc, kb > kb0 || kk > 0);
+          }
+          umma_commit_pair(&empty[s]);
         }
-        umma_commit(&empty[s]);
+        umma_commit_pair(&acc_full[n & 1]);
       }
-      umma_commit(done);
     }
   } else {
-    const int quad = warp & 3;
-    const bool ok = mbar_wait(done, 0, status);
-    tc_fence_after();
-    const int64_t row = m0 + quad * 32 + lane;
-    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
-#pragma unroll 1
-    for (int c = 0; c < TN_COLS; c += 32) {
-      float v[32];
-      tmem_ld32(taddr + c, v);
-      float w[EPI == DUAL ? 32 : 1];
-      if constexpr (EPI == DUAL) tmem_ld32(taddr + 128 + c, w);
-      tmem_ld_wait();
-      const int col0 = n0 + c;
-      if (!ok || row >= g.M || col0 >= g.N) continue;
-      if (num_kb == 0) {  // an empty split-K slice contributes zeros
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+    uint8_t* buf0 = smem + S::EPI_OFF + ew * S::EPI_BYTES;
+    uint8_t* buf1 = buf0 + 4096;
+    const uint32_t drained[2] = {cluster_addr(&acc_empty[0], 0), cluster_addr(&acc_empty[1], 0)};
+    constexpr int HALF = TN_COLS / 2;                          // result columns of a warp
+    constexpr int CW = EPI == STORE || EPI == DUAL ? 64 : 32;  // result columns of a chunk
+    constexpr int CH = HALF / CW;
+    auto row_of = [&](const Tile& tl) { return tl.m0 + rank * 128 + quad * 32; };
+    auto live = [&](const Tile& tl, int c) { return row_of(tl) < g.M && tl.n0 + half * HALF + c * CW < g.N; };
+    // the epilogue's own loads run one chunk ahead: the residual (STORE) or g and u (DACT)
+    const bool loads = EPI == DACT || (EPI == STORE && g.flag);
+    int nis = 0;  // loads issued (lane 0)
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) {  // one answer for the warp
+      return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+    };
+    auto load = [&](int64_t t, int c) {  // chunk c of tile t, or the next tile's first; lane 0
+      if (c == CH) {
+        t += step;
+        c = 0;
       }
-      if constexpr (EPI == PARTIAL) {
-        float* o = g.f32 + ((int64_t)blockIdx.z * g.M + row) * g.N + col0;
-#pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          if (col0 + j < g.N) *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-      } else if constexpr (EPI == DUAL) {
-        if (g.f32) {
-          float* o = g.f32 + row * 2 * g.F + col0;
-#pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            if (col0 + j < g.N) {
-              *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-              *reinterpret_cast<float4*>(o + g.F + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-            }
+      if (t >= tiles) return;
+      const Tile tl = tile_at(t, mt, nt, TN_COLS);
+      if (!live(tl, c)) return;
+      ++nis;
+      const int col = tl.n0 + half * HALF + c * CW, row = (int)row_of(tl);
+      if constexpr (EPI == DACT) {
+        mbar_arrive_expect_tx(&ld_bar[ew], 8192);
+        tma_load_2d(buf0, &maps.in0, &ld_bar[ew], col, row);
+        tma_load_2d(buf1, &maps.in1, &ld_bar[ew], col, row);
+      } else {
+        mbar_arrive_expect_tx(&ld_bar[ew], 4096);
+        tma_load_2d(buf1, &maps.in0, &ld_bar[ew], col, row);
+      }
+    };
+    if (loads && lane == 0) load(t0, 0);
+    int n = 0, nld = 0, nst = 0;  // tiles, loads waited for, stores
+    bool ok = true;
+    for (int64_t t = t0; t < tiles && ok; t += step, ++n) {
+      const Tile tl = tile_at(t, mt, nt, TN_COLS);
+      const int row = (int)row_of(tl), col_h = tl.n0 + half * HALF;
+      ok = wait_all(&acc_full[n & 1], (n >> 1) & 1);
+      tc_fence_after();
+      const uint32_t acc = tmem + (n & 1) * BN + ((uint32_t)(quad * 32) << 16);
+      for (int c = 0; c < CH && ok; ++c) {
+        if (!live(tl, c)) {
+          // outside the result: the next tile's first load, which the last chunk starts, still has to run ahead
+          if (loads && lane == 0 && c == CH - 1) load(t, CH);
+          continue;
         }
+        const int col = col_h + c * CW;
+        if constexpr (EPI == STORE) {
+          float v[64];
+          tmem_ld32(acc + half * HALF + c * CW, v);
+          tmem_ld32(acc + half * HALF + c * CW + 32, v + 32);
+          tmem_ld_wait();
+          if (g.flag) {
+            ok = wait_all(&ld_bar[ew], nld++ & 1);
+            uint32_t r[32];
+            get_row(buf1, lane, r);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = act_only(v[j], g.act) * w[j];
-      } else if constexpr (EPI == DACT) {
-        const float* gp = g.f32 + row * 2 * g.F + col0;
-        uint16_t* o = reinterpret_cast<uint16_t*>(g.out) + row * 2 * g.F + col0;
+            for (int j = 0; j < 32; ++j) {
+              const float2 f = unpack2<F16>(r[j]);
+              v[2 * j] += f.x;
+              v[2 * j + 1] += f.y;
+            }
+          }
+          uint32_t w[32];
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          if (col0 + j >= g.N) break;
-          uint32_t dg[4], du[4];
+          for (int j = 0; j < 32; ++j) w[j] = pack2<F16>(v[2 * j], v[2 * j + 1]);
+          uint8_t* buf = g.flag || (nst & 1) == 0 ? buf0 : buf1;
+          if (lane == 0) {
+            if (g.flag) bulk_wait_read<0>();
+            else bulk_wait_read<1>();
+          }
+          __syncwarp();
+          put_row(buf, lane, w);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (ok) tma_store_2d(&maps.out, buf, col, row);
+            bulk_commit();
+            if (g.flag) load(t, c + 1);
+          }
+          ++nst;
+        } else if constexpr (EPI == PARTIAL) {
+          float v[32];
+          tmem_ld32(acc + half * HALF + c * CW, v);
+          tmem_ld_wait();
+          uint8_t* buf = (nst & 1) == 0 ? buf0 : buf1;
+          if (lane == 0) bulk_wait_read<1>();
+          __syncwarp();
+          put_row(buf, lane, reinterpret_cast<const uint32_t*>(v));
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&maps.out, buf, col, tl.split * mt * BM + row);
+            bulk_commit();
+          }
+          ++nst;
+        } else if constexpr (EPI == DUAL) {
+          uint32_t h[32];
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const float2 gv = *reinterpret_cast<const float2*>(gp + j + 2 * t);
-            const float2 uv = *reinterpret_cast<const float2*>(gp + g.F + j + 2 * t);
+          for (int q = 0; q < 2; ++q) {
+            float v[32], w[32];
+            tmem_ld32(acc + half * HALF + q * 32, v);
+            tmem_ld32(acc + BN / 2 + half * HALF + q * 32, w);
+            tmem_ld_wait();
+            if (g.flag && col + q * 32 < g.N) {
+              if (lane == 0) bulk_wait_read<0>();
+              __syncwarp();
+              put_row(buf0, lane, reinterpret_cast<const uint32_t*>(v));
+              put_row(buf1, lane, reinterpret_cast<const uint32_t*>(w));
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                tma_store_2d(&maps.gate, buf0, col + q * 32, row);
+                tma_store_2d(&maps.up, buf1, col + q * 32, row);
+                bulk_commit();
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              h[q * 16 + j] = pack2<F16>(act_only(v[2 * j], g.act) * w[2 * j], act_only(v[2 * j + 1], g.act) * w[2 * j + 1]);
+          }
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+          put_row(buf0, lane, h);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&maps.out, buf0, col, row);
+            bulk_commit();
+          }
+        } else {  // DACT
+          float v[32];
+          tmem_ld32(acc + half * HALF + c * CW, v);
+          ok = wait_all(&ld_bar[ew], nld++ & 1);
+          uint32_t gr[32], ur[32];
+          get_row(buf0, lane, gr);
+          get_row(buf1, lane, ur);
+          tmem_ld_wait();
+          __syncwarp();  // both buffers have been read: the next chunk may land
+          if (lane == 0) {
+            load(t, c + 1);
+            bulk_wait_read<0>();
+          }
+          uint32_t dg[16], du[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
             float a0, d0, a1, d1;
-            act_grad(gv.x, g.act, a0, d0);
-            act_grad(gv.y, g.act, a1, d1);
-            dg[t] = pack2<F16>(v[j + 2 * t] * uv.x * d0, v[j + 2 * t + 1] * uv.y * d1);
-            du[t] = pack2<F16>(v[j + 2 * t] * a0, v[j + 2 * t + 1] * a1);
+            act_grad(__uint_as_float(gr[2 * j]), g.act, a0, d0);
+            act_grad(__uint_as_float(gr[2 * j + 1]), g.act, a1, d1);
+            dg[j] = pack2<F16>(v[2 * j] * __uint_as_float(ur[2 * j]) * d0,
+                               v[2 * j + 1] * __uint_as_float(ur[2 * j + 1]) * d1);
+            du[j] = pack2<F16>(v[2 * j] * a0, v[2 * j + 1] * a1);
           }
-          *reinterpret_cast<uint4*>(o + j) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
-          *reinterpret_cast<uint4*>(o + g.F + j) = make_uint4(du[0], du[1], du[2], du[3]);
-        }
-      }
-      if constexpr (EPI == STORE || EPI == DUAL) {
-        if (EPI == STORE && g.residual) {
-          const uint16_t* r = reinterpret_cast<const uint16_t*>(g.residual) + row * g.ldr + col0;
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            if (col0 + j >= g.N) break;
-            const uint4 q = *reinterpret_cast<const uint4*>(r + j);
-            const uint32_t qq[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const float2 f = unpack2<F16>(qq[t]);
-              v[j + 2 * t] += f.x;
-              v[j + 2 * t + 1] += f.y;
+          __syncwarp();
+          put_half_row(buf0 + 8192, lane, dg);
+          put_half_row(buf0 + 10240, lane, du);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (ok) {
+              tma_store_2d(&maps.out, buf0 + 8192, col, row);
+              tma_store_2d(&maps.out2, buf0 + 10240, col, row);
             }
+            bulk_commit();
           }
         }
-        uint16_t* o = reinterpret_cast<uint16_t*>(g.out) + row * g.ldo + col0;
-#pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          if (col0 + j >= g.N) break;
-          *reinterpret_cast<uint4*>(o + j) =
-              make_uint4(pack2<F16>(v[j], v[j + 1]), pack2<F16>(v[j + 2], v[j + 3]), pack2<F16>(v[j + 4], v[j + 5]),
-                         pack2<F16>(v[j + 6], v[j + 7]));
-        }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(drained[n & 1]);
+    }
+    if (lane == 0) {
+      if (nis > nld) mbar_wait(&ld_bar[ew], nld & 1, status);  // after a failed wait: the copy in flight lands first
+      bulk_wait<0>();
     }
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   if (warp == 1) {
-    __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, BN);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
-// Fixed-order sum of the split-K partials [splits, M, N] -> out
+// Fixed-order sum of the split-K partials [splits, rows, N] -> out [M, N]
 template <bool F16>
-__global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ part, int splits, int64_t M, int N,
-                                                         void* __restrict__ out, int64_t ldo) {
+__global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ part, int splits, int64_t rows,
+                                                         int64_t M, int N, void* __restrict__ out) {
   grid_dep_wait();
-  const int64_t total = M * N, idx = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
-  if (idx >= total) return;
+  grid_dep_trigger();
+  const int64_t idx = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+  if (idx >= M * N) return;
   float v[8] = {};
   for (int s = 0; s < splits; ++s) {
-    const float4 a = *reinterpret_cast<const float4*>(part + s * total + idx);
-    const float4 b = *reinterpret_cast<const float4*>(part + s * total + idx + 4);
+    const float4 a = *reinterpret_cast<const float4*>(part + s * rows * N + idx);
+    const float4 b = *reinterpret_cast<const float4*>(part + s * rows * N + idx + 4);
     v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
     v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
   }
-  const int64_t row = idx / N;
-  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + row * ldo + idx % N) =
+  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + idx) =
       make_uint4(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7]));
 }
 
-// splits of a result with few tiles (the weight gradients: K is the row count): as many as fill the SMs once, each
-// of at least 16 K blocks
+// K splits of a product: those that minimise waves of tiles x K blocks of a tile (0.28 us each at the full rate), plus
+// the fp32 partials written and read again (about 4 TB/s through L2) and the second launch (3 us)
 static int plan_splits(int64_t M, int N, int64_t K, int num_sms) {
-  const int64_t tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN), kb = (K + BK - 1) / BK;
-  if (tiles < 1 || tiles * 2 > num_sms) return 1;
-  return (int)max((int64_t)1, min((int64_t)(num_sms / tiles), kb / 16));
+  const int64_t tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN), kb = (K + BK - 1) / BK, pairs = num_sms / 2;
+  if (tiles < 1 || tiles >= pairs) return 1;
+  int best = 1;
+  double cost = 1e300;
+  for (int s = 1; s <= 32 && s * 4 <= std::max<int64_t>(kb, 4); ++s) {
+    const double waves = (double)((tiles * s + pairs - 1) / pairs);
+    const double c = waves * (double)((kb + s - 1) / s) * 0.28 +
+                     (s > 1 ? 3. + 8. * s * (double)M * N / 4e6 : 0.);
+    if (c < cost * 0.98) best = s, cost = c;
+  }
+  return best;
 }
 
+struct Ptr {  // a row-major matrix
+  const void* p;
+  int64_t ld;
+};
+
 template <int LAYOUT, int EPI, bool F16>
-static int launch(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t b_rows, int splits, const Args& g,
-                  uint32_t* status, cudaStream_t st) {
+static int launch(Ptr A, Ptr B, int64_t b_rows, Maps& maps, const Args& g, int num_sms, uint32_t* status,
+                  cudaStream_t st) {
   constexpr bool A_MN = LAYOUT == TN, B_MN = LAYOUT != NT;
-  CUtensorMap ta, tb;
-  int rc = A_MN ? make_tmap_2d(&ta, A, 2, g.M, g.K, lda * 2, 64, BK, 1)
-                : make_tmap_2d(&ta, A, 2, g.K, g.M, lda * 2, BK, BM, 1);
+  int rc = A_MN ? make_tmap_2d(&maps.a, A.p, 2, g.M, g.K, A.ld * 2, 64, BK, 1)
+                : make_tmap_2d(&maps.a, A.p, 2, g.K, g.M, A.ld * 2, BK, 128, 1);
   if (rc) return 1000 + rc;
-  rc = B_MN ? make_tmap_2d(&tb, B, 2, b_rows, g.K, ldb * 2, 64, BK, 1)
-            : make_tmap_2d(&tb, B, 2, g.K, b_rows, ldb * 2, BK, 128, 1);
+  rc = B_MN ? make_tmap_2d(&maps.b, B.p, 2, b_rows, g.K, B.ld * 2, 64, BK, 1)
+            : make_tmap_2d(&maps.b, B.p, 2, g.K, b_rows, B.ld * 2, BK, 128, 1);
   if (rc) return 2000 + rc;
   auto kern = ffn_gemm_kernel<LAYOUT, EPI, F16>;
   static std::atomic<uint64_t> devs{0};
-  if (const int e = smem_attr_once(devs, (const void*)kern, SMEM)) return e;
+  if (const int e = smem_attr_once(devs, (const void*)kern, Smem<EPI>::TOTAL)) return e;
   constexpr int cols = EPI == DUAL ? BN / 2 : BN;
-  const dim3 grid((unsigned)((g.M + BM - 1) / BM), (g.N + cols - 1) / cols, splits);
-  return launch_pdl(kern, grid, dim3(192), SMEM, st, ta, tb, g, status);
+  const int64_t tiles = ((g.M + BM - 1) / BM) * ((g.N + cols - 1) / cols) * g.splits;
+  const int pairs = (int)std::min<int64_t>(tiles, std::max(1, num_sms / 2));
+  return launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), Smem<EPI>::TOTAL, st, maps, g, status);
 }
 
-// C [M, N] = A B in LAYOUT, rounded to the element type, split over K where that pays
+// map of a result or epilogue input: boxes of 32 rows x 128 (or 64) bytes
+static int row_map(CUtensorMap* m, const void* p, int bytes, int64_t cols, int64_t rows, int64_t ld, int row_bytes) {
+  return make_tmap_2d(m, p, bytes, cols, rows, ld * bytes, row_bytes / bytes, 32, row_bytes);
+}
+
+// out [M, N] = A B in LAYOUT (+ residual), rounded to the element type, split over K where that pays
 template <int LAYOUT, bool F16>
-static int product(const void* A, int64_t lda, const void* B, int64_t ldb, Args g, float* scratch, int num_sms,
+static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr residual, float* scratch, int num_sms,
                    uint32_t* status, cudaStream_t st) {
-  const int splits = g.residual ? 1 : plan_splits(g.M, g.N, g.K, num_sms);
-  if (splits == 1) return launch<LAYOUT, STORE, F16>(A, lda, B, ldb, g.N, 1, g, status, st);
-  g.f32 = scratch;
-  int rc = launch<LAYOUT, PARTIAL, F16>(A, lda, B, ldb, g.N, splits, g, status, st);
+  Maps maps;
+  Args g;
+  g.M = M, g.N = N, g.K = K;
+  g.splits = residual.p ? 1 : plan_splits(M, N, K, num_sms);
+  int rc;
+  if (g.splits == 1) {
+    if ((rc = row_map(&maps.out, out, 2, N, M, N, 128))) return 3000 + rc;
+    g.flag = residual.p != nullptr;
+    if (g.flag && (rc = row_map(&maps.in0, residual.p, 2, N, M, residual.ld, 128))) return 3100 + rc;
+    return launch<LAYOUT, STORE, F16>(A, B, N, maps, g, num_sms, status, st);
+  }
+  const int64_t rows = (M + BM - 1) / BM * BM;  // of a split's partial sums: whole tiles
+  if ((rc = row_map(&maps.out, scratch, 4, N, rows * g.splits, N, 128))) return 3200 + rc;
+  rc = launch<LAYOUT, PARTIAL, F16>(A, B, N, maps, g, num_sms, status, st);
   if (rc) return rc;
-  const int64_t n8 = g.M * g.N / 8;
-  return launch_pdl(ffn_reduce_kernel<F16>, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, st,
-                    (const float*)scratch, splits, g.M, g.N, g.out, g.ldo);
+  return launch_pdl(ffn_reduce_kernel<F16>, dim3((unsigned)((M * N / 8 + 255) / 256)), dim3(256), 0, st,
+                    (const float*)scratch, g.splits, rows, M, N, out);
 }
 
 static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {
   const int s = plan_splits(M, N, K, num_sms);
-  return s > 1 ? (size_t)s * M * N : 0;
+  return s > 1 ? (size_t)s * ((M + BM - 1) / BM * BM) * N : 0;
 }
 
 template <bool F16>
-static int fwd(const FfnShape& s, const void* x, int64_t ldx, const void* w13, const void* w2, const void* residual,
-               int64_t ldr, void* h, float* gu, void* y, float* scratch, int num_sms, uint32_t* status,
-               cudaStream_t st) {
+static int fwd(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, float* scratch,
+               int num_sms, uint32_t* status, cudaStream_t st) {
+  Maps maps;
   Args g;
-  g.M = s.T, g.N = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.out = h, g.ldo = s.F, g.f32 = gu;
-  int rc = launch<NT, DUAL, F16>(x, ldx, w13, s.H, 2 * s.F, 1, g, status, st);
+  g.M = s.T, g.N = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.flag = gu != nullptr;
+  int rc = row_map(&maps.out, h, 2, s.F, s.T, s.F, 128);
+  if (!rc && gu) rc = row_map(&maps.gate, gu, 4, s.F, s.T, 2 * (int64_t)s.F, 128);
+  if (!rc && gu) rc = row_map(&maps.up, gu + s.F, 4, s.F, s.T, 2 * (int64_t)s.F, 128);
+  if (rc) return 4000 + rc;
+  rc = launch<NT, DUAL, F16>(x, w13, 2 * (int64_t)s.F, maps, g, num_sms, status, st);
   if (rc) return rc;
-  g = Args();
-  g.M = s.T, g.N = s.N, g.K = s.F, g.out = y, g.ldo = s.N, g.residual = residual, g.ldr = ldr;
-  return product<NT, F16>(h, s.F, w2, s.F, g, scratch, num_sms, status, st);
+  return product<NT, F16>({h, s.F}, w2, s.T, s.N, s.F, y, residual, scratch, num_sms, status, st);
 }
 
 template <bool F16>
-static int bwd(const FfnShape& s, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w13,
-               const void* w2, const void* h, const float* gu, void* dgu, void* dx, void* dw13, void* dw2,
-               float* scratch, int num_sms, uint32_t* status, cudaStream_t st) {
+static int bwd(const FfnShape& s, Ptr dy, Ptr x, Ptr w13, Ptr w2, const void* h, const float* gu, void* dgu, void* dx,
+               void* dw13, void* dw2, float* scratch, int num_sms, uint32_t* status, cudaStream_t st) {
+  const Ptr none{nullptr, 0}, d{dgu, 2 * (int64_t)s.F};
   int rc = 0;
-  Args g;
-  if (dw2) {
-    g.M = s.N, g.N = s.F, g.K = s.T, g.out = dw2, g.ldo = s.F;
-    if ((rc = product<TN, F16>(dy, lddy, h, s.F, g, scratch, num_sms, status, st))) return rc;
-  }
+  if (dw2 && (rc = product<TN, F16>(dy, {h, s.F}, s.N, s.F, s.T, dw2, none, scratch, num_sms, status, st))) return rc;
   if (!dx && !dw13) return 0;
-  g = Args();
-  g.M = s.T, g.N = s.F, g.K = s.N, g.F = s.F, g.act = s.act, g.out = dgu, g.f32 = const_cast<float*>(gu);
-  if ((rc = launch<NN, DACT, F16>(dy, lddy, w2, s.F, s.F, 1, g, status, st))) return rc;
-  if (dx) {
-    g = Args();
-    g.M = s.T, g.N = s.H, g.K = 2 * s.F, g.out = dx, g.ldo = s.H;
-    if ((rc = product<NN, F16>(dgu, 2 * s.F, w13, s.H, g, scratch, num_sms, status, st))) return rc;
-  }
-  if (dw13) {
-    g = Args();
-    g.M = 2 * s.F, g.N = s.H, g.K = s.T, g.out = dw13, g.ldo = s.H;
-    if ((rc = product<TN, F16>(dgu, 2 * s.F, x, ldx, g, scratch, num_sms, status, st))) return rc;
-  }
-  return 0;
+  Maps maps;
+  Args g;
+  g.M = s.T, g.N = s.F, g.K = s.N, g.act = s.act;
+  uint16_t* o = reinterpret_cast<uint16_t*>(dgu);
+  rc = row_map(&maps.in0, gu, 4, s.F, s.T, d.ld, 128);
+  if (!rc) rc = row_map(&maps.in1, gu + s.F, 4, s.F, s.T, d.ld, 128);
+  if (!rc) rc = row_map(&maps.out, o, 2, s.F, s.T, d.ld, 64);
+  if (!rc) rc = row_map(&maps.out2, o + s.F, 2, s.F, s.T, d.ld, 64);
+  if (rc) return 4100 + rc;
+  if ((rc = launch<NN, DACT, F16>(dy, w2, s.F, maps, g, num_sms, status, st))) return rc;
+  if (dx && (rc = product<NN, F16>(d, w13, s.T, s.H, 2 * (int64_t)s.F, dx, none, scratch, num_sms, status, st)))
+    return rc;
+  if (dw13) rc = product<TN, F16>(d, x, 2 * (int64_t)s.F, s.H, s.T, dw13, none, scratch, num_sms, status, st);
+  return rc;
 }
 
 static bool valid(const FfnShape& s) {
@@ -380,8 +589,8 @@ int ffn_fwd(const FfnShape& s, const void* x, int64_t ldx, const void* w13, cons
             int64_t ldr, void* h, float* gu, void* y, float* scratch, int num_sms, uint32_t* status, cudaStream_t st) {
   if (!ffn::valid(s)) return 3;
   if (s.T == 0) return 0;
-  return (s.fp16 ? ffn::fwd<true> : ffn::fwd<false>)(s, x, ldx, w13, w2, residual, ldr, h, gu, y, scratch, num_sms,
-                                                     status, st);
+  return (s.fp16 ? ffn::fwd<true> : ffn::fwd<false>)(s, {x, ldx}, {w13, s.H}, {w2, s.F}, {residual, ldr}, h, gu, y,
+                                                     scratch, num_sms, status, st);
 }
 
 int ffn_bwd(const FfnShape& s, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w13,
@@ -389,8 +598,8 @@ int ffn_bwd(const FfnShape& s, const void* dy, int64_t lddy, const void* x, int6
             int num_sms, uint32_t* status, cudaStream_t st) {
   if (!ffn::valid(s)) return 3;
   if (s.T == 0) return 0;  // the caller zeroes the weight gradients
-  return (s.fp16 ? ffn::bwd<true> : ffn::bwd<false>)(s, dy, lddy, x, ldx, w13, w2, h, gu, dgu, dx, dw13, dw2, scratch,
-                                                     num_sms, status, st);
+  return (s.fp16 ? ffn::bwd<true> : ffn::bwd<false>)(s, {dy, lddy}, {x, ldx}, {w13, s.H}, {w2, s.F}, h, gu, dgu, dx,
+                                                     dw13, dw2, scratch, num_sms, status, st);
 }
 
 }  // namespace afb

@@ -44,8 +44,9 @@ int gemm_bf16_tn(const void* A, int lda, const void* B, int ldb, int M, int N, i
 int gemm_bf16_grouped(const void* A, int lda, int rows_a, const void* B, int ldb, int rows_b, int N, int K,
                       const GemmEpilogue& epi, const GemmGroups& g, int max_tiles, uint32_t* status,
                       cudaStream_t stream);
+// swizzle: 0 none, 64 the 64-byte pattern, else the 128-byte one
 int make_tmap_2d(CUtensorMap* map, const void* base, int dtype_bytes, uint64_t inner, uint64_t outer,
-                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle128);
+                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle);
 // bf16, 128-byte swizzle: dims / box innermost first, strides of dims 1 and 2 in bytes
 int make_tmap_3d_bf16(CUtensorMap* map, const void* base, const uint64_t dims[3], const uint64_t strides_bytes[2],
                       const uint32_t box[3]);

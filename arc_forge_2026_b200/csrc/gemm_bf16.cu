@@ -276,7 +276,7 @@ static bool ensure_context() {
 }
 
 int make_tmap_2d(CUtensorMap* map, const void* base, int dtype_bytes, uint64_t inner, uint64_t outer,
-                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle128) {
+                 uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle) {
   auto encode = get_encode();
   if (!encode) return -1;
   CUtensorMapDataType dt = dtype_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -288,7 +288,9 @@ int make_tmap_2d(CUtensorMap* map, const void* base, int dtype_bytes, uint64_t i
   cuuint32_t estr[2] = {1, 1};
   auto run = [&] {
     return encode(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                  : swizzle     ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : CU_TENSOR_MAP_SWIZZLE_NONE,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   };
   CUresult r = run();
