@@ -1,5 +1,8 @@
 // Bindings of the gated feed-forward block, the norms with trainable weights and dropout: argument checks,
-// allocation of results and scratch on the tensors' own device, launch on that device's current stream.
+// allocation of results and scratch on the tensors' own device, launch on that device's current stream, and their
+// autograd nodes (in C++: a small call's time is the host's, and a Python node costs several times the kernels).
+#include <torch/csrc/autograd/custom_function.h>
+
 #include "binding_utils.h"
 #include "ffn.h"
 
@@ -8,6 +11,18 @@ using namespace afb_bind;
 namespace {
 
 using OptT = c10::optional<at::Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+bool wants_grad(const OptT& t) { return t.has_value() && wants_grad(*t); }
+at::Tensor val(const OptT& t) { return t.has_value() ? *t : at::Tensor(); }
+OptT opt(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+// x with its leading dimensions as one
+at::Tensor rows2d(const at::Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+void differentiable_once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: create_graph=True is not supported");
+}
 
 int elem_type(const at::Tensor& t, const char* what) {
   switch (t.scalar_type()) {
@@ -217,17 +232,127 @@ at::Tensor dropout_op(const at::Tensor& x_, OptT residual, int64_t threshold, in
   return y;
 }
 
+// ------------------------------------------------------------------------------------------ autograd
+struct GatedFfn : torch::autograd::Function<GatedFfn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2,
+                            const OptT& residual, int64_t act) {
+    const bool need_gu = wants_grad(x) || wants_grad(w13);
+    auto [y, h, gu] = gated_ffn_fwd(rows2d(x), w13, w2, residual ? OptT(rows2d(*residual)) : OptT(), act, need_gu);
+    ctx->save_for_backward({x, w13, w2, wants_grad(w2) ? h : at::Tensor(), val(gu)});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["residual"] = residual.has_value();
+    auto shape = x.sizes().vec();
+    shape.back() = w2.size(0);
+    return y.view(shape);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    differentiable_once("gated_ffn");
+    const variable_list v = ctx->get_saved_variables();
+    const at::Tensor& dy = grads[0];
+    const bool need_x = ctx->needs_input_grad(0), need_w13 = ctx->needs_input_grad(1),
+               need_w2 = ctx->needs_input_grad(2);
+    variable_list out(5);
+    if (need_x || need_w13 || need_w2) {
+      auto [dx, dw13, dw2] = gated_ffn_bwd(rows2d(dy), rows2d(v[0]), v[1], v[2], opt(v[3]), opt(v[4]),
+                                           ctx->saved_data["act"].toInt(), need_x, need_w13, need_w2);
+      if (dx) out[0] = dx->view(v[0].sizes());
+      out[1] = val(dw13);
+      out[2] = val(dw2);
+    }
+    if (ctx->saved_data["residual"].toBool()) out[3] = dy;
+    return out;
+  }
+};
+
+at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, const OptT& residual,
+                     int64_t act) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "gated_ffn: x [..., H]");
+  if (residual)
+    TORCH_CHECK(residual->dim() == x.dim() && residual->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+                "gated_ffn: residual has x's leading dimensions");
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w13) || wants_grad(w2) || wants_grad(residual)))
+    return GatedFfn::apply(x, w13, w2, residual, act);
+  const at::Tensor y = std::get<0>(
+      gated_ffn_fwd(rows2d(x), w13, w2, residual ? OptT(rows2d(*residual)) : OptT(), act, false));
+  if (x.dim() == 2) return y;
+  auto shape = x.sizes().vec();
+  shape.back() = w2.size(0);
+  return y.view(shape);
+}
+
+// x [..., width] as rows with unit inner stride
+at::Tensor norm_rows(const at::Tensor& x) {
+  const at::Tensor r = rows2d(x);
+  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+
+struct TrainNorm : torch::autograd::Function<TrainNorm> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const OptT& b, double eps,
+                            bool rms) {
+    const at::Tensor wc = w.contiguous();
+    auto [y, mean, rstd] = norm_train_fwd(norm_rows(x), wc, b ? OptT(b->contiguous()) : OptT(), eps, rms, true);
+    ctx->save_for_backward({x, w, val(mean), val(rstd)});
+    ctx->saved_data["rms"] = rms;
+    ctx->saved_data["bias"] = b.has_value();
+    return y.view(x.sizes());
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    differentiable_once(ctx->saved_data["rms"].toBool() ? "rms_norm" : "layer_norm");
+    const variable_list v = ctx->get_saved_variables();
+    auto [dx, dw, db] = norm_train_bwd(rows2d(grads[0]), norm_rows(v[0]), v[1].contiguous(), opt(v[2]), v[3],
+                                       ctx->saved_data["rms"].toBool(), ctx->needs_input_grad(0),
+                                       ctx->needs_input_grad(1),
+                                       ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2));
+    variable_list out(5);
+    if (dx) out[0] = dx->view(v[0].sizes());
+    out[1] = val(dw);
+    out[2] = val(db);
+    return out;
+  }
+};
+
+at::Tensor train_norm(const at::Tensor& x, const at::Tensor& w, const OptT& b, double eps, bool rms) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "norm: x [..., width]");
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
+    return TrainNorm::apply(x, w, b, eps, rms);
+  const at::Tensor y = std::get<0>(norm_train_fwd(norm_rows(x), w.contiguous(), b ? OptT(b->contiguous()) : OptT(), eps,
+                                                  rms, false));
+  return x.dim() == 2 ? y : y.view(x.sizes());
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptT& residual, const OptT& rng,
+                            int64_t threshold, int64_t seed, int64_t offset) {
+    ctx->save_for_backward({val(rng)});
+    ctx->saved_data["threshold"] = threshold;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["residual"] = residual.has_value();
+    return dropout_op(x, residual, threshold, seed, offset, rng);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    differentiable_once("dropout");
+    variable_list out(6);
+    if (ctx->needs_input_grad(0))
+      out[0] = dropout_op(grads[0], OptT(), ctx->saved_data["threshold"].toInt(), ctx->saved_data["seed"].toInt(),
+                          ctx->saved_data["offset"].toInt(), opt(ctx->get_saved_variables()[0]));
+    if (ctx->saved_data["residual"].toBool()) out[1] = grads[0];
+    return out;
+  }
+};
+
+at::Tensor dropout(const at::Tensor& x, const OptT& residual, int64_t threshold, int64_t seed, int64_t offset,
+                   const OptT& rng) {
+  if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(residual)))
+    return Dropout::apply(x, residual, rng, threshold, seed, offset);
+  return dropout_op(x, residual, threshold, seed, offset, rng);
+}
+
 }  // namespace
 
 void register_ffn(pybind11::module& m) {
-  m.def("gated_ffn_fwd", &gated_ffn_fwd, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("residual"),
-        py::arg("act"), py::arg("save"));
-  m.def("gated_ffn_bwd", &gated_ffn_bwd, py::arg("dy"), py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("h"),
-        py::arg("gu"), py::arg("act"), py::arg("need_dx"), py::arg("need_dw13"), py::arg("need_dw2"));
-  m.def("norm_train_fwd", &norm_train_fwd, py::arg("x"), py::arg("w"), py::arg("b"), py::arg("eps"), py::arg("rms"),
-        py::arg("save"));
-  m.def("norm_train_bwd", &norm_train_bwd, py::arg("dy"), py::arg("x"), py::arg("w"), py::arg("mean"),
-        py::arg("rstd"), py::arg("rms"), py::arg("need_dx"), py::arg("need_dw"), py::arg("need_db"));
-  m.def("dropout", &dropout_op, py::arg("x"), py::arg("residual"), py::arg("threshold"), py::arg("seed"),
+  m.def("gated_ffn", &gated_ffn, py::arg("x"), py::arg("w13"), py::arg("w2"), py::arg("residual"), py::arg("act"));
+  m.def("train_norm", &train_norm, py::arg("x"), py::arg("w"), py::arg("b"), py::arg("eps"), py::arg("rms"));
+  m.def("dropout", &dropout, py::arg("x"), py::arg("residual"), py::arg("threshold"), py::arg("seed"),
         py::arg("offset"), py::arg("rng"));
 }

@@ -19,7 +19,6 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 ACTS = {"silu": 0, "gelu_tanh": 1, "gelu": 2}
 
@@ -41,26 +40,6 @@ def gated_ffn_reference(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, ac
     if residual is not None:
         y = y + residual.to(ct)
     return y.to(x.dtype)
-
-
-class _GatedFFN(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w13, w2, residual, act):
-        need_x, need_w13, need_w2 = ctx.needs_input_grad[:3]
-        y, h, gu = _ext().gated_ffn_fwd(x, w13, w2, residual, act, need_x or need_w13)
-        ctx.save_for_backward(x, w13, w2, h if need_w2 else None, gu)
-        ctx.act = act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w13, w2, h, gu = ctx.saved_tensors
-        need_x, need_w13, need_w2, need_r, _ = ctx.needs_input_grad
-        dx = dw13 = dw2 = None
-        if need_x or need_w13 or need_w2:
-            dx, dw13, dw2 = _ext().gated_ffn_bwd(dy, x, w13, w2, h, gu, ctx.act, need_x, need_w13, need_w2)
-        return dx, dw13, dw2, dy if need_r else None, None
 
 
 def native_ok(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> bool:
@@ -89,11 +68,4 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, act: str = "
         raise ValueError(f"gated_ffn: residual {tuple(residual.shape)}, result {out_shape}")
     if not native_ok(x, w13, w2):
         return gated_ffn_reference(x, w13, w2, act, residual)
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    r2 = residual if residual is None or residual.dim() == 2 else residual.reshape(-1, w2.shape[0])
-    if torch.is_grad_enabled() and (x.requires_grad or w13.requires_grad or w2.requires_grad
-                                    or (r2 is not None and r2.requires_grad)):
-        y = _GatedFFN.apply(x2, w13, w2, r2, ACTS[act])
-    else:
-        y = _ext().gated_ffn_fwd(x2, w13, w2, r2, ACTS[act], False)[0]
-    return y if x.dim() == 2 else y.view(out_shape)
+    return _ext().gated_ffn(x, w13, w2, residual, ACTS[act])

@@ -103,26 +103,6 @@ def _norm_ok(x, w) -> bool:
     return _gpu_bf16(x) and x.shape[-1] in _NORM_H and x.dim() >= 2 and not w.requires_grad
 
 
-class _TrainNorm(torch.autograd.Function):
-    """LayerNorm / zero-centred RMSNorm with gradients of x, w and b (``csrc/norm_train.cu``); x [rows, width]."""
-
-    @staticmethod
-    def forward(ctx, x, w, b, eps, rms):
-        save = any(ctx.needs_input_grad[:3])
-        y, mean, rstd = _ext().norm_train_fwd(x, w, b, eps, rms, save)
-        ctx.save_for_backward(x, w, mean, rstd)
-        ctx.rms = rms
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx, dw, db = _ext().norm_train_bwd(dy, x, w, mean, rstd, ctx.rms, need_x, need_w, need_b)
-        return dx, dw, db, None, None
-
-
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 _NORM_MAX_WIDTH = 16384
 
@@ -130,19 +110,6 @@ _NORM_MAX_WIDTH = 16384
 def _train_norm_ok(x, w) -> bool:
     return (x.is_cuda and w.device == x.device and x.dtype in _FLOATS and w.dtype in (x.dtype, torch.float32)
             and 1 <= x.shape[-1] <= _NORM_MAX_WIDTH)
-
-
-def _train_norm(x, w, b, eps, rms):
-    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x2.stride(-1) != 1:
-        x2 = x2.contiguous()
-    w = w.contiguous()
-    b = None if b is None else b.contiguous()
-    if torch.is_grad_enabled() and (x2.requires_grad or w.requires_grad or (b is not None and b.requires_grad)):
-        y = _TrainNorm.apply(x2, w, b, eps, rms)
-    else:
-        y = _ext().norm_train_fwd(x2, w, b, eps, rms, False)[0]
-    return y if x.dim() == 2 else y.view(x.shape)
 
 
 def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
@@ -154,7 +121,7 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
         return _RMSNorm.apply(x, w.float().contiguous(), eps, None)
     if kernels.use("rms_norm") and w.shape == x.shape[-1:] and _train_norm_ok(x, w):
         kernels.hit("rms_norm", True)
-        return _train_norm(x, w, None, eps, True)
+        return _ext().train_norm(x, w, None, eps, True)
     if x.is_cuda:
         kernels.hit("rms_norm", False)
     return R.rms_norm(x, w, eps)
@@ -180,7 +147,7 @@ def layer_norm(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, 
         raise ValueError("layer_norm: w and b on x's device, b in w's type")
     if kernels.use("layer_norm") and _train_norm_ok(x, w):
         kernels.hit("layer_norm", True)
-        return _train_norm(x, w, b, eps, False)
+        return _ext().train_norm(x, w, b, eps, False)
     if x.is_cuda:
         kernels.hit("layer_norm", False)
     return layer_norm_reference(x, w, b, eps)
@@ -228,26 +195,18 @@ def _dropout_plain(x, residual, p, seed, offset, rng):
     return (y if residual is None else y + residual.to(ct)).to(x.dtype)
 
 
-def _dropout_any(x, residual, p, seed, offset, rng, native):
-    if native:
-        return _ext().dropout(x, residual, dropout_threshold(p), _i64(seed), _i64(offset), rng)
-    return _dropout_plain(x, residual, p, seed, offset, rng)
-
-
-class _Dropout(torch.autograd.Function):
+class _DropoutPlain(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, p, seed, offset, rng, native):
+    def forward(ctx, x, residual, p, seed, offset, rng):
         ctx.save_for_backward(rng)
-        ctx.args = (p, seed, offset, native)
-        return _dropout_any(x, residual, p, seed, offset, rng, native)
+        ctx.args = (p, seed, offset)
+        return _dropout_plain(x, residual, p, seed, offset, rng)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (rng,) = ctx.saved_tensors
-        p, seed, offset, native = ctx.args
-        dx = _dropout_any(dy, None, p, seed, offset, rng, native) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
+        dx = _dropout_plain(dy, None, *ctx.args, *ctx.saved_tensors) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -275,9 +234,9 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
     native = x.is_cuda and x.dtype in _FLOATS and kernels.use("dropout")
     if x.is_cuda:
         kernels.hit("dropout", native)
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _Dropout.apply(x, residual, float(p), int(seed), int(offset), rng, native)
-    return _dropout_any(x, residual, float(p), int(seed), int(offset), rng, native)
+    if native:
+        return _ext().dropout(x, residual, dropout_threshold(p), _i64(int(seed)), _i64(int(offset)), rng)
+    return _DropoutPlain.apply(x, residual, float(p), int(seed), int(offset), rng)
 
 
 def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:

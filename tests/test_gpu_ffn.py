@@ -487,3 +487,55 @@ def test_lora_dropout_on_the_native_products():
     dx2, dA2, dB2 = torch.autograd.grad(y2.square().sum(), [xd, ad.A, ad.B])
     assert torch.equal(y, y2) and torch.equal(dA, dA2) and torch.equal(dB, dB2)
     assert torch.equal(dx, fused.dropout(dx2, 0.2, 9, 3 << 36))
+
+
+def test_checkpointed_student_layer_and_second_derivatives():
+    """Activation checkpointing recomputes the same values (dropout masks among them) through the C++ autograd nodes;
+    create_graph is refused instead of giving second derivatives that lack terms."""
+    from arc_forge_2026_b200.config import preset
+    from arc_forge_2026_b200.train import lora
+    from arc_forge_2026_b200.train.student import random_student
+    ids = torch.randint(0, 200, (1, 192), generator=torch.Generator().manual_seed(3)).to(dev)
+
+    def grads(ckpt):
+        st = random_student(preset("tiny_gpu"), dev, seed=0, checkpoint_layers=ckpt)
+        ps = lora.attach_lora(st, 16, 16.0, seed=1, dropout=0.25)
+        with torch.no_grad():
+            for i, p in enumerate(ps):
+                p.add_(torch.randn(p.shape, generator=torch.Generator().manual_seed(i)).to(dev) * 0.05)
+        lora.set_dropout_step(st, 4)
+        return torch.autograd.grad(st.hidden(ids).float().square().sum(), ps)
+    (a, ca), (b, cb) = _with_opt_in(lambda: grads(True)), _with_opt_in(lambda: grads(False))
+    assert ca["native"]["gated_ffn"] > cb["native"]["gated_ffn"] > 0 and ca["native"]["dropout"] > 0
+    for u, v in zip(a, b):
+        assert torch.equal(u, v)
+    x, w13, w2, res, dy = ffn_inputs(8, 16, 8, 16, BF)
+    for f in (lambda t: gated_ffn(t, w13, w2), lambda t: fused.layer_norm(t, w2[0].new_ones(16), None),
+              lambda t: fused.dropout(t, 0.5, 1)):
+        leaf = x.clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(f(leaf).float().sum(), leaf, create_graph=True)
+
+
+def test_gpu_refusals():
+    x, w13, w2, res, dy = ffn_inputs(8, 16, 8, 16, BF)
+    for kw in (dict(act="relu"), dict(w2=w2[:, :4]), dict(w2=w2.float()), dict(w13=w13.cpu()), dict(residual=res[:4]),
+               dict(residual=res.float())):
+        with pytest.raises(ValueError):
+            gated_ffn(**{**dict(x=x, w13=w13, w2=w2), **kw})
+    with pytest.raises(ValueError):
+        fused.layer_norm(x, torch.ones(15, device=dev))
+    with pytest.raises(ValueError):
+        fused.layer_norm(x, torch.ones(16))
+    with pytest.raises(ValueError):
+        fused.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64))
+    # outside what the kernels take: the plain form, counted as such where the registry counts
+    y = gated_ffn(x[:, :12], w13[:, :12], w2)
+    assert y.shape == (8, 16)
+    wide = torch.randn(2, 16392, device=dev)
+    kernels.reset()
+    y = fused.layer_norm(wide, torch.ones(16392, device=dev), None, 1e-6)
+    assert kernels.counts()["fallback"] == {"layer_norm": 1}
+    check(y, *norm_oracle(wide, torch.ones(16392, device=dev), None, wide, 1e-6, False)["y"], "wide")
+    z = torch.randn(4, 16, dtype=torch.float64, device=dev)
+    assert torch.equal(fused.dropout(z, 0.5, 3).cpu(), fused.dropout(z.cpu(), 0.5, 3))
