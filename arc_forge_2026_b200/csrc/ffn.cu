@@ -527,6 +527,242 @@ static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr res
                     (const float*)scratch, g.splits, rows, M, N, out);
 }
 
+// ------------------------------------------------------------------------------------------ few rows
+// Up to FEW rows the weights' bytes are the time. The weights take the M side of the MMA (128 weight rows a CTA, gate
+// and up tiles side by side in TMEM for DUAL) and the rows the N side, padded to NT; the C CTAs of a cluster take a
+// share of K each and add their partial sums through distributed shared memory, so no partial goes through HBM and
+// there is one launch a product. h is kept as two terms (value and rounding error, rows 0.. and T.. of a [2T, F]
+// buffer): the second MMA column block costs nothing here and leaves the result with its own rounding only.
+constexpr int FEW = 128;
+
+template <bool DUAL_, int NT>
+struct Few {
+  static constexpr int NA = DUAL_ ? 2 : 1, NB = DUAL_ ? NT : 2 * NT;  // weight tiles and MMA columns
+  static constexpr uint32_t STAGE = NA * 16384 + NB * 128;
+  static constexpr uint32_t BUDGET = NT <= 32 ? 110592 : 204800;  // two CTAs an SM up to 32 rows
+  static constexpr int STAGES = BUDGET / STAGE;
+  static constexpr uint32_t TOTAL = STAGES * STAGE + (2 * STAGES + 1) * 8 + 16 + 1024;
+  static_assert(STAGES * STAGE >= NA * NT * 512u, "partial sums reuse the ring");
+};
+struct FewArgs {
+  int T = 0, n = 0;  // rows; weight rows (DUAL: F)
+  int K = 0, F = 0, act = 0;
+  void* out = nullptr;             // DUAL: h [2T, F]; else y [T, n]
+  float* gu = nullptr;             // DUAL: [T, 2F] or null
+  const void* residual = nullptr;  // else: [T, n] or null
+  int64_t ldr = 0;
+};
+
+template <bool DUAL_, int NT, bool F16>
+__global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CUtensorMap tm_w,
+                                                      const __grid_constant__ CUtensorMap tm_x, FewArgs g,
+                                                      uint32_t* status) {
+  using S = Few<DUAL_, NT>;
+  constexpr int STAGES = S::STAGES, NB = S::NB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * S::STAGE);
+  uint64_t* empty = full + STAGES;
+  uint64_t* done = empty + STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int C = gridDim.x, rank = blockIdx.x, w0 = blockIdx.y * 128;
+  const int kb_total = (g.K + BK - 1) / BK, kb0 = kb_total * rank / C, num_kb = kb_total * (rank + 1) / C - kb0;
+  constexpr uint32_t TMEM_COLS = 2 * NT;
+
+  // the weights: for DUAL the previous kernel in the stream may have written them (prefetched into L2, which is never
+  // stale); for the down projection it is the DUAL kernel, which waited for everything before it, so they are loaded
+  auto load_w = [&](int i) {
+    uint8_t* a = smem + (i % STAGES) * S::STAGE;
+    uint64_t* bar = &full[i % STAGES];
+    mbar_arrive_expect_tx(bar, S::STAGE);
+    tma_load_2d(a, &tm_w, bar, (kb0 + i) * BK, w0);
+    if constexpr (DUAL_) tma_load_2d(a + 16384, &tm_w, bar, (kb0 + i) * BK, g.F + w0);
+  };
+  auto load_x = [&](int i) {
+    uint8_t* b = smem + (i % STAGES) * S::STAGE + S::NA * 16384;
+    tma_load_2d(b, &tm_x, &full[i % STAGES], (kb0 + i) * BK, 0);
+    if constexpr (!DUAL_) tma_load_2d(b + NT * 128, &tm_x, &full[i % STAGES], (kb0 + i) * BK, g.T);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    if constexpr (DUAL_) {
+      for (int i = 0; i < min(num_kb, STAGES); ++i) {
+        tma_prefetch_l2_2d(&tm_w, (kb0 + i) * BK, w0);
+        tma_prefetch_l2_2d(&tm_w, (kb0 + i) * BK, g.F + w0);
+      }
+    } else {
+      for (int i = 0; i < min(num_kb, STAGES); ++i) load_w(i);
+    }
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dep_wait();
+  if (threadIdx.x == 0) grid_dep_trigger();
+
+  bool ok = true;
+  if (warp == 0) {
+    if (lane == 0) {
+      int issued = 0;
+      for (int i = 0; i < num_kb; ++i) {
+        if (i >= STAGES && !mbar_wait(&empty[i % STAGES], ((i / STAGES) & 1) ^ 1, status)) break;
+        if (DUAL_ || i >= STAGES) load_w(i);
+        load_x(i);
+        ++issued;
+      }
+      for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, status);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_f16(128, NB, F16 ? 0 : 1);
+      for (int i = 0; i < num_kb; ++i) {
+        const int s = i % STAGES;
+        if (!mbar_wait(&full[s], (i / STAGES) & 1, status)) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + s * S::STAGE), b = a + S::NA * 16384;
+#pragma unroll
+        for (int kk = 0; kk < BK / 16; ++kk) {
+          umma_f16(tmem, sw128_desc(a) + 2 * kk, sw128_desc(b) + 2 * kk, idesc, (i | kk) != 0);
+          if constexpr (DUAL_)
+            umma_f16(tmem + NT, sw128_desc(a + 16384) + 2 * kk, sw128_desc(b) + 2 * kk, idesc, (i | kk) != 0);
+        }
+        umma_commit(&empty[s]);
+      }
+      umma_commit(done);
+    }
+  } else {
+    // partial sums to shared memory (the ring is free: every MMA has read it): [NA][T][128]
+    const int quad = warp & 3;
+    ok = mbar_wait(done, 0, status);
+    tc_fence_after();
+    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
+    float* p = reinterpret_cast<float*>(smem) + quad * 32 + lane;
+#pragma unroll 1
+    for (int c = 0; c < NT; c += 16) {
+      if (c >= g.T) break;
+      float v[16], w[16];
+      tmem_ld16(taddr + c, v);
+      tmem_ld16(taddr + NT + c, w);  // DUAL: up; else the second term of h
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (c + j >= g.T) break;
+        if constexpr (DUAL_) {
+          p[(c + j) * 128] = v[j];
+          p[(g.T + c + j) * 128] = w[j];
+        } else {
+          p[(c + j) * 128] = v[j] + w[j];
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync();
+  if (warp >= 2 && ok) {
+    uint32_t part[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) part[c] = cluster_addr(smem, min(c, C - 1));
+    auto sum = [&](uint32_t off) {
+      float2 s = ld_cluster_f2(part[0] + off);
+#pragma unroll
+      for (int c = 1; c < 8; ++c)
+        if (c < C) {
+          const float2 q = ld_cluster_f2(part[c] + off);
+          s.x += q.x;
+          s.y += q.y;
+        }
+      return s;
+    };
+    const int pairs = g.T * 64;  // (row, two weight rows), dealt to the cluster's epilogue threads
+    for (int e = rank * 128 + (threadIdx.x - 64); e < pairs; e += C * 128) {
+      const int t = e >> 6, f = (e & 63) * 2, col = w0 + f;
+      if (col >= g.n) continue;
+      float2 a = sum((t * 128 + f) * 4);
+      if constexpr (DUAL_) {
+        const float2 u = sum(((g.T + t) * 128 + f) * 4);
+        if (g.gu) {
+          *reinterpret_cast<float2*>(g.gu + (int64_t)t * 2 * g.F + col) = a;
+          *reinterpret_cast<float2*>(g.gu + (int64_t)t * 2 * g.F + g.F + col) = u;
+        }
+        a = make_float2(act_only(a.x, g.act) * u.x, act_only(a.y, g.act) * u.y);
+        uint32_t* h = reinterpret_cast<uint32_t*>(g.out);
+        const uint32_t hi = pack2<F16>(a.x, a.y);
+        const float2 r = unpack2<F16>(hi);
+        const int64_t at = ((int64_t)t * g.F + col) >> 1;
+        h[at] = hi;
+        h[at + ((int64_t)g.T * g.F >> 1)] =
+            pack2<F16>(isfinite(r.x) ? a.x - r.x : 0.f, isfinite(r.y) ? a.y - r.y : 0.f);
+      } else {
+        if (g.residual) {
+          const float2 r = unpack2<F16>(*reinterpret_cast<const uint32_t*>(
+              reinterpret_cast<const uint16_t*>(g.residual) + t * g.ldr + col));
+          a.x += r.x;
+          a.y += r.y;
+        }
+        reinterpret_cast<uint32_t*>(g.out)[((int64_t)t * g.n + col) >> 1] = pack2<F16>(a.x, a.y);
+      }
+    }
+  }
+  cluster_sync();  // no CTA leaves while another reads its partial sums
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+template <bool DUAL_, int NT, bool F16>
+static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArgs& g, int num_sms, uint32_t* status,
+                      cudaStream_t st) {
+  using S = Few<DUAL_, NT>;
+  CUtensorMap tw, tx;
+  int rc = make_tmap_2d(&tw, w.p, 2, g.K, w_rows, w.ld * 2, BK, 128, 1);
+  if (!rc) rc = make_tmap_2d(&tx, x.p, 2, g.K, x_rows, x.ld * 2, BK, NT, 1);
+  if (rc) return 5000 + rc;
+  auto kern = ffn_few_kernel<DUAL_, NT, F16>;
+  static std::atomic<uint64_t> devs{0};
+  if (const int e = smem_attr_once(devs, (const void*)kern, S::TOTAL)) return e;
+  // CTAs of a cluster: enough to cover the SMs (twice where two fit), at least two K blocks each
+  const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK, want = num_sms * (NT <= 32 ? 2 : 1);
+  const int C = std::max(1, std::min({8, want / tiles, kb / 2}));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, tiles);
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = S::TOTAL;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)C, 1, 1};
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, g, status);
+  return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+}
+
+template <int NT, bool F16>
+static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, int num_sms,
+                   uint32_t* status, cudaStream_t st) {
+  FewArgs g;
+  g.T = (int)s.T, g.n = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.out = h, g.gu = gu;
+  const int rc = launch_few<true, NT, F16>(w13, 2 * (int64_t)s.F, x, s.T, g, num_sms, status, st);
+  if (rc) return rc;
+  g = FewArgs();
+  g.T = (int)s.T, g.n = s.N, g.K = s.F, g.out = y, g.residual = residual.p, g.ldr = residual.ld;
+  return launch_few<false, NT, F16>(w2, s.N, {h, s.F}, 2 * s.T, g, num_sms, status, st);
+}
+
 static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {
   const int s = plan_splits(M, N, K, num_sms);
   return s > 1 ? (size_t)s * ((M + BM - 1) / BM * BM) * N : 0;
@@ -535,6 +771,10 @@ static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {
 template <bool F16>
 static int fwd(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, float* scratch,
                int num_sms, uint32_t* status, cudaStream_t st) {
+  if (s.T <= FEW) {
+    auto f = s.T <= 16 ? fwd_few<16, F16> : s.T <= 32 ? fwd_few<32, F16> : s.T <= 64 ? fwd_few<64, F16> : fwd_few<128, F16>;
+    return f(s, x, w13, w2, residual, h, gu, y, num_sms, status, st);
+  }
   Maps maps;
   Args g;
   g.M = s.T, g.N = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.flag = gu != nullptr;
@@ -578,8 +818,9 @@ static bool valid(const FfnShape& s) {
 }  // namespace ffn
 
 size_t ffn_fwd_scratch(const FfnShape& s, int num_sms) {
-  return ffn::product_scratch(s.T, s.N, s.F, num_sms);
+  return s.T <= ffn::FEW ? 0 : ffn::product_scratch(s.T, s.N, s.F, num_sms);
 }
+int64_t ffn_h_rows(const FfnShape& s) { return s.T <= ffn::FEW ? 2 * s.T : s.T; }
 size_t ffn_bwd_scratch(const FfnShape& s, int num_sms) {
   return std::max({ffn::product_scratch(s.N, s.F, s.T, num_sms), ffn::product_scratch(s.T, s.H, 2 * s.F, num_sms),
                    ffn::product_scratch(2 * s.F, s.H, s.T, num_sms)});

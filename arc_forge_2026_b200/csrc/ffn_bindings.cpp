@@ -54,8 +54,8 @@ afb::FfnShape ffn_shape(const at::Tensor& x, const at::Tensor& w13, const at::Te
   TORCH_CHECK(x.size(1) > 0 && w2.size(1) > 0 && w2.size(0) > 0 && x.size(1) % 8 == 0 && w2.size(1) % 8 == 0 &&
                   w2.size(0) % 8 == 0,
               "gated_ffn: H, F and N are multiples of 8");
-  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 1024 && x.size(1) < (1 << 24) && w13.size(0) < (1 << 24) &&
-                  w2.size(0) < (1 << 24),
+  TORCH_CHECK(x.size(0) < (int64_t(1) << 31) - 1024 && x.size(1) < (1 << 22) && w13.size(0) < (1 << 22) &&
+                  w2.size(0) < (1 << 22),
               "gated_ffn: size out of range");
   TORCH_CHECK(act >= 0 && act <= 2, "gated_ffn: act is 0 (silu), 1 (tanh-GELU) or 2 (erf-GELU)");
   for (const at::Tensor* t : {&w13, &w2})
@@ -84,12 +84,14 @@ std::tuple<at::Tensor, at::Tensor, OptT> gated_ffn_fwd(const at::Tensor& x_, con
                 "gated_ffn: residual is [T, N] in x's type on its device");
     r = tma_rows(*residual);
   }
-  at::Tensor y = at::empty({s.T, s.N}, x.options()), h = at::empty({s.T, s.F}, x.options());
+  at::Tensor y = at::empty({s.T, s.N}, x.options()), h = at::empty({afb::ffn_h_rows(s), s.F}, x.options());
   OptT gu;
   if (save) gu = at::empty({s.T, 2 * (int64_t)s.F}, x.options().dtype(at::kFloat));
-  const at::Tensor scr = scratch_of(afb::ffn_fwd_scratch(s, num_sms()), x);
+  const size_t n_scr = afb::ffn_fwd_scratch(s, num_sms());
+  const at::Tensor scr = n_scr ? scratch_of(n_scr, x) : at::Tensor();
   check_rc(afb::ffn_fwd(s, x.data_ptr(), ld(x), w13.data_ptr(), w2.data_ptr(), r.defined() ? r.data_ptr() : nullptr,
-                        r.defined() ? ld(r) : 0, h.data_ptr(), optr<float>(gu), y.data_ptr(), ptr<float>(scr), num_sms(), status_ptr(x.get_device()), stream()),
+                        r.defined() ? ld(r) : 0, h.data_ptr(), optr<float>(gu), y.data_ptr(),
+                        n_scr ? ptr<float>(scr) : nullptr, num_sms(), status_ptr(x.get_device()), stream()),
            "gated_ffn_fwd");
   return {y, h, gu};
 }
@@ -104,7 +106,7 @@ std::tuple<OptT, OptT, OptT> gated_ffn_bwd(const at::Tensor& dy_, const at::Tens
               "gated_ffn: dy is [T, N] in x's type on its device");
   if (need_dw2)
     TORCH_CHECK(h.has_value() && h->is_contiguous() && h->scalar_type() == x_.scalar_type() && h->dim() == 2 &&
-                    h->size(0) == s.T && h->size(1) == s.F && h->device() == x_.device(),
+                    h->size(0) >= s.T && h->size(1) == s.F && h->device() == x_.device(),
                 "gated_ffn: h of the forward pass");
   if (need_dx || need_dw13)
     TORCH_CHECK(gu.has_value() && gu->is_contiguous() && gu->scalar_type() == at::kFloat && gu->dim() == 2 &&
@@ -264,12 +266,23 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
   }
 };
 
-at::Tensor gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, const OptT& residual,
-                     int64_t act) {
-  TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "gated_ffn: x [..., H]");
-  if (residual)
-    TORCH_CHECK(residual->dim() == x.dim() && residual->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
-                "gated_ffn: residual has x's leading dimensions");
+// The block, or None where the kernels do not cover the type or the sizes (the caller's plain form does)
+OptT gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, const OptT& residual, int64_t act) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w13.dim() == 2 && w2.dim() == 2 && w13.size(1) == x.size(-1) &&
+                        w13.size(0) == 2 * w2.size(1),
+                    "gated_ffn: x [..., H], w13 [2F, H], w2 [N, F]; got ", x.sizes(), ", ", w13.sizes(), ", ",
+                    w2.sizes());
+  TORCH_CHECK_VALUE(w13.numel() > 0 && w2.numel() > 0, "gated_ffn: empty feature dimension");
+  for (const at::Tensor* t : {&w13, &w2, residual ? &*residual : &w2})
+    TORCH_CHECK_VALUE(t->device() == x.device() && t->scalar_type() == x.scalar_type(),
+                      "gated_ffn: weights and residual have x's type and device");
+  if (residual) {
+    TORCH_CHECK_VALUE(residual->dim() == x.dim() && residual->size(-1) == w2.size(0) &&
+                          residual->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1),
+                      "gated_ffn: residual [..., N] with x's leading dimensions");
+  }
+  const bool half = x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf;
+  if (!x.is_cuda() || !half || x.size(-1) % 8 || w2.size(0) % 8 || w2.size(1) % 8) return OptT();
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w13) || wants_grad(w2) || wants_grad(residual)))
     return GatedFfn::apply(x, w13, w2, residual, act);
   const at::Tensor y = std::get<0>(

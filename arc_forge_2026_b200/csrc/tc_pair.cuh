@@ -1,4 +1,4 @@
-// tcgen05 with cta_group::2 (a pair of CTAs on one MMA tile) and TMA stores.
+// Thread-block clusters, tcgen05 with cta_group::2 (a pair of CTAs on one MMA tile) and TMA stores.
 #pragma once
 #include "common.cuh"
 
@@ -23,6 +23,11 @@ AFB_DEV uint32_t cluster_addr(const void* p, uint32_t rank) {
 }
 AFB_DEV void mbar_arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+AFB_DEV float2 ld_cluster_f2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
 }
 // load into this CTA's shared memory that completes on a barrier of either CTA of the pair
 AFB_DEV void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t cluster_bar, int c0, int c1) {

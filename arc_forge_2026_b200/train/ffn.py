@@ -17,12 +17,15 @@ and the drafter trainer's feed-forward use it when the registry name ``gated_ffn
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn.functional as F
 
 ACTS = {"silu": 0, "gelu_tanh": 1, "gelu": 2}
 
 
+@functools.cache
 def _ext():
     from ..ops import C
     return C()
@@ -47,13 +50,7 @@ def native_ok(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> bool:
             and x.shape[-1] % 8 == 0 and w2.shape[0] % 8 == 0 and w2.shape[1] % 8 == 0)
 
 
-def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, act: str = "silu",
-              residual: torch.Tensor | None = None) -> torch.Tensor:
-    """``(act(g) * u) @ w2.T (+ residual)`` with ``[g | u] = x @ w13.T``; x [..., H], w13 [2F, H] (gate rows, then up
-    rows), w2 [N, F], residual [..., N]; ``act``: ``silu``, ``gelu_tanh`` or ``gelu``. Differentiable (once) in x,
-    w13, w2 and residual."""
-    if act not in ACTS:
-        raise ValueError(f"gated_ffn: unknown act {act!r}; known: {', '.join(ACTS)}")
+def _check(x, w13, w2, residual):
     if w13.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w13.shape[1] != x.shape[-1] \
             or w13.shape[0] != 2 * w2.shape[1]:
         raise ValueError(f"gated_ffn: x [..., H], w13 [2F, H], w2 [N, F]; got {tuple(x.shape)}, {tuple(w13.shape)}, "
@@ -63,9 +60,21 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, act: str = "
     for name, t in (("w13", w13), ("w2", w2), ("residual", residual)):
         if t is not None and (t.device != x.device or t.dtype != x.dtype):
             raise ValueError(f"gated_ffn: {name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
-    out_shape = (*x.shape[:-1], w2.shape[0])
-    if residual is not None and residual.shape != out_shape:
-        raise ValueError(f"gated_ffn: residual {tuple(residual.shape)}, result {out_shape}")
-    if not native_ok(x, w13, w2):
-        return gated_ffn_reference(x, w13, w2, act, residual)
-    return _ext().gated_ffn(x, w13, w2, residual, ACTS[act])
+    if residual is not None and residual.shape != (*x.shape[:-1], w2.shape[0]):
+        raise ValueError(f"gated_ffn: residual {tuple(residual.shape)} does not fit x and w2")
+
+
+def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, act: str = "silu",
+              residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``(act(g) * u) @ w2.T (+ residual)`` with ``[g | u] = x @ w13.T``; x [..., H], w13 [2F, H] (gate rows, then up
+    rows), w2 [N, F], residual [..., N]; ``act``: ``silu``, ``gelu_tanh`` or ``gelu``. Differentiable (once) in x,
+    w13, w2 and residual."""
+    code = ACTS.get(act)
+    if code is None:
+        raise ValueError(f"gated_ffn: unknown act {act!r}; known: {', '.join(ACTS)}")
+    if x.is_cuda:  # the binding checks the arguments and returns None for what the kernels do not cover
+        y = _ext().gated_ffn(x, w13, w2, residual, code)
+        if y is not None:
+            return y
+    _check(x, w13, w2, residual)
+    return gated_ffn_reference(x, w13, w2, act, residual)

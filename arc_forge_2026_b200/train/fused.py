@@ -12,6 +12,8 @@ Beside them, with trainable weights: :func:`layer_norm` and :func:`rms_norm` (``
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
@@ -23,6 +25,7 @@ _BF = torch.bfloat16
 _NORM_H = (128, 256, 512, 1024, 2048)
 
 
+@functools.cache
 def _ext():
     from ..ops import C
     return C()
