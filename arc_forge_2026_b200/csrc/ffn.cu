@@ -31,32 +31,34 @@ constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
 enum Epi { STORE = 0, PARTIAL = 1, DUAL = 2, DACT = 3 };
 enum Layout { NT = 0, NN = 1, TN = 2 };  // A K-major B K-major | A K-major B MN-major | both MN-major
 
-template <int EPI>
-struct Smem {
-  // epilogue staging of a warp: two 4 KB buffers (a 32-row box of 128-byte rows each); DACT two more of 2 KB
-  static constexpr uint32_t EPI_BYTES = EPI == DACT ? 12288 : 8192;
-  static constexpr int STAGES = EPI == DACT ? 4 : 5;
-  static constexpr uint32_t EPI_OFF = STAGES * 2 * OP_BYTES, BAR_OFF = EPI_OFF + EPI_WARPS * EPI_BYTES;
-  static constexpr uint32_t TOTAL = BAR_OFF + (2 * STAGES + 4 + EPI_WARPS) * 8 + 16 + 1024;
-};
+constexpr int STAGES = 6;
+constexpr uint32_t EPI_OFF = STAGES * 2 * OP_BYTES;
+constexpr uint32_t EPI_BYTES = 4096;  // staging of an epilogue warp: 32 rows of 128 bytes
+constexpr uint32_t BAR_OFF = EPI_OFF + EPI_WARPS * EPI_BYTES;
+constexpr uint32_t SMEM = BAR_OFF + (2 * STAGES + 4) * 8 + 16 + 1024;
 
 struct Args {
   int64_t M = 0;  // rows of the result
   int N = 0;      // columns of the result (DUAL: F)
   int64_t K = 0;
-  int F = 0;      // DUAL: columns of one half of w13
+  int F = 0;      // DUAL, DACT: columns of one half of w13
   int act = 0;
-  int splits = 1;  // PARTIAL
-  int flag = 0;    // STORE: a residual is added; DUAL: g and u are kept
+  int splits = 1;                  // PARTIAL
+  const void* residual = nullptr;  // STORE, optional
+  int64_t ldr = 0;
+  float* f32 = nullptr;  // PARTIAL: sums [splits, M in whole tiles, N]; DUAL: g and u (at_gu) or null; DACT: g and u
 };
-// tensor maps: operands, results and what the epilogue reads
+// tensor maps: operands; the 16-bit result (STORE, DUAL h, DACT dg), and DACT's du
 struct Maps {
-  CUtensorMap a, b;
-  CUtensorMap out;         // STORE result, PARTIAL sums, DUAL h, DACT dg
-  CUtensorMap out2;        // DACT du
-  CUtensorMap in0, in1;    // STORE residual | DACT g, u
-  CUtensorMap gate, up;    // DUAL g, u
+  CUtensorMap a, b, out, out2;
 };
+
+// g and u are kept as the epilogue's threads hold them, 32 rows x 8 columns (32 bytes a row) at a time: a warp's access
+// is 1 KB in one piece. (Row-major, a warp's 32-byte pieces of 32 rows cost four times the L1 cycles, which the MMAs'
+// operands need too: 187 against 152 us for the forward product at 4,100 x 2,048 x 6,144.)
+AFB_DEV int64_t at_gu(int64_t row, int col, int F, int half) {
+  return ((row >> 5) * 2 + half) * F * 32 + (int64_t)(col >> 3) * 256 + (row & 31) * 8 + (col & 7);
+}
 
 template <bool F16>
 AFB_DEV uint32_t pack2(float a, float b) {
@@ -104,37 +106,41 @@ AFB_DEV void with_act(int act, F&& f) {
 }
 
 struct Tile {
-  int64_t m0;
-  int n0, split;
+  int m, n, split;  // row tile, column tile, K split
 };
-// tile order: bands of 8 row tiles, down the band first, so that the tiles in flight share both operands in L2
-AFB_DEV Tile tile_at(int64_t t, int mt, int nt, int tn) {
+// tile order: bands of 8 row tiles, down the band first, so that the tiles in flight share both operands in L2.
+// 32-bit: the tile count is checked on the host, and a 64-bit division costs the producer some 200 cycles.
+AFB_DEV Tile tile_at(uint32_t t, uint32_t mt, uint32_t nt) {
   Tile r;
-  const int64_t per = (int64_t)mt * nt;
-  r.split = (int)(t / per);
+  const uint32_t per = mt * nt;
+  r.split = t / per;
   t -= r.split * per;
-  const int64_t band = t / (8ll * nt);
-  const int rows = (int)min((int64_t)8, mt - band * 8);
-  const int64_t in = t - band * 8ll * nt;
-  r.m0 = (band * 8 + in % rows) * BM;
-  r.n0 = (int)(in / rows) * tn;
+  const uint32_t band = t / (8u * nt), in = t - band * 8u * nt, rows = min(8u, mt - band * 8u), n = in / rows;
+  r.m = band * 8u + in - n * rows;
+  r.n = n;
   return r;
 }
 
-// fp32 row of 32 columns / 16-bit row of 64 columns <-> a 128-byte swizzled staging row
+AFB_DEV void st32(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+AFB_DEV void ld32(const void* p, uint32_t* r) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p)
+               : "memory");
+}
+AFB_DEV void st_gu(float* p, const float* v) { st32(p, reinterpret_cast<const uint32_t*>(v)); }
+AFB_DEV void ld_gu(const float* p, float* v) { ld32(p, reinterpret_cast<uint32_t*>(v)); }
+
+// a 16-bit row of 64 columns (or fp32 of 32) -> a 128-byte swizzled staging row; of 32 columns -> a 64-byte one
 AFB_DEV void put_row(uint8_t* buf, int row, const uint32_t* w) {
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     *reinterpret_cast<uint4*>(buf + sw128_offset(row, j)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
 }
-AFB_DEV void get_row(const uint8_t* buf, int row, uint32_t* w) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint4 q = *reinterpret_cast<const uint4*>(buf + sw128_offset(row, j));
-    w[4 * j] = q.x, w[4 * j + 1] = q.y, w[4 * j + 2] = q.z, w[4 * j + 3] = q.w;
-  }
-}
-// 16-bit row of 32 columns -> a 64-byte swizzled staging row
 AFB_DEV void put_half_row(uint8_t* buf, int row, const uint32_t* w) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -145,30 +151,29 @@ AFB_DEV void put_half_row(uint8_t* buf, int row, const uint32_t* w) {
 // Persistent: pair p of the grid takes tiles p, p + pairs, ... Each CTA: warp 0 loads its halves of the operands by
 // TMA into a STAGES-deep ring, one thread of the leader's warp 1 issues the MMAs of both CTAs into one of two TMEM
 // accumulators, and 8 epilogue warps drain the other one (two warps a lane quadrant, half of the columns each) through
-// swizzled staging rows and TMA stores, so the tensor cores work through the next tile meanwhile.
+// swizzled staging rows and TMA stores, so the tensor cores work through the next tile meanwhile. What bounds the tiles
+// is shared memory's bandwidth (a K block moves 80 KB of it a CTA: 600 cycles, where its MMAs take 512), so the
+// epilogue is kept to whole 128-byte lines.
 template <int LAYOUT, int EPI, bool F16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     ffn_gemm_kernel(const __grid_constant__ Maps maps, Args g, uint32_t* status) {
-  using S = Smem<EPI>;
-  constexpr int STAGES = S::STAGES;
   constexpr bool A_MN = LAYOUT == TN, B_MN = LAYOUT != NT;
   constexpr int TN_COLS = EPI == DUAL ? BN / 2 : BN;  // result columns per tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);  // leader's: both CTAs' operands have landed
-  uint64_t* empty = full + STAGES;                                  // the pair's MMAs of the stage are done
-  uint64_t* acc_full = empty + STAGES;                              // [2] accumulator complete
-  uint64_t* acc_empty = acc_full + 2;                               // [2] leader's: drained by both CTAs' epilogues
-  uint64_t* ld_bar = acc_empty + 2;                                 // [EPI_WARPS] a warp's epilogue loads
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ld_bar + EPI_WARPS);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + BAR_OFF);  // leader's: both CTAs' operands have landed
+  uint64_t* empty = full + STAGES;                               // the pair's MMAs of the stage are done
+  uint64_t* acc_full = empty + STAGES;                           // [2] accumulator complete
+  uint64_t* acc_empty = acc_full + 2;                            // [2] leader's: drained by both CTAs' epilogues
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_cta_rank();
-  const int mt = (int)((g.M + BM - 1) / BM), nt = (g.N + TN_COLS - 1) / TN_COLS;
-  const int64_t tiles = (int64_t)mt * nt * g.splits;
-  const int64_t t0 = blockIdx.x >> 1, step = gridDim.x >> 1;
-  const int kb_total = (int)((g.K + BK - 1) / BK);
-  auto kb_lo = [&](int split) { return (int)((int64_t)kb_total * split / g.splits); };
+  const uint32_t mt = (uint32_t)((g.M + BM - 1) / BM), nt = (g.N + TN_COLS - 1) / TN_COLS, tiles = mt * nt * g.splits;
+  const uint32_t t0 = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const uint32_t kb_total = (uint32_t)((g.K + BK - 1) / BK);
+  // first K block of a split; at most 32 splits of 2^25 blocks
+  auto kb_lo = [&](uint32_t split) { return EPI == PARTIAL ? kb_total * split / (uint32_t)g.splits : split * kb_total; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -179,7 +184,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       mbar_init(&acc_full[s], 1);
       mbar_init(&acc_empty[s], 2 * EPI_WARPS);
     }
-    for (int s = 0; s < EPI_WARPS; ++s) mbar_init(&ld_bar[s], 1);
     fence_mbar_init();
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
@@ -195,16 +199,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       prefetch_tmap(&maps.a);
       prefetch_tmap(&maps.b);
-      int64_t i = 0;  // stages issued
+      uint32_t i = 0, s = 0, ph = 1;  // stages issued, the ring's next stage and its empty barrier's parity
       bool ok = true;
-      for (int64_t t = t0; t < tiles && ok; t += step) {
-        const Tile tl = tile_at(t, mt, nt, TN_COLS);
-        const int kb1 = kb_lo(tl.split + 1);
-        const int ma = (int)tl.m0 + (int)rank * 128;
-        const int nb = EPI == DUAL ? (int)rank * g.F + tl.n0 : tl.n0 + (int)rank * 128;
-        for (int kb = kb_lo(tl.split); kb < kb1; ++kb, ++i) {
-          const int s = (int)(i % STAGES);
-          if (i >= STAGES && !mbar_wait(&empty[s], ((i / STAGES) & 1) ^ 1, status)) {
+      for (uint32_t t = t0; t < tiles && ok; t += step) {
+        const Tile tl = tile_at(t, mt, nt);
+        const uint32_t kb1 = kb_lo(tl.split + 1);
+        const int ma = tl.m * BM + (int)rank * 128;
+        const int nb = EPI == DUAL ? (int)rank * g.F + tl.n * TN_COLS : tl.n * TN_COLS + (int)rank * 128;
+        for (uint32_t kb = kb_lo(tl.split); kb < kb1; ++kb, ++i) {
+          if (!mbar_wait(&empty[s], ph, status)) {  // (passes at once in the ring's first round)
             ok = false;
             break;
           }
@@ -212,7 +215,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const uint32_t bar = cluster_addr(&full[s], 0);
           uint8_t* a = smem + s * 2 * OP_BYTES;
           uint8_t* b = a + OP_BYTES;
-          const int k = kb * BK;
+          const int k = (int)kb * BK;
           if constexpr (A_MN) {
             tma_load_2d_pair(a, &maps.a, bar, ma, k);
             tma_load_2d_pair(a + 8192, &maps.a, bar, ma + 64, k);
@@ -225,27 +228,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           } else {
             tma_load_2d_pair(b, &maps.b, bar, k, nb);
           }
+          if (++s == STAGES) s = 0, ph ^= 1;
         }
       }
       // every stage issued has been read (so its copies have landed) before the CTA may leave
-      for (int64_t j = max((int64_t)0, i - STAGES); j < i; ++j)
+      for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j)
         mbar_wait(&empty[j % STAGES], (j / STAGES) & 1, status);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       constexpr uint32_t idesc =
           idesc_f16(BM, BN, F16 ? 0 : 1) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16);
-      int64_t i = 0;
-      int n = 0;  // tiles of this pair
+      uint32_t n = 0, s = 0, ph = 0;  // tiles of this pair; ring stage and its full barrier's parity
       bool ok = true;
-      for (int64_t t = t0; t < tiles && ok; t += step, ++n) {
-        const int split = (int)(t / ((int64_t)mt * nt)), kb0 = kb_lo(split), kb1 = kb_lo(split + 1);
+      for (uint32_t t = t0; t < tiles && ok; t += step, ++n) {
+        const uint32_t split = EPI == PARTIAL ? t / (mt * nt) : 0, kb0 = kb_lo(split), kb1 = kb_lo(split + 1);
         const uint32_t acc = tmem + (n & 1) * BN;
         if (!mbar_wait(&acc_empty[n & 1], ((n >> 1) & 1) ^ 1, status)) break;
         tc_fence_after();
-        for (int kb = kb0; kb < kb1; ++kb, ++i) {
-          const int s = (int)(i % STAGES);
-          if (!mbar_wait(&full[s], (i / STAGES) & 1, status)) {
+        for (uint32_t kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(&full[s], ph, status)) {
             ok = false;
             break;
           }
@@ -258,129 +260,123 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             umma_f16_pair(acc, da, db, idesc, kb > kb0 || kk > 0);
           }
           umma_commit_pair(&empty[s]);
+          if (++s == STAGES) s = 0, ph ^= 1;
         }
         umma_commit_pair(&acc_full[n & 1]);
       }
     }
   } else {
-    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
-    uint8_t* buf0 = smem + S::EPI_OFF + ew * S::EPI_BYTES;
-    uint8_t* buf1 = buf0 + 4096;
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* buf = smem + EPI_OFF + (warp - 2) * EPI_BYTES;
     const uint32_t drained[2] = {cluster_addr(&acc_empty[0], 0), cluster_addr(&acc_empty[1], 0)};
-    constexpr int HALF = TN_COLS / 2;                          // result columns of a warp
-    constexpr int CW = EPI == STORE || EPI == DUAL ? 64 : 32;  // result columns of a chunk
-    constexpr int CH = HALF / CW;
-    auto row_of = [&](const Tile& tl) { return tl.m0 + rank * 128 + quad * 32; };
-    auto live = [&](const Tile& tl, int c) { return row_of(tl) < g.M && tl.n0 + half * HALF + c * CW < g.N; };
-    // the epilogue's own loads run one chunk ahead: the residual (STORE) or g and u (DACT)
-    const bool loads = EPI == DACT || (EPI == STORE && g.flag);
-    int nis = 0;  // loads issued (lane 0)
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) {  // one answer for the warp
-      return (bool)__all_sync(0xffffffffu, mbar_wait(bar, parity, status));
+    constexpr int HALF = TN_COLS / 2;  // result columns of a warp
+    const int warp_row = (int)rank * 128 + quad * 32, lane_col = half * HALF;
+    // the staging rows are free once the last store has read them; written, they go to the async proxy
+    auto begin_put = [&] {
+      if (lane == 0) bulk_wait_read<0>();
+      __syncwarp();
     };
-    auto load = [&](int64_t t, int c) {  // chunk c of tile t, or the next tile's first; lane 0
-      if (c == CH) {
-        t += step;
-        c = 0;
-      }
+    auto end_put = [&] {
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    // DACT: g and u of 16 columns, two chunks ahead of their use
+    float gq[2][EPI == DACT ? 16 : 1], uq[2][EPI == DACT ? 16 : 1];
+    auto load_gu = [&](uint32_t t, int c, float* gp, float* up) {
       if (t >= tiles) return;
-      const Tile tl = tile_at(t, mt, nt, TN_COLS);
-      if (!live(tl, c)) return;
-      ++nis;
-      const int col = tl.n0 + half * HALF + c * CW, row = (int)row_of(tl);
-      if constexpr (EPI == DACT) {
-        mbar_arrive_expect_tx(&ld_bar[ew], 8192);
-        tma_load_2d(buf0, &maps.in0, &ld_bar[ew], col, row);
-        tma_load_2d(buf1, &maps.in1, &ld_bar[ew], col, row);
-      } else {
-        mbar_arrive_expect_tx(&ld_bar[ew], 4096);
-        tma_load_2d(buf1, &maps.in0, &ld_bar[ew], col, row);
-      }
-    };
-    if (loads && lane == 0) load(t0, 0);
-    int n = 0, nld = 0, nst = 0;  // tiles, loads waited for, stores
-    bool ok = true;
-    for (int64_t t = t0; t < tiles && ok; t += step, ++n) {
-      const Tile tl = tile_at(t, mt, nt, TN_COLS);
-      const int row = (int)row_of(tl), col_h = tl.n0 + half * HALF;
-      ok = wait_all(&acc_full[n & 1], (n >> 1) & 1);
-      tc_fence_after();
-      const uint32_t acc = tmem + (n & 1) * BN + ((uint32_t)(quad * 32) << 16);
-      for (int c = 0; c < CH && ok; ++c) {
-        if (!live(tl, c)) {
-          // outside the result: the next tile's first load, which the last chunk starts, still has to run ahead
-          if (loads && lane == 0 && c == CH - 1) load(t, CH);
-          continue;
-        }
-        const int col = col_h + c * CW;
-        if constexpr (EPI == STORE) {
-          float v[64];
-          tmem_ld32(acc + half * HALF + c * CW, v);
-          tmem_ld32(acc + half * HALF + c * CW + 32, v + 32);
-          tmem_ld_wait();
-          if (g.flag) {
-            ok = wait_all(&ld_bar[ew], nld++ & 1);
-            uint32_t r[32];
-            get_row(buf1, lane, r);
+      const Tile tl = tile_at(t, mt, nt);
+      const int64_t row = (int64_t)tl.m * BM + warp_row + lane;
+      const int col = tl.n * TN_COLS + lane_col + c * 16;
+      if (row >= g.M) return;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float2 f = unpack2<F16>(r[j]);
-              v[2 * j] += f.x;
-              v[2 * j + 1] += f.y;
-            }
+      for (int j = 0; j < 16; j += 8)
+        if (col + j < g.N) {
+          ld_gu(g.f32 + at_gu(row, col + j, g.F, 0), gp + j);
+          ld_gu(g.f32 + at_gu(row, col + j, g.F, 1), up + j);
+        }
+    };
+    if constexpr (EPI == DACT) {
+      load_gu(t0, 0, gq[0], uq[0]);
+      load_gu(t0, 1, gq[1], uq[1]);
+    }
+    uint32_t n = 0;  // tiles of this pair
+    for (uint32_t t = t0; t < tiles; t += step, ++n) {
+      const Tile tl = tile_at(t, mt, nt);
+      const int row0 = tl.m * BM + warp_row, col0 = tl.n * TN_COLS + lane_col;
+      const int64_t row = (int64_t)row0 + lane;
+      const bool live = row < g.M, any = row0 < g.M;  // this lane's row, one of the warp's
+      // one answer for the warp
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[n & 1], (n >> 1) & 1, status))) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + (n & 1) * BN + ((uint32_t)(quad * 32) << 16) + half * HALF;
+      if constexpr (EPI == STORE) {
+#pragma unroll 1
+        for (int c = 0; c < HALF && any; c += 64) {
+          const int col = col0 + c;
+          if (col >= g.N) break;
+          float v[64];
+          tmem_ld32(acc + c, v);
+          tmem_ld32(acc + c + 32, v + 32);
+          tmem_ld_wait();
+          if (g.residual && live) {
+            const uint16_t* rp = reinterpret_cast<const uint16_t*>(g.residual) + row * g.ldr + col;
+#pragma unroll
+            for (int j = 0; j < 64; j += 8)
+              if (col + j < g.N) {
+                const uint4 q = *reinterpret_cast<const uint4*>(rp + j);
+                const uint32_t r[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = unpack2<F16>(r[i]);
+                  v[j + 2 * i] += f.x;
+                  v[j + 2 * i + 1] += f.y;
+                }
+              }
           }
           uint32_t w[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) w[j] = pack2<F16>(v[2 * j], v[2 * j + 1]);
-          uint8_t* buf = g.flag || (nst & 1) == 0 ? buf0 : buf1;
-          if (lane == 0) {
-            if (g.flag) bulk_wait_read<0>();
-            else bulk_wait_read<1>();
-          }
-          __syncwarp();
+          begin_put();
           put_row(buf, lane, w);
-          fence_proxy_async_smem();
-          __syncwarp();
+          end_put();
           if (lane == 0) {
-            if (ok) tma_store_2d(&maps.out, buf, col, row);
+            tma_store_2d(&maps.out, buf, col, row0);
             bulk_commit();
-            if (g.flag) load(t, c + 1);
           }
-          ++nst;
-        } else if constexpr (EPI == PARTIAL) {
+        }
+      } else if constexpr (EPI == PARTIAL) {
+#pragma unroll 1
+        for (int c = 0; c < HALF && any; c += 32) {
+          const int col = col0 + c;
+          if (col >= g.N) break;
           float v[32];
-          tmem_ld32(acc + half * HALF + c * CW, v);
+          tmem_ld32(acc + c, v);
           tmem_ld_wait();
-          uint8_t* buf = (nst & 1) == 0 ? buf0 : buf1;
-          if (lane == 0) bulk_wait_read<1>();
-          __syncwarp();
+          begin_put();
           put_row(buf, lane, reinterpret_cast<const uint32_t*>(v));
-          fence_proxy_async_smem();
-          __syncwarp();
+          end_put();
           if (lane == 0) {
-            tma_store_2d(&maps.out, buf, col, tl.split * mt * BM + row);
+            tma_store_2d(&maps.out, buf, col, tl.split * (int)mt * BM + row0);
             bulk_commit();
           }
-          ++nst;
-        } else if constexpr (EPI == DUAL) {
+        }
+      } else if constexpr (EPI == DUAL) {
+        if (any && col0 < g.N) {
           uint32_t h[32];
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             float v[32], w[32];
-            tmem_ld32(acc + half * HALF + q * 32, v);
-            tmem_ld32(acc + BN / 2 + half * HALF + q * 32, w);
+            tmem_ld32(acc + q * 32, v);
+            tmem_ld32(acc + BN / 2 + q * 32, w);
             tmem_ld_wait();
-            if (g.flag && col + q * 32 < g.N) {
-              if (lane == 0) bulk_wait_read<0>();
-              __syncwarp();
-              put_row(buf0, lane, reinterpret_cast<const uint32_t*>(v));
-              put_row(buf1, lane, reinterpret_cast<const uint32_t*>(w));
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                tma_store_2d(&maps.gate, buf0, col + q * 32, row);
-                tma_store_2d(&maps.up, buf1, col + q * 32, row);
-                bulk_commit();
+            if (g.f32 && live) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 8) {
+                const int col = col0 + q * 32 + j;
+                if (col < g.N) {
+                  st_gu(g.f32 + at_gu(row, col, g.F, 0), v + j);
+                  st_gu(g.f32 + at_gu(row, col, g.F, 1), w + j);
+                }
               }
             }
             with_act(g.act, [&](auto A) {
@@ -390,50 +386,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                                            act_only<A.value>(v[2 * j + 1]) * w[2 * j + 1]);
             });
           }
-          if (lane == 0) bulk_wait_read<0>();
-          __syncwarp();
-          put_row(buf0, lane, h);
-          fence_proxy_async_smem();
-          __syncwarp();
+          begin_put();
+          put_row(buf, lane, h);
+          end_put();
           if (lane == 0) {
-            tma_store_2d(&maps.out, buf0, col, row);
+            tma_store_2d(&maps.out, buf, col0, row0);
             bulk_commit();
           }
-        } else {  // DACT
-          float v[32];
-          tmem_ld32(acc + half * HALF + c * CW, v);
-          ok = wait_all(&ld_bar[ew], nld++ & 1);
-          uint32_t gr[32], ur[32];
-          get_row(buf0, lane, gr);
-          get_row(buf1, lane, ur);
+        }
+      } else {  // DACT
+        constexpr int CH = HALF / 16;
+        uint32_t dg[16], du[16];  // 32 columns
+        auto chunk = [&](int c, float* gp, float* up, uint32_t* dgp, uint32_t* dup) {
+          float v[16];
+          tmem_ld16(acc + c * 16, v);
           tmem_ld_wait();
-          __syncwarp();  // both buffers have been read: the next chunk may land
-          if (lane == 0) {
-            load(t, c + 1);
-            bulk_wait_read<0>();
-          }
-          uint32_t dg[16], du[16];
           with_act(g.act, [&](auto A) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
+            for (int j = 0; j < 8; ++j) {
               float a0, d0, a1, d1;
-              act_grad<A.value>(__uint_as_float(gr[2 * j]), a0, d0);
-              act_grad<A.value>(__uint_as_float(gr[2 * j + 1]), a1, d1);
-              dg[j] = pack2<F16>(v[2 * j] * __uint_as_float(ur[2 * j]) * d0,
-                                 v[2 * j + 1] * __uint_as_float(ur[2 * j + 1]) * d1);
-              du[j] = pack2<F16>(v[2 * j] * a0, v[2 * j + 1] * a1);
+              act_grad<A.value>(gp[2 * j], a0, d0);
+              act_grad<A.value>(gp[2 * j + 1], a1, d1);
+              dgp[j] = pack2<F16>(v[2 * j] * up[2 * j] * d0, v[2 * j + 1] * up[2 * j + 1] * d1);
+              dup[j] = pack2<F16>(v[2 * j] * a0, v[2 * j + 1] * a1);
             }
           });
-          __syncwarp();
-          put_half_row(buf0 + 8192, lane, dg);
-          put_half_row(buf0 + 10240, lane, du);
-          fence_proxy_async_smem();
-          __syncwarp();
+          load_gu(c + 2 < CH ? t : t + step, (c + 2) % CH, gp, up);
+        };
+#pragma unroll 1
+        for (int c = 0; c < CH; c += 2) {
+          chunk(c, gq[0], uq[0], dg, du);
+          chunk(c + 1, gq[1], uq[1], dg + 8, du + 8);
+          const int col = col0 + c * 16;
+          if (!any || col >= g.N) continue;
+          begin_put();
+          put_half_row(buf, lane, dg);
+          put_half_row(buf + 2048, lane, du);
+          end_put();
           if (lane == 0) {
-            if (ok) {
-              tma_store_2d(&maps.out, buf0 + 8192, col, row);
-              tma_store_2d(&maps.out2, buf0 + 10240, col, row);
-            }
+            tma_store_2d(&maps.out, buf, col, row0);
+            tma_store_2d(&maps.out2, buf + 2048, col, row0);
             bulk_commit();
           }
         }
@@ -442,10 +434,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(drained[n & 1]);
     }
-    if (lane == 0) {
-      if (nis > nld) mbar_wait(&ld_bar[ew], nld & 1, status);  // after a failed wait: the copy in flight lands first
-      bulk_wait<0>();
-    }
+    if (lane == 0) bulk_wait<0>();
   }
   tc_fence_before();
   __syncthreads();
@@ -475,7 +464,7 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict
       make_uint4(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7]));
 }
 
-// K splits of a product: those that minimise waves of tiles x K blocks of a tile (0.28 us each at the full rate), plus
+// K splits of a product: those that minimise waves of tiles x K blocks of a tile (0.37 us each at the rate the products reach), plus
 // the fp32 partials written and read again (about 4 TB/s through L2) and the second launch (3 us)
 static int plan_splits(int64_t M, int N, int64_t K, int num_sms) {
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN), kb = (K + BK - 1) / BK, pairs = num_sms / 2;
@@ -484,7 +473,7 @@ static int plan_splits(int64_t M, int N, int64_t K, int num_sms) {
   double cost = 1e300;
   for (int s = 1; s <= 32 && s * 4 <= std::max<int64_t>(kb, 4); ++s) {
     const double waves = (double)((tiles * s + pairs - 1) / pairs);
-    const double c = waves * (double)((kb + s - 1) / s) * 0.28 +
+    const double c = waves * (double)((kb + s - 1) / s) * 0.37 +
                      (s > 1 ? 3. + 8. * s * (double)M * N / 4e6 : 0.);
     if (c < cost * 0.98) best = s, cost = c;
   }
@@ -508,16 +497,18 @@ static int launch(Ptr A, Ptr B, int64_t b_rows, Maps& maps, const Args& g, int n
   if (rc) return 2000 + rc;
   auto kern = ffn_gemm_kernel<LAYOUT, EPI, F16>;
   static std::atomic<uint64_t> devs{0};
-  if (const int e = smem_attr_once(devs, (const void*)kern, Smem<EPI>::TOTAL)) return e;
+  if (const int e = smem_attr_once(devs, (const void*)kern, SMEM)) return e;
   constexpr int cols = EPI == DUAL ? BN / 2 : BN;
   const int64_t tiles = ((g.M + BM - 1) / BM) * ((g.N + cols - 1) / cols) * g.splits;
+  if (tiles >= (1 << 30)) return 5;
   const int pairs = (int)std::min<int64_t>(tiles, std::max(1, num_sms / 2));
-  return launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), Smem<EPI>::TOTAL, st, maps, g, status);
+  return launch_pdl(kern, dim3(2 * pairs), dim3(THREADS), SMEM, st, maps, g, status);
 }
 
-// map of a result or epilogue input: boxes of 32 rows x 128 (or 64) bytes
+// map of a result: boxes of 32 rows x 128 (or 64) bytes
 static int row_map(CUtensorMap* m, const void* p, int bytes, int64_t cols, int64_t rows, int64_t ld, int row_bytes) {
-  return make_tmap_2d(m, p, bytes, cols, rows, ld * bytes, row_bytes / bytes, 32, row_bytes);
+  const int rc = make_tmap_2d(m, p, bytes, cols, rows, ld * bytes, row_bytes / bytes, 32, row_bytes);
+  return rc ? 3000 + rc : 0;
 }
 
 // out [M, N] = A B in LAYOUT (+ residual), rounded to the element type, split over K where that pays
@@ -526,17 +517,13 @@ static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr res
                    uint32_t* status, cudaStream_t st) {
   Maps maps;
   Args g;
-  g.M = M, g.N = N, g.K = K;
+  g.M = M, g.N = N, g.K = K, g.residual = residual.p, g.ldr = residual.ld;
   g.splits = residual.p ? 1 : plan_splits(M, N, K, num_sms);
-  int rc;
-  if (g.splits == 1) {
-    if ((rc = row_map(&maps.out, out, 2, N, M, N, 128))) return 3000 + rc;
-    g.flag = residual.p != nullptr;
-    if (g.flag && (rc = row_map(&maps.in0, residual.p, 2, N, M, residual.ld, 128))) return 3100 + rc;
-    return launch<LAYOUT, STORE, F16>(A, B, N, maps, g, num_sms, status, st);
-  }
   const int64_t rows = (M + BM - 1) / BM * BM;  // of a split's partial sums: whole tiles
-  if ((rc = row_map(&maps.out, scratch, 4, N, rows * g.splits, N, 128))) return 3200 + rc;
+  int rc = g.splits == 1 ? row_map(&maps.out, out, 2, N, M, N, 128)
+                         : row_map(&maps.out, scratch, 4, N, rows * g.splits, N, 128);
+  if (rc) return rc;
+  if (g.splits == 1) return launch<LAYOUT, STORE, F16>(A, B, N, maps, g, num_sms, status, st);
   rc = launch<LAYOUT, PARTIAL, F16>(A, B, N, maps, g, num_sms, status, st);
   if (rc) return rc;
   return launch_pdl(ffn_reduce_kernel<F16>, dim3((unsigned)((M * N / 8 + 255) / 256)), dim3(256), 0, st,
@@ -564,7 +551,7 @@ struct FewArgs {
   int T = 0, n = 0;  // rows; weight rows (DUAL: F)
   int K = 0, F = 0, act = 0;
   void* out = nullptr;             // DUAL: h [2T, F]; else y [T, n]
-  float* gu = nullptr;             // DUAL: [T, 2F] or null
+  float* gu = nullptr;             // DUAL: g and u (at_gu) or null
   const void* residual = nullptr;  // else: [T, n] or null
   int64_t ldr = 0;
 };
@@ -707,8 +694,8 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
       if constexpr (DUAL_) {
         const float2 u = sum(((g.T + t) * 128 + f) * 4);
         if (g.gu) {
-          *reinterpret_cast<float2*>(g.gu + (int64_t)t * 2 * g.F + col) = a;
-          *reinterpret_cast<float2*>(g.gu + (int64_t)t * 2 * g.F + g.F + col) = u;
+          *reinterpret_cast<float2*>(g.gu + at_gu(t, col, g.F, 0)) = a;
+          *reinterpret_cast<float2*>(g.gu + at_gu(t, col, g.F, 1)) = u;
         }
         with_act(g.act, [&](auto A) {
           a = make_float2(act_only<A.value>(a.x) * u.x, act_only<A.value>(a.y) * u.y);
@@ -795,12 +782,9 @@ static int fwd(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h,
   }
   Maps maps;
   Args g;
-  g.M = s.T, g.N = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.flag = gu != nullptr;
+  g.M = s.T, g.N = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.f32 = gu;
   int rc = row_map(&maps.out, h, 2, s.F, s.T, s.F, 128);
-  if (!rc && gu) rc = row_map(&maps.gate, gu, 4, s.F, s.T, 2 * (int64_t)s.F, 128);
-  if (!rc && gu) rc = row_map(&maps.up, gu + s.F, 4, s.F, s.T, 2 * (int64_t)s.F, 128);
-  if (rc) return 4000 + rc;
-  rc = launch<NT, DUAL, F16>(x, w13, 2 * (int64_t)s.F, maps, g, num_sms, status, st);
+  if (!rc) rc = launch<NT, DUAL, F16>(x, w13, 2 * (int64_t)s.F, maps, g, num_sms, status, st);
   if (rc) return rc;
   return product<NT, F16>({h, s.F}, w2, s.T, s.N, s.F, y, residual, scratch, num_sms, status, st);
 }
@@ -814,14 +798,12 @@ static int bwd(const FfnShape& s, Ptr dy, Ptr x, Ptr w13, Ptr w2, const void* h,
   if (!dx && !dw13) return 0;
   Maps maps;
   Args g;
-  g.M = s.T, g.N = s.F, g.K = s.N, g.act = s.act;
+  g.M = s.T, g.N = s.F, g.K = s.N, g.F = s.F, g.act = s.act, g.f32 = const_cast<float*>(gu);
   uint16_t* o = reinterpret_cast<uint16_t*>(dgu);
-  rc = row_map(&maps.in0, gu, 4, s.F, s.T, d.ld, 128);
-  if (!rc) rc = row_map(&maps.in1, gu + s.F, 4, s.F, s.T, d.ld, 128);
-  if (!rc) rc = row_map(&maps.out, o, 2, s.F, s.T, d.ld, 64);
+  rc = row_map(&maps.out, o, 2, s.F, s.T, d.ld, 64);
   if (!rc) rc = row_map(&maps.out2, o + s.F, 2, s.F, s.T, d.ld, 64);
-  if (rc) return 4100 + rc;
-  if ((rc = launch<NN, DACT, F16>(dy, w2, s.F, maps, g, num_sms, status, st))) return rc;
+  if (!rc) rc = launch<NN, DACT, F16>(dy, w2, s.F, maps, g, num_sms, status, st);
+  if (rc) return rc;
   if (dx && (rc = product<NN, F16>(d, w13, s.T, s.H, 2 * (int64_t)s.F, dx, none, scratch, num_sms, status, st)))
     return rc;
   if (dw13) rc = product<TN, F16>(d, x, 2 * (int64_t)s.F, s.H, s.T, dw13, none, scratch, num_sms, status, st);

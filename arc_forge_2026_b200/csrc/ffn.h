@@ -19,7 +19,8 @@ struct FfnShape {
 size_t ffn_fwd_scratch(const FfnShape& s, int num_sms);
 size_t ffn_bwd_scratch(const FfnShape& s, int num_sms);
 int64_t ffn_h_rows(const FfnShape& s);  // rows of the buffer for h: T, or 2T where a second term is kept
-// h [ffn_h_rows, F], h itself in the first T rows; gu [T, 2F] fp32 (the pre-activations, for the backward pass) or null; y [T, N]
+// h [ffn_h_rows, F], h itself in the first T rows; gu [T rounded up to 32, 2F] fp32 (the pre-activations in the
+// kernels' own order, for the backward pass), 32-byte aligned, or null; y [T, N]
 int ffn_fwd(const FfnShape& s, const void* x, int64_t ldx, const void* w13, const void* w2, const void* residual,
             int64_t ldr, void* h, float* gu, void* y, float* scratch, int num_sms, uint32_t* status,
             cudaStream_t stream);

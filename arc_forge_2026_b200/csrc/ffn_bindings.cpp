@@ -86,7 +86,7 @@ std::tuple<at::Tensor, at::Tensor, OptT> gated_ffn_fwd(const at::Tensor& x_, con
   }
   at::Tensor y = at::empty({s.T, s.N}, x.options()), h = at::empty({afb::ffn_h_rows(s), s.F}, x.options());
   OptT gu;
-  if (save) gu = at::empty({s.T, 2 * (int64_t)s.F}, x.options().dtype(at::kFloat));
+  if (save) gu = at::empty({(s.T + 31) / 32 * 32, 2 * (int64_t)s.F}, x.options().dtype(at::kFloat));
   const size_t n_scr = afb::ffn_fwd_scratch(s, num_sms());
   const at::Tensor scr = n_scr ? scratch_of(n_scr, x) : at::Tensor();
   check_rc(afb::ffn_fwd(s, x.data_ptr(), ld(x), w13.data_ptr(), w2.data_ptr(), r.defined() ? r.data_ptr() : nullptr,
@@ -110,7 +110,7 @@ std::tuple<OptT, OptT, OptT> gated_ffn_bwd(const at::Tensor& dy_, const at::Tens
                 "gated_ffn: h of the forward pass");
   if (need_dx || need_dw13)
     TORCH_CHECK(gu.has_value() && gu->is_contiguous() && gu->scalar_type() == at::kFloat && gu->dim() == 2 &&
-                    gu->size(0) == s.T && gu->size(1) == 2 * (int64_t)s.F && gu->device() == x_.device(),
+                    gu->size(0) >= s.T && gu->size(1) == 2 * (int64_t)s.F && gu->device() == x_.device(),
                 "gated_ffn: gu of the forward pass");
   c10::cuda::CUDAGuard g(x_.device());
   const at::Tensor x = tma_rows(x_), w13 = tma_rows(w13_.contiguous()), w2 = tma_rows(w2_.contiguous()),
