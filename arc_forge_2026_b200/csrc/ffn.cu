@@ -175,6 +175,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   // first K block of a split; at most 32 splits of 2^25 blocks
   auto kb_lo = [&](uint32_t split) { return EPI == PARTIAL ? kb_total * split / (uint32_t)g.splits : split * kb_total; };
 
+  if (threadIdx.x == 32) {
+    prefetch_tmap(&maps.a);
+    prefetch_tmap(&maps.b);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -197,8 +201,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 
   if (warp == 0) {
     if (lane == 0) {
-      prefetch_tmap(&maps.a);
-      prefetch_tmap(&maps.b);
       uint32_t i = 0, s = 0, ph = 1;  // stages issued, the ring's next stage and its empty barrier's parity
       bool ok = true;
       for (uint32_t t = t0; t < tiles && ok; t += step) {
@@ -282,22 +284,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     };
     // DACT: g and u of 16 columns, two chunks ahead of their use
     float gq[2][EPI == DACT ? 16 : 1], uq[2][EPI == DACT ? 16 : 1];
-    auto load_gu = [&](uint32_t t, int c, float* gp, float* up) {
-      if (t >= tiles) return;
+    struct GuTile {
+      const float *g, *u;  // this lane's first column of the tile, or null where its row is outside the result
+      int col;
+    };
+    auto gu_tile = [&](uint32_t t) {
+      GuTile r{nullptr, nullptr, 0};
+      if (EPI != DACT || t >= tiles) return r;
       const Tile tl = tile_at(t, mt, nt);
       const int64_t row = (int64_t)tl.m * BM + warp_row + lane;
-      const int col = tl.n * TN_COLS + lane_col + c * 16;
-      if (row >= g.M) return;
+      r.col = tl.n * TN_COLS + lane_col;
+      if (row < g.M) r.g = g.f32 + at_gu(row, r.col, g.F, 0), r.u = g.f32 + at_gu(row, r.col, g.F, 1);
+      return r;
+    };
+    auto load_gu = [&](const GuTile& p, int c, float* gp, float* up) {
+      if (!p.g) return;
 #pragma unroll
       for (int j = 0; j < 16; j += 8)
-        if (col + j < g.N) {
-          ld_gu(g.f32 + at_gu(row, col + j, g.F, 0), gp + j);
-          ld_gu(g.f32 + at_gu(row, col + j, g.F, 1), up + j);
+        if (p.col + c * 16 + j < g.N) {  // 8 columns further is 256 floats further
+          ld_gu(p.g + (c * 16 + j) * 32, gp + j);
+          ld_gu(p.u + (c * 16 + j) * 32, up + j);
         }
     };
+    GuTile gu_now = gu_tile(t0);
     if constexpr (EPI == DACT) {
-      load_gu(t0, 0, gq[0], uq[0]);
-      load_gu(t0, 1, gq[1], uq[1]);
+      load_gu(gu_now, 0, gq[0], uq[0]);
+      load_gu(gu_now, 1, gq[1], uq[1]);
     }
     uint32_t n = 0;  // tiles of this pair
     for (uint32_t t = t0; t < tiles; t += step, ++n) {
@@ -309,6 +321,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[n & 1], (n >> 1) & 1, status))) break;
       tc_fence_after();
       const uint32_t acc = tmem + (n & 1) * BN + ((uint32_t)(quad * 32) << 16) + half * HALF;
+      // the accumulator is free as soon as this warp's last column is in registers
+      bool told = false;
+      auto tell = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote_relaxed(drained[n & 1]);
+        told = true;
+      };
       if constexpr (EPI == STORE) {
 #pragma unroll 1
         for (int c = 0; c < HALF && any; c += 64) {
@@ -318,6 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           tmem_ld32(acc + c, v);
           tmem_ld32(acc + c + 32, v + 32);
           tmem_ld_wait();
+          if (c + 64 >= HALF) tell();
           if (g.residual && live) {
             const uint16_t* rp = reinterpret_cast<const uint16_t*>(g.residual) + row * g.ldr + col;
 #pragma unroll
@@ -352,6 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           float v[32];
           tmem_ld32(acc + c, v);
           tmem_ld_wait();
+          if (c + 32 >= HALF) tell();
           begin_put();
           put_row(buf, lane, reinterpret_cast<const uint32_t*>(v));
           end_put();
@@ -369,6 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tmem_ld32(acc + q * 32, v);
             tmem_ld32(acc + BN / 2 + q * 32, w);
             tmem_ld_wait();
+            if (q == 1) tell();
             if (g.f32 && live) {
 #pragma unroll
               for (int j = 0; j < 32; j += 8) {
@@ -396,11 +419,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         }
       } else {  // DACT
         constexpr int CH = HALF / 16;
+        const GuTile gu_next = gu_tile(t + step);
         uint32_t dg[16], du[16];  // 32 columns
         auto chunk = [&](int c, float* gp, float* up, uint32_t* dgp, uint32_t* dup) {
           float v[16];
           tmem_ld16(acc + c * 16, v);
           tmem_ld_wait();
+          if (c == CH - 1) tell();
           with_act(g.act, [&](auto A) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -411,7 +436,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
               dup[j] = pack2<F16>(v[2 * j] * a0, v[2 * j + 1] * a1);
             }
           });
-          load_gu(c + 2 < CH ? t : t + step, (c + 2) % CH, gp, up);
+          load_gu(c + 2 < CH ? gu_now : gu_next, (c + 2) % CH, gp, up);
         };
 #pragma unroll 1
         for (int c = 0; c < CH; c += 2) {
@@ -429,10 +454,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             bulk_commit();
           }
         }
+        gu_now = gu_next;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote(drained[n & 1]);
+      if (!told) tell();
     }
     if (lane == 0) bulk_wait<0>();
   }

@@ -21,8 +21,10 @@ AFB_DEV uint32_t cluster_addr(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
-AFB_DEV void mbar_arrive_remote(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+// relaxed: orders nothing but itself. Enough after tcgen05.wait::ld to say that TMEM has been read; a release would
+// first wait for every global store of the thread (some 4,000 cycles in the middle of an epilogue).
+AFB_DEV void mbar_arrive_remote_relaxed(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 AFB_DEV float2 ld_cluster_f2(uint32_t a) {
   float2 v;
