@@ -50,9 +50,11 @@ struct NormArgs {
   void* dx = nullptr;           // or null
   void* dw = nullptr;           // or null
   void* db = nullptr;           // or null
-  float* partial = nullptr;     // norm_bwd_partials() rows of 2 x width floats
+  float* partial = nullptr;     // with dw or db: `partials` rows of 2 x width floats
+  int partials = 0;             // norm_bwd_partials()
+  uint32_t* status = nullptr;   // kernel status word
 };
-int norm_bwd_partials(const NormArgs& a, int num_sms);  // rows of `partial` the backward pass writes
+int norm_bwd_partials(const NormArgs& a, int num_sms);  // rows of `partial` the backward pass writes; 0: it cannot run
 int norm_fwd(const NormArgs& a, int num_sms, cudaStream_t stream);
 int norm_bwd(const NormArgs& a, int num_sms, cudaStream_t stream);
 

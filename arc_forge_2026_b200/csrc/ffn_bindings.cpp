@@ -146,6 +146,7 @@ afb::NormArgs norm_args(const at::Tensor& x, const at::Tensor& w, bool rms, doub
   TORCH_CHECK(w.device() == x.device() && w.dim() == 1 && w.size(0) == x.size(1) && w.is_contiguous(),
               "norm: w is contiguous [width] on x's device");
   a.x = x.data_ptr(), a.ldx = x.stride(0), a.w = w.data_ptr();
+  a.status = status_ptr(x.get_device());
   return a;
 }
 
@@ -200,7 +201,9 @@ std::tuple<OptT, OptT, OptT> norm_train_bwd(const at::Tensor& dy_, const at::Ten
   a.dx = optr<void>(dx), a.dw = optr<void>(dw), a.db = optr<void>(db);
   at::Tensor part;
   if (need_dw || need_db) {
-    part = scratch_of((size_t)afb::norm_bwd_partials(a, num_sms()) * 2 * a.width, x);
+    a.partials = afb::norm_bwd_partials(a, num_sms());
+    TORCH_CHECK(a.partials > 0, "norm_train_bwd: no launch plan");
+    part = scratch_of((size_t)a.partials * 2 * a.width, x);
     a.partial = ptr<float>(part);
   }
   check_rc(afb::norm_bwd(a, num_sms(), stream()), "norm_train_bwd");

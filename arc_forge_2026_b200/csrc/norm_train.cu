@@ -4,11 +4,13 @@
 //   v = dy w (or dy (1 + w)); dx = rstd (v - mean(v) - xh mean(v xh))   (rms: without mean(v))
 //   dw = sum_rows dy xh, db = sum_rows dy
 //
-// Memory bounds both directions (forward 2, backward 3 row transfers). A row lives in the registers of WPR warps
-// (NV chunks of 8 elements a lane), so it is read once: the variance is the mean square about the mean already known,
-// not a difference of two sums. In the backward pass a thread owns the same columns in every row its CTA takes, so dw
-// and db add up in its registers over the rows; each CTA writes one row of partial sums and a second kernel adds
-// those in a fixed order (no atomics: results are bitwise reproducible).
+// Memory bounds both directions (forward 2, backward 3 row transfers), and some 45 KB have to be on the way to an SM at
+// any time to use it. CTAs stay and walk the rows; bulk copies bring the next rows of x (and dy) into a ring in shared
+// memory, several rows ahead. A group of warps takes a row into registers, NV chunks of 8 elements a lane, so it is read
+// once: the variance is the mean square about the mean already known, not a difference of two sums. A thread owns the
+// same columns in every row, so the weights are read once and dw and db add up in registers. Each CTA writes one row of
+// partial sums of dw and db and a second kernel adds those in a fixed order (no atomics: results are bitwise
+// reproducible).
 #include <algorithm>
 #include <type_traits>
 
@@ -30,104 +32,255 @@ AFB_DEV T from_f(float v) {
   else if constexpr (std::is_same<T, __half>::value) return __float2half(v);
   else return v;
 }
-// 8 elements from a 16-byte aligned address
+// 8 elements as they lie in memory
 template <typename T>
-AFB_DEV void load8(const T* p, float* f) {
+struct alignas(16) Raw {
+  T v[8];
+};
+template <typename T>
+AFB_DEV void unpack(const Raw<T>& r, float* f) {
   if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  } else {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f(h[i]);
+    for (int i = 0; i < 8; ++i) f[i] = r.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 p;
+      if constexpr (std::is_same<T, __half>::value) p = __half22float2(reinterpret_cast<const __half2*>(&r)[i]);
+      else p = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&r)[i]);
+      f[2 * i] = p.x;
+      f[2 * i + 1] = p.y;
+    }
   }
 }
 template <typename T>
-AFB_DEV void store8(T* p, const float* f) {
+AFB_DEV Raw<T> pack(const float* f) {
+  Raw<T> r;
   if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    uint4 q;
-    T* h = reinterpret_cast<T*>(&q);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = from_f<T>(f[i]);
-    *reinterpret_cast<uint4*>(p) = q;
+    for (int i = 0; i < 8; ++i) r.v[i] = f[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint32_t*>(&r)[i] = std::is_same<T, __half>::value ? pack_f16x2(f[2 * i], f[2 * i + 1])
+                                                                           : pack_bf16x2(f[2 * i], f[2 * i + 1]);
   }
+  return r;
 }
-// chunk at column c of a row of `width`: elements past the row's end read 0. VEC: width and every row start are
-// multiples of 16 bytes, so a chunk is whole or absent.
+// a CTA's rows at a time: `groups` groups of `wpr` warps
+struct Group {
+  int wpr, lanes, idx, t;  // warps and threads of a group, this thread's group and its place in it
+  AFB_DEV explicit Group(int wpr_) : wpr(wpr_), lanes(wpr_ * 32), idx(threadIdx.x / lanes), t(threadIdx.x - idx * lanes) {}
+};
+// column of element i of a lane's chunk p. VEC (width and every row start are multiples of 16 bytes): eight in a row, so
+// a chunk is whole or absent. Else one by one across the lanes, so that a warp's 2- or 4-byte accesses are contiguous.
+template <bool VEC>
+AFB_DEV int col_of(const Group& g, int p, int i) {
+  return VEC ? (p * g.lanes + g.t) * 8 + i : (p * 8 + i) * g.lanes + g.t;
+}
+// elements past the row's end read 0
 template <bool VEC, typename T>
-AFB_DEV void load_chunk(const T* row, int c, int width, float* f) {
+AFB_DEV Raw<T> load_chunk(const T* row, const Group& g, int p, int width) {
+  Raw<T> r;
   if constexpr (VEC) {
+    const int c = col_of<true>(g, p, 0);
     if (c < width) {
-      load8(row + c, f);
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(&r)[0] = reinterpret_cast<const float4*>(row + c)[0];
+        reinterpret_cast<float4*>(&r)[1] = reinterpret_cast<const float4*>(row + c)[1];
+      } else {
+        *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(row + c);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = 0.f;
+      for (int i = 0; i < 8; ++i) r.v[i] = from_f<T>(0.f);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = c + i < width ? to_f(row[c + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const int c = col_of<false>(g, p, i);
+      r.v[i] = c < width ? row[c] : from_f<T>(0.f);
+    }
   }
+  return r;
 }
 template <bool VEC, typename T>
-AFB_DEV void store_chunk(T* row, int c, int width, const float* f) {
+AFB_DEV void store_chunk(T* row, const Group& g, int p, int width, const float* f) {
   if constexpr (VEC) {
-    if (c < width) store8(row + c, f);
+    const int c = col_of<true>(g, p, 0);
+    if (c < width) {
+      Raw<T> r = pack<T>(f);
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(row + c)[0] = reinterpret_cast<float4*>(&r)[0];
+        reinterpret_cast<float4*>(row + c)[1] = reinterpret_cast<float4*>(&r)[1];
+      } else {
+        *reinterpret_cast<uint4*>(row + c) = *reinterpret_cast<uint4*>(&r);
+      }
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < width) row[c + i] = from_f<T>(f[i]);
+    for (int i = 0; i < 8; ++i) {
+      const int c = col_of<false>(g, p, i);
+      if (c < width) row[c] = from_f<T>(f[i]);
+    }
   }
 }
-// weights: fp32 or the rows' type
+// weights (fp32 or the rows' type) as factors, 0 past the row's end
 template <bool VEC, typename T>
-AFB_DEV void load_weight(const void* w, int w32, int c, int width, float* f) {
-  if (w32) load_chunk<VEC>(reinterpret_cast<const float*>(w), c, width, f);
-  else load_chunk<VEC>(reinterpret_cast<const T*>(w), c, width, f);
+AFB_DEV void load_weight(const void* w, int w32, const Group& g, int p, int width, float* f) {
+  if (w32) unpack(load_chunk<VEC>(reinterpret_cast<const float*>(w), g, p, width), f);
+  else unpack(load_chunk<VEC>(reinterpret_cast<const T*>(w), g, p, width), f);
+}
+template <bool VEC, typename T>
+AFB_DEV void load_factor(const NormArgs& a, const Group& g, int p, float* f) {
+  load_weight<VEC, T>(a.w, a.wtype == ELEM_FP32, g, p, a.width, f);
+  if (a.rms) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = col_of<VEC>(g, p, i) < a.width ? 1.f + f[i] : 0.f;
+  }
 }
 
-// sums over the WPR warps of a row; `red` holds WPR slots per row group, `bar` is the group's named barrier
-template <int WPR>
-AFB_DEV float2 row_sum2(float2 v, float2* red, int wr, int bar) {
+constexpr int MAX_WPR = 32;
+// two sums over the warps of a row. Each warp leaves its sums in a slot and after one barrier adds up all of them;
+// two sets of slots in turn (`ph`) make a second barrier unnecessary: a warp that writes a set again has passed the
+// barrier of the other one, which every warp reaches after its last read of this one.
+struct Slots {
+  float2 v[2][MAX_WPR];
+};
+AFB_DEV float row_sum(float v, Slots& slots, const Group& g, int& ph) {
+  v = warp_sum(v);
+  if (g.wpr > 1) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) slots.v[ph][g.t >> 5].x = v;
+    named_bar_sync(1 + g.idx, g.lanes);
+    v = warp_sum(lane < g.wpr ? slots.v[ph][lane].x : 0.f);
+    ph ^= 1;
+  }
+  return v;
+}
+AFB_DEV float2 row_sum2(float2 v, Slots& slots, const Group& g, int& ph) {
   v.x = warp_sum(v.x);
   v.y = warp_sum(v.y);
-  if constexpr (WPR > 1) {
-    if ((threadIdx.x & 31) == 0) red[wr] = v;
-    named_bar_sync(bar, WPR * 32);
-    v = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < WPR; ++i) {
-      const float2 r = red[i];
-      v.x += r.x;
-      v.y += r.y;
-    }
-    named_bar_sync(bar, WPR * 32);  // the slots may be written again
+  if (g.wpr > 1) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) slots.v[ph][g.t >> 5] = v;
+    named_bar_sync(1 + g.idx, g.lanes);
+    v = lane < g.wpr ? slots.v[ph][lane] : make_float2(0.f, 0.f);
+    v.x = warp_sum(v.x);
+    v.y = warp_sum(v.y);
+    ph ^= 1;
   }
   return v;
 }
 
-template <int WPR>
-struct Block {
-  static constexpr int THREADS = WPR > 8 ? WPR * 32 : 256, GROUPS = THREADS / (WPR * 32);
+// The ring of a group: `depth` slots, a row of x (and of dy) each. A row is copied as the 16-byte blocks that hold it
+// (none of them is without a byte of the row, so none lies outside the allocation).
+constexpr int MAX_DEPTH = 8;
+struct RingShape {
+  int depth, part;  // slots; bytes of one row in a slot: the row rounded up to 16, and 16 more for its offset
+};
+// 16-byte blocks of `bytes` bytes at p
+AFB_DEV uint32_t span(const uint8_t* p, int bytes) {
+  return (uint32_t)(((reinterpret_cast<uintptr_t>(p) & 15) + bytes + 15) & ~uintptr_t(15));
+}
+AFB_DEV const void* block_of(const uint8_t* p) {
+  return reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+}
+// What every thread of a group keeps of its ring: the slot of the row at hand and that slot's parity; and the thread
+// that fetches: the next row to fetch and its place. Counted, not divided: a division would cost as much as an element's
+// arithmetic does.
+template <int PARTS>
+struct Ring {
+  uint8_t *base, *slot;
+  uint64_t *full0, *full;
+  int slot_bytes, part, depth, at;
+  uint32_t parity;
+  const uint8_t *x, *dy;  // the row at hand (PARTS 1: x alone)
+  int64_t x_step, dy_step;
+  int bytes;
+  uint32_t* status;
+
+  AFB_DEV void fetch(uint8_t* dst, uint64_t* bar, const uint8_t* xs, const uint8_t* ds) const {
+    const uint32_t nx = span(xs, bytes), nd = PARTS > 1 ? span(ds, bytes) : 0u;
+    mbar_arrive_expect_tx(bar, nx + nd);
+    bulk_load_1d(dst, block_of(xs), nx, bar);
+    if (PARTS > 1) bulk_load_1d(dst + part, block_of(ds), nd, bar);
+  }
+  AFB_DEV void start(int n) const {  // one thread: the first rows
+    for (int k = 0; k < min(n, depth); ++k)
+      fetch(base + k * slot_bytes, full0 + k, x + k * x_step, PARTS > 1 ? dy + k * dy_step : nullptr);
+  }
+  AFB_DEV bool wait() const { return mbar_wait(full, parity, status); }
+  AFB_DEV void refill() const {  // one thread: the row `depth` further into the slot at hand
+    fetch(slot, full, x + depth * x_step, PARTS > 1 ? dy + depth * dy_step : nullptr);
+  }
+  AFB_DEV void next() {
+    x += x_step;
+    if (PARTS > 1) dy += dy_step;
+    slot += slot_bytes;
+    ++full;
+    if (++at == depth) at = 0, slot = base, full = full0, parity ^= 1;
+  }
 };
 
-template <typename T, int WPR, int NV, bool VEC>
-__global__ void __launch_bounds__(Block<WPR>::THREADS) norm_fwd_kernel(NormArgs a) {
+// a group's threads leave together: one that gave up waiting says so before the row's barrier
+AFB_DEV void group_sync(const Group& g) {
+  if (g.wpr > 1) named_bar_sync(1 + g.idx, g.lanes);
+  else __syncwarp();
+}
+
+template <typename T, int NV, bool VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_fwd_kernel(NormArgs a, int wpr, int groups, RingShape rs) {
+  extern __shared__ __align__(16) uint8_t ring_smem[];
+  __shared__ Slots slots_s[8];
+  __shared__ uint64_t full_s[8][MAX_DEPTH];
+  __shared__ int bad_s[8];
+  const Group g(wpr);
+  Slots& slots = slots_s[g.idx];
+  volatile int* bad = &bad_s[g.idx];
+  if (g.t == 0) {
+    for (int i = 0; i < rs.depth; ++i) mbar_init(&full_s[g.idx][i], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    *bad = 0;
+  }
+  __syncthreads();
   grid_dep_wait();
   grid_dep_trigger();
-  constexpr int G = Block<WPR>::GROUPS;
-  __shared__ float2 red[G][WPR];
-  const int grp = threadIdx.x / (WPR * 32), t = threadIdx.x % (WPR * 32), wr = t >> 5;
-  const int w32 = a.wtype == ELEM_FP32;
+  int ph = 0;
   const float inv = 1.f / a.width;
-  for (int64_t row = (int64_t)blockIdx.x * G + grp; row < a.rows; row += (int64_t)gridDim.x * G) {
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+  const int64_t stride = (int64_t)gridDim.x * groups, row0 = (int64_t)blockIdx.x * groups + g.idx;
+  const int n = row0 < a.rows ? (int)((a.rows - 1 - row0) / stride) + 1 : 0;  // rows of this group
+  Ring<1> ring;
+  ring.part = ring.slot_bytes = rs.part, ring.depth = rs.depth, ring.at = 0, ring.parity = 0, ring.status = a.status;
+  ring.base = ring.slot = ring_smem + (size_t)g.idx * rs.depth * rs.part;
+  ring.full0 = ring.full = full_s[g.idx];
+  ring.bytes = a.width * (int)sizeof(T);
+  ring.x = reinterpret_cast<const uint8_t*>(reinterpret_cast<const T*>(a.x) + row0 * a.ldx);
+  ring.x_step = stride * a.ldx * (int64_t)sizeof(T);
+  if (g.t == 0) ring.start(n);
+  float m[NV][8], b[NV][8];
+#pragma unroll
+  for (int p = 0; p < NV; ++p) {
+    load_factor<VEC, T>(a, g, p, m[p]);
+    if (a.b) {
+      load_weight<VEC, T>(a.b, a.wtype == ELEM_FP32, g, p, a.width, b[p]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) b[p][i] = 0.f;
+    }
+  }
+  T* y = reinterpret_cast<T*>(a.y) + row0 * a.width;
+  int k = 0;
+  for (; k < n; ++k, ring.next(), y += stride * a.width) {
+    if (!ring.wait()) *bad = 1;
+    const T* x = reinterpret_cast<const T*>(ring.slot + (VEC ? 0 : reinterpret_cast<uintptr_t>(ring.x) & 15));
     float v[NV][8];
 #pragma unroll
-    for (int p = 0; p < NV; ++p) load_chunk<VEC>(x, (p * WPR * 32 + t) * 8, a.width, v[p]);
+    for (int p = 0; p < NV; ++p) unpack(load_chunk<VEC>(x, g, p, a.width), v[p]);
+    group_sync(g);  // the slot has been read
+    if (*bad) break;
+    if (g.t == 0 && k + rs.depth < n) ring.refill();
     float mean = 0.f;
     if (!a.rms) {
       float s = 0.f;
@@ -135,90 +288,120 @@ __global__ void __launch_bounds__(Block<WPR>::THREADS) norm_fwd_kernel(NormArgs 
       for (int p = 0; p < NV; ++p)
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += v[p][i];
-      mean = row_sum2<WPR>(make_float2(s, 0.f), red[grp], wr, 1 + grp).x * inv;
+      mean = row_sum(s, slots, g, ph) * inv;
+#pragma unroll
+      for (int p = 0; p < NV; ++p)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[p][i] -= mean;
     }
     float q = 0.f;
 #pragma unroll
-    for (int p = 0; p < NV; ++p)
+    for (int p = 0; p < NV; ++p) {
+      if (VEC && col_of<VEC>(g, p, 0) >= a.width) continue;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[p][i] - mean;
-        if ((p * WPR * 32 + t) * 8 + i < a.width) q += d * d;
-      }
-    const float rstd = rsqrtf(row_sum2<WPR>(make_float2(q, 0.f), red[grp], wr, 1 + grp).x * inv + a.eps);
-    if (t == 0) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
+      for (int i = 0; i < 8; ++i)
+        if (VEC || col_of<VEC>(g, p, i) < a.width) q += v[p][i] * v[p][i];
     }
-    T* y = reinterpret_cast<T*>(a.y) + row * a.width;
+    const float rstd = rsqrtf(row_sum(q, slots, g, ph) * inv + a.eps);
+    if (g.t == 0) {
+      if (a.mean) a.mean[row0 + k * stride] = mean;
+      if (a.rstd) a.rstd[row0 + k * stride] = rstd;
+    }
 #pragma unroll
     for (int p = 0; p < NV; ++p) {
-      const int c = (p * WPR * 32 + t) * 8;
-      float w[8], b[8];
-      load_weight<VEC, T>(a.w, w32, c, a.width, w);
-      if (a.b) load_weight<VEC, T>(a.b, w32, c, a.width, b);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float xh = (v[p][i] - mean) * rstd;
-        v[p][i] = a.rms ? xh * (1.f + w[i]) : (a.b ? xh * w[i] + b[i] : xh * w[i]);
-      }
-      store_chunk<VEC>(y, c, a.width, v[p]);
+      for (int i = 0; i < 8; ++i) v[p][i] = v[p][i] * rstd * m[p][i] + b[p][i];
+      store_chunk<VEC>(y, g, p, a.width, v[p]);
     }
   }
+  if (k < n && g.t == 0)  // after a failed wait: the copies in flight land first
+    for (int j = k; j < min(n, k + rs.depth); ++j, ring.next()) ring.wait();
 }
 
-template <typename T, int WPR, int NV, bool VEC>
-__global__ void __launch_bounds__(Block<WPR>::THREADS) norm_bwd_kernel(NormArgs a) {
+template <typename T, int NV, bool VEC, int MAXT, int MINB = 1>
+__global__ void __launch_bounds__(MAXT, MINB) norm_bwd_kernel(NormArgs a, int wpr, int groups, RingShape rs) {
+  extern __shared__ __align__(16) uint8_t ring_smem[];
+  __shared__ Slots slots_s[8];
+  __shared__ uint64_t full_s[8][MAX_DEPTH];
+  __shared__ int bad_s[8];
+  __shared__ float comb[256 * 8];  // more than one group: 256 threads at most
+  const Group g(wpr);
+  Slots& slots = slots_s[g.idx];
+  volatile int* bad = &bad_s[g.idx];
+  if (g.t == 0) {
+    for (int i = 0; i < rs.depth; ++i) mbar_init(&full_s[g.idx][i], 1);
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    *bad = 0;
+  }
+  __syncthreads();
   grid_dep_wait();
   grid_dep_trigger();
-  constexpr int G = Block<WPR>::GROUPS;
-  __shared__ float2 red[G][WPR];
-  __shared__ float comb[G > 1 ? Block<WPR>::THREADS * 8 : 1];
-  const int grp = threadIdx.x / (WPR * 32), t = threadIdx.x % (WPR * 32), wr = t >> 5;
-  const int w32 = a.wtype == ELEM_FP32;
+  int ph = 0;
   const float inv = 1.f / a.width;
+  const int lane = threadIdx.x & 31;
   float dw[NV][8] = {}, db[NV][8] = {};
-  for (int64_t row = (int64_t)blockIdx.x * G + grp; row < a.rows; row += (int64_t)gridDim.x * G) {
-    const T* x = reinterpret_cast<const T*>(a.x) + row * a.ldx;
-    const T* dy = reinterpret_cast<const T*>(a.dy) + row * a.width;
-    const float rstd = a.rstd[row], mean = a.rms ? 0.f : a.mean[row];
-    float xh[NV][8], v[NV][8];
+  const int64_t stride = (int64_t)gridDim.x * groups, row0 = (int64_t)blockIdx.x * groups + g.idx;
+  const int n = row0 < a.rows ? (int)((a.rows - 1 - row0) / stride) + 1 : 0;
+  Ring<2> ring;
+  ring.part = rs.part, ring.slot_bytes = 2 * rs.part, ring.depth = rs.depth, ring.at = 0, ring.parity = 0;
+  ring.base = ring.slot = ring_smem + (size_t)g.idx * rs.depth * rs.part * 2;
+  ring.full0 = ring.full = full_s[g.idx];
+  ring.bytes = a.width * (int)sizeof(T), ring.status = a.status;
+  ring.x = reinterpret_cast<const uint8_t*>(reinterpret_cast<const T*>(a.x) + row0 * a.ldx);
+  ring.dy = reinterpret_cast<const uint8_t*>(reinterpret_cast<const T*>(a.dy) + row0 * a.width);
+  ring.x_step = stride * a.ldx * (int64_t)sizeof(T);
+  ring.dy_step = stride * a.width * (int64_t)sizeof(T);
+  if (g.t == 0) ring.start(n);
+  float m[NV][8];
+#pragma unroll
+  for (int p = 0; p < NV; ++p) load_factor<VEC, T>(a, g, p, m[p]);
+  float my_rstd = 0.f, my_mean = 0.f;  // of 32 rows, one a lane
+  T* dx = reinterpret_cast<T*>(a.dx) + row0 * a.width;
+  int k = 0;
+  for (; k < n; ++k, ring.next(), dx += stride * a.width) {
+    if ((k & 31) == 0 && k + lane < n) {
+      my_rstd = a.rstd[row0 + (k + lane) * stride];
+      if (!a.rms) my_mean = a.mean[row0 + (k + lane) * stride];
+    }
+    if (!ring.wait()) *bad = 1;
+    const T* x = reinterpret_cast<const T*>(ring.slot + (VEC ? 0 : reinterpret_cast<uintptr_t>(ring.x) & 15));
+    const T* dy = reinterpret_cast<const T*>(ring.slot + rs.part + (VEC ? 0 : reinterpret_cast<uintptr_t>(ring.dy) & 15));
+    float h[NV][8], v[NV][8];
+#pragma unroll
+    for (int p = 0; p < NV; ++p) {
+      unpack(load_chunk<VEC>(x, g, p, a.width), h[p]);
+      unpack(load_chunk<VEC>(dy, g, p, a.width), v[p]);
+    }
+    group_sync(g);  // the slot has been read
+    if (*bad) break;
+    if (g.t == 0 && k + rs.depth < n) ring.refill();
+    const float r = __shfl_sync(0xffffffffu, my_rstd, k & 31), mu = __shfl_sync(0xffffffffu, my_mean, k & 31);
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int p = 0; p < NV; ++p) {
-      const int c = (p * WPR * 32 + t) * 8;
-      load_chunk<VEC>(x, c, a.width, xh[p]);
-      load_chunk<VEC>(dy, c, a.width, v[p]);
-    }
+    for (int p = 0; p < NV; ++p)
 #pragma unroll
-    for (int p = 0; p < NV; ++p) {
-      const int c = (p * WPR * 32 + t) * 8;
-      float w[8];
-      load_weight<VEC, T>(a.w, w32, c, a.width, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[p][i], h = (xh[p][i] - mean) * rstd;  // past the row's end d and so v are 0
-        dw[p][i] += d * h;
-        db[p][i] += d;
-        xh[p][i] = h;
-        v[p][i] = c + i < a.width ? d * (a.rms ? 1.f + w[i] : w[i]) : 0.f;
-        s.x += v[p][i] * h;
+      for (int i = 0; i < 8; ++i) {  // past the row's end dy and the factor are 0, and so is what they enter
+        h[p][i] = (h[p][i] - mu) * r;
+        dw[p][i] += v[p][i] * h[p][i];
+        db[p][i] += v[p][i];
+        v[p][i] *= m[p][i];
+        s.x += v[p][i] * h[p][i];
         s.y += v[p][i];
       }
-    }
     if (a.dx) {
-      s = row_sum2<WPR>(s, red[grp], wr, 1 + grp);
+      s = row_sum2(s, slots, g, ph);
       const float m1 = s.x * inv, m0 = a.rms ? 0.f : s.y * inv;
-      T* dx = reinterpret_cast<T*>(a.dx) + row * a.width;
 #pragma unroll
       for (int p = 0; p < NV; ++p) {
-        float o[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = rstd * (v[p][i] - m0 - xh[p][i] * m1);
-        store_chunk<VEC>(dx, (p * WPR * 32 + t) * 8, a.width, o);
+        for (int i = 0; i < 8; ++i) v[p][i] = r * (v[p][i] - m0 - h[p][i] * m1);
+        store_chunk<VEC>(dx, g, p, a.width, v[p]);
       }
     }
   }
+  if (k < n && g.t == 0)  // after a failed wait: the copies in flight land first
+    for (int j = k; j < min(n, k + rs.depth); ++j, ring.next()) ring.wait();
   if (!a.dw && !a.db) return;
   float* out = a.partial + (int64_t)blockIdx.x * 2 * a.width;
 #pragma unroll
@@ -226,44 +409,42 @@ __global__ void __launch_bounds__(Block<WPR>::THREADS) norm_bwd_kernel(NormArgs 
     float(*acc)[8] = k ? db : dw;
 #pragma unroll
     for (int p = 0; p < NV; ++p) {
-      const int c = (p * WPR * 32 + t) * 8;
-      if constexpr (G > 1) {  // the CTA's row groups, in order
+      if (groups > 1) {  // the CTA's row groups, in order
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) comb[(i * G + grp) * WPR * 32 + t] = acc[p][i];
+        for (int i = 0; i < 8; ++i) comb[(i * groups + g.idx) * g.lanes + g.t] = acc[p][i];
         __syncthreads();
-        if (grp == 0) {
+        if (g.idx == 0) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             float f = 0.f;
-#pragma unroll
-            for (int j = 0; j < G; ++j) f += comb[(i * G + j) * WPR * 32 + t];
+            for (int j = 0; j < groups; ++j) f += comb[(i * groups + j) * g.lanes + g.t];
             acc[p][i] = f;
           }
         }
       }
-      if (grp == 0) store_chunk<false>(out + k * a.width, c, a.width, acc[p]);
+      if (g.idx == 0) store_chunk<VEC>(out + k * a.width, g, p, a.width, acc[p]);
     }
   }
 }
 
-// column sums of the partial rows: CTA of 32 columns x 8 row lanes
+// column sums of the partial rows: CTA of 32 columns x 32 row lanes
 template <typename T>
-__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* __restrict__ part, int n, int width,
+__global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restrict__ part, int n, int width,
                                                           void* __restrict__ dw, void* __restrict__ db, int w32) {
   grid_dep_wait();
-  __shared__ float red[8][33];
+  __shared__ float red[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int col = blockIdx.x * 32 + cx;  // over [dw | db]
   float s = 0.f;
   if (col < 2 * width)
-    for (int r = ry; r < n; r += 8) s += part[(int64_t)r * 2 * width + col];
+    for (int r = ry; r < n; r += 32) s += part[(int64_t)r * 2 * width + col];
   red[ry][cx] = s;
   __syncthreads();
   if (ry || col >= 2 * width) return;
   float f = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f += red[j][cx];
+  for (int j = 0; j < 32; ++j) f += red[j][cx];
   void* out = col < width ? dw : db;
   const int c = col < width ? col : col - width;
   if (!out) return;
@@ -274,64 +455,99 @@ __global__ void __launch_bounds__(256) norm_reduce_kernel(const float* __restric
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 static bool vec_ok(const NormArgs& a) {
   return a.width % 8 == 0 && a.ldx % 8 == 0 && aligned16(a.x) && aligned16(a.y) && aligned16(a.w) && aligned16(a.b) &&
-         aligned16(a.dy) && aligned16(a.dx);
+         aligned16(a.dy) && aligned16(a.dx) && aligned16(a.partial);
 }
 
 struct Shape {
-  int wpr, nv;
+  int nv, wpr, groups, grid;
+  RingShape ring;
+  int smem;
 };
-// warps per row and chunks per lane: at most 4 chunks (32 elements) a lane, so a backward row and its two sums stay
-// in registers
-static Shape shape_of(const NormArgs& a) {
-  const int chunks = (a.width + 7) / 8;
-  int wpr = 1;
-  while (wpr < 16 && chunks > wpr * 32 * 4) wpr *= 2;
-  int nv = (chunks + wpr * 32 - 1) / (wpr * 32);
-  if (!vec_ok(a)) nv = 4;  // one unaligned variant for each row size
-  return {wpr, nv};
-}
-static int grid_of(const NormArgs& a, const Shape& s, int num_sms, int per_sm) {
-  const int groups = s.wpr > 8 ? 1 : 8 / s.wpr;
-  const int64_t blocks = (a.rows + groups - 1) / groups;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)num_sms * per_sm));
-}
-constexpr int FWD_PER_SM = 8, BWD_PER_SM = 2;
+using Kernel = void (*)(NormArgs, int, int, RingShape);
 
-template <typename T, int WPR, int NV, bool VEC>
-static int run_fwd(const NormArgs& a, int grid, cudaStream_t st) {
-  return launch_pdl(norm_fwd_kernel<T, WPR, NV, VEC>, dim3(grid), dim3(Block<WPR>::THREADS), 0, st, a);
+template <typename T, bool BWD, int NV>
+static Kernel kernel_of(bool vec, int wpr) {
+  if constexpr (BWD && NV == 3) {
+    return vec ? norm_bwd_kernel<T, 3, true, 192, 2> : norm_bwd_kernel<T, 3, false, 192, 2>;
+  } else if constexpr (BWD) {
+    if (wpr > 8) return vec ? norm_bwd_kernel<T, NV, true, 512> : norm_bwd_kernel<T, NV, false, 512>;
+    return vec ? norm_bwd_kernel<T, NV, true, 256> : norm_bwd_kernel<T, NV, false, 256>;
+  } else {
+    if (wpr > 8) return vec ? norm_fwd_kernel<T, NV, true, 512> : norm_fwd_kernel<T, NV, false, 512>;
+    return vec ? norm_fwd_kernel<T, NV, true, 256> : norm_fwd_kernel<T, NV, false, 256>;
+  }
 }
-template <typename T, int WPR, int NV, bool VEC>
-static int run_bwd(const NormArgs& a, int grid, cudaStream_t st) {
-  return launch_pdl(norm_bwd_kernel<T, WPR, NV, VEC>, dim3(grid), dim3(Block<WPR>::THREADS), 0, st, a);
+template <typename T, bool BWD>
+static Kernel kernel_of(int nv, bool vec, int wpr) {
+  switch (nv) {
+    case 1: return kernel_of<T, BWD, 1>(vec, wpr);
+    case 2: return kernel_of<T, BWD, 2>(vec, wpr);
+    case 3: return kernel_of<T, BWD, 3>(vec, wpr);
+    default: return kernel_of<T, BWD, 4>(vec, wpr);
+  }
+}
+
+constexpr int RING_SMEM = 180 * 1024;  // of an SM; the kernels' static shared memory is below 16 KB a CTA
+
+// Chunks a lane, warps a row, rows a CTA, CTAs, ring. Forward, the instructions a row takes decide the first two: some 8
+// an element and 75 a warp for its sums, so few warps with much each, as far as the lanes' last chunks are not left
+// idle. Backward, two chunks a lane (16,384 rows of 2,048 in bf16: 46 us; one chunk 61, for the sums of twice the warps;
+// three 70 and four 65, for want of registers), one where a row is 512 columns or less, four where it passes 8,192, and
+// three from 4,097 to 4,608, where two would leave an SM one CTA.
+// CTAs: as many as are resident (a second wave would wait for the first). The ring takes what shared memory the SM's
+// CTAs leave each other, up to 8 rows.
+template <typename T, bool BWD>
+static int plan(const NormArgs& a, int num_sms, Shape& s, Kernel& kern) {
+  const int chunks = (a.width + 7) / 8;
+  auto warps_of = [&](int nv) { return (chunks + 32 * nv - 1) / (32 * nv); };
+  if (BWD) {
+    s.nv = chunks <= 64 ? 1 : warps_of(2) > 8 && warps_of(3) <= 6 ? 3 : warps_of(2) <= 16 ? 2 : 4;
+  } else {
+    int best = INT32_MAX;
+    for (int nv = 1; nv <= 4; ++nv) {
+      const int cost = warps_of(nv) * (nv * 8 * 8 + 75);
+      if (warps_of(nv) <= 16 && cost < best) best = cost, s.nv = nv;
+    }
+  }
+  s.wpr = warps_of(s.nv);
+  s.groups = std::max(1, 4 / s.wpr);
+  const int warps = s.groups * s.wpr;
+  kern = kernel_of<T, BWD>(s.nv, vec_ok(a), s.wpr);
+  // resident CTAs by registers, asked for once a kernel and CTA size
+  static std::atomic<int> resident[4][2][17];
+  std::atomic<int>& r = resident[s.nv - 1][vec_ok(a)][warps];
+  int per_sm = r.load(std::memory_order_relaxed);
+  if (!per_sm) {
+    cudaError_t e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_SMEM);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, warps * 32, 0);
+    if (e != cudaSuccess) return (int)e;
+    per_sm = std::max(1, std::min(per_sm, 8));
+    r.store(per_sm, std::memory_order_relaxed);
+  }
+  const int64_t blocks = (a.rows + s.groups - 1) / s.groups;
+  s.ring.part = (a.width * (int)sizeof(T) + 15) / 16 * 16 + 16;
+  const int slot = s.ring.part * (BWD ? 2 : 1) * s.groups;
+  per_sm = std::max(1, std::min(per_sm, RING_SMEM / slot));
+  s.grid = (int)std::max<int64_t>(1, std::min(blocks, (int64_t)num_sms * per_sm));
+  s.ring.depth = std::max(1, std::min(MAX_DEPTH, RING_SMEM / per_sm / slot));
+  s.smem = s.ring.depth * slot;
+  return 0;
 }
 
 template <typename T, bool BWD>
 static int dispatch(const NormArgs& a, int num_sms, cudaStream_t st) {
-  const Shape s = shape_of(a);
-  const int grid = grid_of(a, s, num_sms, BWD ? BWD_PER_SM : FWD_PER_SM);
-  const bool vec = vec_ok(a);
-#define AFB_NORM(W, N, V) \
-  if (s.wpr == W && s.nv == N && vec == V) return BWD ? run_bwd<T, W, N, V>(a, grid, st) : run_fwd<T, W, N, V>(a, grid, st);
-  AFB_NORM(1, 1, true)
-  AFB_NORM(1, 2, true)
-  AFB_NORM(1, 3, true)
-  AFB_NORM(1, 4, true)
-  AFB_NORM(2, 3, true)
-  AFB_NORM(2, 4, true)
-  AFB_NORM(4, 3, true)
-  AFB_NORM(4, 4, true)
-  AFB_NORM(8, 3, true)
-  AFB_NORM(8, 4, true)
-  AFB_NORM(16, 3, true)
-  AFB_NORM(16, 4, true)
-  AFB_NORM(1, 4, false)
-  AFB_NORM(2, 4, false)
-  AFB_NORM(4, 4, false)
-  AFB_NORM(8, 4, false)
-  AFB_NORM(16, 4, false)
-#undef AFB_NORM
-  return 3;
+  Shape s;
+  Kernel kern;
+  if (const int e = plan<T, BWD>(a, num_sms, s, kern)) return e;
+  static std::atomic<uint64_t> devs[4][2][17];
+  if (const int e = smem_attr_once(devs[s.nv - 1][vec_ok(a)][s.groups * s.wpr], (const void*)kern, RING_SMEM)) return e;
+  return launch_pdl(kern, dim3(s.grid), dim3(s.groups * s.wpr * 32), s.smem, st, a, s.wpr, s.groups, s.ring);
+}
+template <typename T>
+static int partials(const NormArgs& a, int num_sms) {
+  Shape s;
+  Kernel kern;
+  return plan<T, true>(a, num_sms, s, kern) ? 0 : s.grid;
 }
 
 static bool valid(const NormArgs& a) {
@@ -342,7 +558,8 @@ static bool valid(const NormArgs& a) {
 }  // namespace norm
 
 int norm_bwd_partials(const NormArgs& a, int num_sms) {
-  return norm::grid_of(a, norm::shape_of(a), num_sms, norm::BWD_PER_SM);
+  if (a.dtype == ELEM_BF16) return norm::partials<__nv_bfloat16>(a, num_sms);
+  return a.dtype == ELEM_FP16 ? norm::partials<__half>(a, num_sms) : norm::partials<float>(a, num_sms);
 }
 
 int norm_fwd(const NormArgs& a, int num_sms, cudaStream_t st) {
@@ -356,20 +573,21 @@ int norm_fwd(const NormArgs& a, int num_sms, cudaStream_t st) {
 int norm_bwd(const NormArgs& a, int num_sms, cudaStream_t st) {
   if (!norm::valid(a)) return 3;
   if (a.rows == 0) return 0;  // the caller zeroes dw and db
+  if ((a.dw || a.db) && a.partials != norm_bwd_partials(a, num_sms)) return 4;
   int rc;
   if (a.dtype == ELEM_BF16) rc = norm::dispatch<__nv_bfloat16, true>(a, num_sms, st);
   else if (a.dtype == ELEM_FP16) rc = norm::dispatch<__half, true>(a, num_sms, st);
   else rc = norm::dispatch<float, true>(a, num_sms, st);
   if (rc || (!a.dw && !a.db)) return rc;
   const dim3 grid((2 * a.width + 31) / 32);
-  const int n = norm_bwd_partials(a, num_sms), w32 = a.wtype == ELEM_FP32;
+  const int n = a.partials, w32 = a.wtype == ELEM_FP32;
   if (a.dtype == ELEM_BF16)
-    return launch_pdl(norm::norm_reduce_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, (const float*)a.partial, n,
+    return launch_pdl(norm::norm_reduce_kernel<__nv_bfloat16>, grid, dim3(1024), 0, st, (const float*)a.partial, n,
                       a.width, a.dw, a.db, w32);
   if (a.dtype == ELEM_FP16)
-    return launch_pdl(norm::norm_reduce_kernel<__half>, grid, dim3(256), 0, st, (const float*)a.partial, n, a.width,
+    return launch_pdl(norm::norm_reduce_kernel<__half>, grid, dim3(1024), 0, st, (const float*)a.partial, n, a.width,
                       a.dw, a.db, w32);
-  return launch_pdl(norm::norm_reduce_kernel<float>, grid, dim3(256), 0, st, (const float*)a.partial, n, a.width,
+  return launch_pdl(norm::norm_reduce_kernel<float>, grid, dim3(1024), 0, st, (const float*)a.partial, n, a.width,
                     a.dw, a.db, w32);
 }
 
