@@ -636,7 +636,6 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
   grid_dep_wait();
   if (threadIdx.x == 0) grid_dep_trigger();
 
-  bool ok = true;
   if (warp == 0) {
     if (lane == 0) {
       int issued = 0;
@@ -669,25 +668,29 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
   } else {
     // partial sums to shared memory (the ring is free: every MMA has read it): [NA][T][128]
     const int quad = warp & 3;
-    ok = mbar_wait(done, 0, status);
+    mbar_wait(done, 0, status);  // (a wait that gives up is in the status word)
     tc_fence_after();
     const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16);
     float* p = reinterpret_cast<float*>(smem) + quad * 32 + lane;
+    constexpr int CW = NT < 32 ? NT : 32;  // columns at a time
 #pragma unroll 1
-    for (int c = 0; c < NT; c += 16) {
-      if (c >= g.T) break;
-      float v[16], w[16];
-      tmem_ld16(taddr + c, v);
-      tmem_ld16(taddr + NT + c, w);  // DUAL: up; else the second term of h
+    for (int c = 0; c < g.T; c += CW) {
+      float v[CW], w[CW];
+      if constexpr (CW == 16) {
+        tmem_ld16(taddr + c, v);
+        tmem_ld16(taddr + NT + c, w);  // DUAL: up; else the second term of h
+      } else {
+        tmem_ld32(taddr + c, v);
+        tmem_ld32(taddr + NT + c, w);
+      }
       tmem_ld_wait();
+      const int n = g.T - c;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        if (c + j >= g.T) break;
+      for (int j = 0; j < CW; ++j) {
         if constexpr (DUAL_) {
-          p[(c + j) * 128] = v[j];
-          p[(g.T + c + j) * 128] = w[j];
+          if (j < n) p[(c + j) * 128] = v[j], p[(g.T + c + j) * 128] = w[j];
         } else {
-          p[(c + j) * 128] = v[j] + w[j];
+          if (j < n) p[(c + j) * 128] = v[j] + w[j];
         }
       }
     }
@@ -695,50 +698,54 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
   }
   __syncthreads();
   cluster_sync();
-  if (warp >= 2 && ok) {
+  {
     uint32_t part[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) part[c] = cluster_addr(smem, min(c, C - 1));
+    // four weight rows of one row: the cluster's partial sums in their order, all on the way at once
     auto sum = [&](uint32_t off) {
-      float2 s = ld_cluster_f2(part[0] + off);
+      float4 q[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < C) q[c] = ld_cluster_f4(part[c] + off);
+      float4 s = q[0];
 #pragma unroll
       for (int c = 1; c < 8; ++c)
-        if (c < C) {
-          const float2 q = ld_cluster_f2(part[c] + off);
-          s.x += q.x;
-          s.y += q.y;
-        }
+        if (c < C) s.x += q[c].x, s.y += q[c].y, s.z += q[c].z, s.w += q[c].w;
       return s;
     };
-    const int pairs = g.T * 64;  // (row, two weight rows), dealt to the cluster's epilogue threads
-    for (int e = rank * 128 + (threadIdx.x - 64); e < pairs; e += C * 128) {
-      const int t = e >> 6, f = (e & 63) * 2, col = w0 + f;
+    const int quads = g.T * 32;  // (row, four weight rows), dealt to the cluster's threads
+#pragma unroll 1
+    for (int e = rank * 192 + threadIdx.x; e < quads; e += C * 192) {
+      const int t = e >> 5, f = (e & 31) * 4, col = w0 + f;
       if (col >= g.n) continue;
-      float2 a = sum((t * 128 + f) * 4);
+      float4 a = sum((t * 128 + f) * 4);
       if constexpr (DUAL_) {
-        const float2 u = sum(((g.T + t) * 128 + f) * 4);
+        const float4 u = sum(((g.T + t) * 128 + f) * 4);
         if (g.gu) {
-          *reinterpret_cast<float2*>(g.gu + at_gu(t, col, g.F, 0)) = a;
-          *reinterpret_cast<float2*>(g.gu + at_gu(t, col, g.F, 1)) = u;
+          *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 0)) = a;
+          *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 1)) = u;
         }
         with_act(g.act, [&](auto A) {
-          a = make_float2(act_only<A.value>(a.x) * u.x, act_only<A.value>(a.y) * u.y);
+          a = make_float4(act_only<A.value>(a.x) * u.x, act_only<A.value>(a.y) * u.y, act_only<A.value>(a.z) * u.z,
+                          act_only<A.value>(a.w) * u.w);
         });
-        uint32_t* h = reinterpret_cast<uint32_t*>(g.out);
-        const uint32_t hi = pack2<F16>(a.x, a.y);
-        const float2 r = unpack2<F16>(hi);
-        const int64_t at = ((int64_t)t * g.F + col) >> 1;
-        h[at] = hi;
-        h[at + ((int64_t)g.T * g.F >> 1)] =
-            pack2<F16>(isfinite(r.x) ? a.x - r.x : 0.f, isfinite(r.y) ? a.y - r.y : 0.f);
+        const uint2 hi = make_uint2(pack2<F16>(a.x, a.y), pack2<F16>(a.z, a.w));
+        const float2 r0 = unpack2<F16>(hi.x), r1 = unpack2<F16>(hi.y);
+        const uint2 lo = make_uint2(
+            pack2<F16>(isfinite(r0.x) ? a.x - r0.x : 0.f, isfinite(r0.y) ? a.y - r0.y : 0.f),
+            pack2<F16>(isfinite(r1.x) ? a.z - r1.x : 0.f, isfinite(r1.y) ? a.w - r1.y : 0.f));
+        uint16_t* h = reinterpret_cast<uint16_t*>(g.out) + (int64_t)t * g.F + col;
+        *reinterpret_cast<uint2*>(h) = hi;
+        *reinterpret_cast<uint2*>(h + (int64_t)g.T * g.F) = lo;
       } else {
         if (g.residual) {
-          const float2 r = unpack2<F16>(*reinterpret_cast<const uint32_t*>(
-              reinterpret_cast<const uint16_t*>(g.residual) + t * g.ldr + col));
-          a.x += r.x;
-          a.y += r.y;
+          const uint2 q = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(g.residual) + t * g.ldr + col);
+          const float2 r0 = unpack2<F16>(q.x), r1 = unpack2<F16>(q.y);
+          a.x += r0.x, a.y += r0.y, a.z += r1.x, a.w += r1.y;
         }
-        reinterpret_cast<uint32_t*>(g.out)[((int64_t)t * g.n + col) >> 1] = pack2<F16>(a.x, a.y);
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(g.out) + (int64_t)t * g.n + col) =
+            make_uint2(pack2<F16>(a.x, a.y), pack2<F16>(a.z, a.w));
       }
     }
   }
@@ -751,8 +758,7 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
 }
 
 template <bool DUAL_, int NT, bool F16>
-static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArgs& g, int num_sms, uint32_t* status,
-                      cudaStream_t st) {
+static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArgs& g, uint32_t* status, cudaStream_t st) {
   using S = Few<DUAL_, NT>;
   CUtensorMap tw, tx;
   int rc = make_tmap_2d(&tw, w.p, 2, g.K, w_rows, w.ld * 2, BK, 128, 1);
@@ -760,36 +766,57 @@ static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArg
   if (rc) return 5000 + rc;
   auto kern = ffn_few_kernel<DUAL_, NT, F16>;
   static std::atomic<uint64_t> devs{0};
-  if (const int e = smem_attr_once(devs, (const void*)kern, S::TOTAL)) return e;
-  // CTAs of a cluster: enough to cover the SMs (twice where two fit), at least two K blocks each
-  const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK, want = num_sms * (NT <= 32 ? 2 : 1);
-  const int C = std::max(1, std::min({8, want / tiles, kb / 2}));
+  if (const int err = smem_attr_once(devs, (const void*)kern, S::TOTAL)) return err;
+  const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(C, tiles);
   cfg.blockDim = dim3(192);
   cfg.dynamicSmemBytes = S::TOTAL;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
+  // CTAs of a cluster: as many of 8, 4, 2 or 1 as leave each two K blocks and all clusters resident at once (a cluster
+  // that has to wait for another costs the kernel's time again: at 64 rows 48 clusters of 4 take 25 us, 48 of 2 take
+  // 18). How many are resident is asked for once a kernel, size and device.
+  static std::atomic<int> resident[64][4];
+  int dev = 0, C = 1;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  for (int i = 3; i > 0; --i) {
+    if (kb / (1 << i) < 2) continue;
+    int clusters = resident[dev & 63][i].load(std::memory_order_relaxed);
+    if (!clusters) {
+      at[0].val.clusterDim = {1u << i, 1, 1};
+      cfg.gridDim = dim3(1 << i, 1), cfg.attrs = at, cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
+      if (e != cudaSuccess) return (int)e;
+      clusters = std::max(clusters * (NT <= 32 ? 2 : 1), 1);  // (counted at one CTA an SM)
+      resident[dev & 63][i].store(clusters, std::memory_order_relaxed);
+    }
+    if (tiles <= clusters) {
+      C = 1 << i;
+      break;
+    }
+  }
+  cfg.gridDim = dim3(C, tiles);
   at[0].val.clusterDim = {(unsigned)C, 1, 1};
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, g, status);
+  e = cudaLaunchKernelEx(&cfg, kern, tw, tx, g, status);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
 }
 
 template <int NT, bool F16>
-static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, int num_sms,
-                   uint32_t* status, cudaStream_t st) {
+static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, uint32_t* status,
+                   cudaStream_t st) {
   FewArgs g;
   g.T = (int)s.T, g.n = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.out = h, g.gu = gu;
-  const int rc = launch_few<true, NT, F16>(w13, 2 * (int64_t)s.F, x, s.T, g, num_sms, status, st);
+  const int rc = launch_few<true, NT, F16>(w13, 2 * (int64_t)s.F, x, s.T, g, status, st);
   if (rc) return rc;
   g = FewArgs();
   g.T = (int)s.T, g.n = s.N, g.K = s.F, g.out = y, g.residual = residual.p, g.ldr = residual.ld;
-  return launch_few<false, NT, F16>(w2, s.N, {h, s.F}, 2 * s.T, g, num_sms, status, st);
+  return launch_few<false, NT, F16>(w2, s.N, {h, s.F}, 2 * s.T, g, status, st);
 }
 
 static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {
@@ -802,7 +829,7 @@ static int fwd(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h,
                int num_sms, uint32_t* status, cudaStream_t st) {
   if (s.T <= FEW) {
     auto f = s.T <= 16 ? fwd_few<16, F16> : s.T <= 32 ? fwd_few<32, F16> : s.T <= 64 ? fwd_few<64, F16> : fwd_few<128, F16>;
-    return f(s, x, w13, w2, residual, h, gu, y, num_sms, status, st);
+    return f(s, x, w13, w2, residual, h, gu, y, status, st);
   }
   Maps maps;
   Args g;
