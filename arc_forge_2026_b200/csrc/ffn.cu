@@ -573,6 +573,7 @@ struct Few {
 };
 struct FewArgs {
   int T = 0, n = 0;  // rows; weight rows (DUAL: F)
+  int chunk = 0;     // rows of a CTA (gridDim.z chunks)
   int K = 0, F = 0, act = 0;
   void* out = nullptr;             // DUAL: h [2T, F]; else y [T, n]
   float* gu = nullptr;             // DUAL: g and u (at_gu) or null
@@ -594,6 +595,7 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int C = gridDim.x, rank = blockIdx.x, w0 = blockIdx.y * 128;
+  const int t0 = blockIdx.z * g.chunk, rows = min(g.chunk, g.T - t0);
   const int kb_total = (g.K + BK - 1) / BK, kb0 = kb_total * rank / C, num_kb = kb_total * (rank + 1) / C - kb0;
   constexpr uint32_t TMEM_COLS = 2 * NT;
 
@@ -608,8 +610,8 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
   };
   auto load_x = [&](int i) {
     uint8_t* b = smem + (i % STAGES) * S::STAGE + S::NA * 16384;
-    tma_load_2d(b, &tm_x, &full[i % STAGES], (kb0 + i) * BK, 0);
-    if constexpr (!DUAL_) tma_load_2d(b + NT * 128, &tm_x, &full[i % STAGES], (kb0 + i) * BK, g.T);
+    tma_load_2d(b, &tm_x, &full[i % STAGES], (kb0 + i) * BK, t0);
+    if constexpr (!DUAL_) tma_load_2d(b + NT * 128, &tm_x, &full[i % STAGES], (kb0 + i) * BK, g.T + t0);
   };
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -666,7 +668,7 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
       umma_commit(done);
     }
   } else {
-    // partial sums to shared memory (the ring is free: every MMA has read it): [NA][T][128]
+    // partial sums to shared memory (the ring is free: every MMA has read it): [NA][rows][128]
     const int quad = warp & 3;
     mbar_wait(done, 0, status);  // (a wait that gives up is in the status word)
     tc_fence_after();
@@ -674,7 +676,7 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
     float* p = reinterpret_cast<float*>(smem) + quad * 32 + lane;
     constexpr int CW = NT < 32 ? NT : 32;  // columns at a time
 #pragma unroll 1
-    for (int c = 0; c < g.T; c += CW) {
+    for (int c = 0; c < rows; c += CW) {
       float v[CW], w[CW];
       if constexpr (CW == 16) {
         tmem_ld16(taddr + c, v);
@@ -684,11 +686,11 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
         tmem_ld32(taddr + NT + c, w);
       }
       tmem_ld_wait();
-      const int n = g.T - c;
+      const int n = rows - c;
 #pragma unroll
       for (int j = 0; j < CW; ++j) {
         if constexpr (DUAL_) {
-          if (j < n) p[(c + j) * 128] = v[j], p[(g.T + c + j) * 128] = w[j];
+          if (j < n) p[(c + j) * 128] = v[j], p[(rows + c + j) * 128] = w[j];
         } else {
           if (j < n) p[(c + j) * 128] = v[j] + w[j];
         }
@@ -714,14 +716,14 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
         if (c < C) s.x += q[c].x, s.y += q[c].y, s.z += q[c].z, s.w += q[c].w;
       return s;
     };
-    const int quads = g.T * 32;  // (row, four weight rows), dealt to the cluster's threads
+    const int quads = rows * 32;  // (row, four weight rows), dealt to the cluster's threads
 #pragma unroll 1
     for (int e = rank * 192 + threadIdx.x; e < quads; e += C * 192) {
-      const int t = e >> 5, f = (e & 31) * 4, col = w0 + f;
+      const int r = e >> 5, t = t0 + r, f = (e & 31) * 4, col = w0 + f;
       if (col >= g.n) continue;
-      float4 a = sum((t * 128 + f) * 4);
+      float4 a = sum((r * 128 + f) * 4);
       if constexpr (DUAL_) {
-        const float4 u = sum(((g.T + t) * 128 + f) * 4);
+        const float4 u = sum(((rows + r) * 128 + f) * 4);
         if (g.gu) {
           *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 0)) = a;
           *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 1)) = u;
@@ -757,54 +759,75 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
   }
 }
 
+// CTAs of a cluster: as many of 8, 4, 2 or 1 as leave each two K blocks and all clusters resident at once (a cluster that
+// has to wait for another costs the kernel's time again: at 64 rows 48 clusters of 4 take 25 us, 48 of 2 take 18). How
+// many are resident is asked for once a kernel, size and device. Negative: an error.
 template <bool DUAL_, int NT, bool F16>
-static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArgs& g, uint32_t* status, cudaStream_t st) {
+static int few_cluster(int clusters, int kb) {
+  auto kern = ffn_few_kernel<DUAL_, NT, F16>;
+  static std::atomic<uint64_t> devs{0};
+  if (const int e = smem_attr_once(devs, (const void*)kern, Few<DUAL_, NT>::TOTAL)) return -e;
+  static std::atomic<int> resident[64][4];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return -(int)e;
+  for (int i = 3; i > 0; --i) {
+    if (kb / (1 << i) < 2) continue;
+    int most = resident[dev & 63][i].load(std::memory_order_relaxed);
+    if (!most) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute at;
+      at.id = cudaLaunchAttributeClusterDimension;
+      at.val.clusterDim = {1u << i, 1, 1};
+      cfg.gridDim = dim3(1 << i), cfg.blockDim = dim3(192), cfg.dynamicSmemBytes = Few<DUAL_, NT>::TOTAL;
+      cfg.attrs = &at, cfg.numAttrs = 1;
+      e = cudaOccupancyMaxActiveClusters(&most, kern, &cfg);
+      if (e != cudaSuccess) return -(int)e;
+      most = std::max(most * (NT <= 32 ? 2 : 1), 1);  // (counted at one CTA an SM)
+      resident[dev & 63][i].store(most, std::memory_order_relaxed);
+    }
+    if (clusters <= most) return 1 << i;
+  }
+  return 1;
+}
+
+template <bool DUAL_, int NT, bool F16>
+static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, FewArgs g, int chunks, int C, uint32_t* status,
+                      cudaStream_t st) {
   using S = Few<DUAL_, NT>;
   CUtensorMap tw, tx;
   int rc = make_tmap_2d(&tw, w.p, 2, g.K, w_rows, w.ld * 2, BK, 128, 1);
   if (!rc) rc = make_tmap_2d(&tx, x.p, 2, g.K, x_rows, x.ld * 2, BK, NT, 1);
   if (rc) return 5000 + rc;
-  auto kern = ffn_few_kernel<DUAL_, NT, F16>;
-  static std::atomic<uint64_t> devs{0};
-  if (const int err = smem_attr_once(devs, (const void*)kern, S::TOTAL)) return err;
-  const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK;
+  g.chunk = (g.T + chunks - 1) / chunks;
   cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(C, (g.n + 127) / 128, chunks);
   cfg.blockDim = dim3(192);
   cfg.dynamicSmemBytes = S::TOTAL;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  // CTAs of a cluster: as many of 8, 4, 2 or 1 as leave each two K blocks and all clusters resident at once (a cluster
-  // that has to wait for another costs the kernel's time again: at 64 rows 48 clusters of 4 take 25 us, 48 of 2 take
-  // 18). How many are resident is asked for once a kernel, size and device.
-  static std::atomic<int> resident[64][4];
-  int dev = 0, C = 1;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return (int)e;
-  for (int i = 3; i > 0; --i) {
-    if (kb / (1 << i) < 2) continue;
-    int clusters = resident[dev & 63][i].load(std::memory_order_relaxed);
-    if (!clusters) {
-      at[0].val.clusterDim = {1u << i, 1, 1};
-      cfg.gridDim = dim3(1 << i, 1), cfg.attrs = at, cfg.numAttrs = 1;
-      e = cudaOccupancyMaxActiveClusters(&clusters, kern, &cfg);
-      if (e != cudaSuccess) return (int)e;
-      clusters = std::max(clusters * (NT <= 32 ? 2 : 1), 1);  // (counted at one CTA an SM)
-      resident[dev & 63][i].store(clusters, std::memory_order_relaxed);
-    }
-    if (tiles <= clusters) {
-      C = 1 << i;
-      break;
-    }
-  }
-  cfg.gridDim = dim3(C, tiles);
   at[0].val.clusterDim = {(unsigned)C, 1, 1};
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, tw, tx, g, status);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ffn_few_kernel<DUAL_, NT, F16>, tw, tx, g, status);
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
+}
+
+// The rows go as one chunk, or as two where that costs the clusters no CTA: the partial sums that a cluster exchanges
+// are halved (80 rows at 2,560 x 640: 16.5 us in one chunk, 15.1 in two)
+template <bool DUAL_, int NT, bool F16>
+static int few_rows(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArgs& g, uint32_t* status, cudaStream_t st) {
+  const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK, C = few_cluster<DUAL_, NT, F16>(tiles, kb);
+  if (C < 0) return -C;
+  if constexpr (NT > 32) {
+    const int C2 = few_cluster<DUAL_, NT / 2, F16>(2 * tiles, kb);
+    if (C2 < 0) return -C2;
+    if (C2 >= C) return launch_few<DUAL_, NT / 2, F16>(w, w_rows, x, x_rows, g, 2, C2, status, st);
+  }
+  return launch_few<DUAL_, NT, F16>(w, w_rows, x, x_rows, g, 1, C, status, st);
 }
 
 template <int NT, bool F16>
@@ -812,11 +835,11 @@ static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void
                    cudaStream_t st) {
   FewArgs g;
   g.T = (int)s.T, g.n = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.out = h, g.gu = gu;
-  const int rc = launch_few<true, NT, F16>(w13, 2 * (int64_t)s.F, x, s.T, g, status, st);
+  const int rc = few_rows<true, NT, F16>(w13, 2 * (int64_t)s.F, x, s.T, g, status, st);
   if (rc) return rc;
   g = FewArgs();
   g.T = (int)s.T, g.n = s.N, g.K = s.F, g.out = y, g.residual = residual.p, g.ldr = residual.ld;
-  return launch_few<false, NT, F16>(w2, s.N, {h, s.F}, 2 * s.T, g, status, st);
+  return few_rows<false, NT, F16>(w2, s.N, {h, s.F}, 2 * s.T, g, status, st);
 }
 
 static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {
