@@ -561,6 +561,7 @@ static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr res
 // there is one launch a product. h is kept as two terms (value and rounding error, rows 0.. and T.. of a [2T, F]
 // buffer): the second MMA column block costs nothing here and leaves the result with its own rounding only.
 constexpr int FEW = 128;
+constexpr int64_t PREFETCH = 48 << 20;  // of the down projection's weights, into the 126 MB of L2
 
 template <bool DUAL_, int NT>
 struct Few {
@@ -579,6 +580,8 @@ struct FewArgs {
   float* gu = nullptr;             // DUAL: g and u (at_gu) or null
   const void* residual = nullptr;  // else: [T, n] or null
   int64_t ldr = 0;
+  const void* next = nullptr;      // DUAL: the down projection's weights, `next_bytes` of them (a multiple of 16)
+  int64_t next_bytes = 0;
 };
 
 template <bool DUAL_, int NT, bool F16>
@@ -646,6 +649,14 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
         if (DUAL_ || i >= STAGES) load_w(i);
         load_x(i);
         ++issued;
+      }
+      if constexpr (DUAL_) {
+        // this CTA's share of the next kernel's weights into L2: HBM works on through the sums and the epilogue
+        const int64_t ctas = (int64_t)gridDim.x * gridDim.y * gridDim.z;
+        const int64_t id = ((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+        const int64_t each = (g.next_bytes / 16 + ctas - 1) / ctas * 16, end = min(g.next_bytes, (id + 1) * each);
+        for (int64_t at = id * each; at < end; at += 16384)
+          bulk_prefetch_l2(reinterpret_cast<const uint8_t*>(g.next) + at, (uint32_t)min((int64_t)16384, end - at));
       }
       for (int i = max(0, issued - STAGES); i < issued; ++i) mbar_wait(&full[i % STAGES], (i / STAGES) & 1, status);
     }
@@ -835,6 +846,7 @@ static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void
                    cudaStream_t st) {
   FewArgs g;
   g.T = (int)s.T, g.n = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.out = h, g.gu = gu;
+  g.next = w2.p, g.next_bytes = std::min<int64_t>((int64_t)s.N * s.F * 2, PREFETCH);
   const int rc = few_rows<true, NT, F16>(w13, 2 * (int64_t)s.F, x, s.T, g, status, st);
   if (rc) return rc;
   g = FewArgs();

@@ -71,6 +71,10 @@ AFB_DEV void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c
                "r"(c1), "r"(smem_u32(src))
                : "memory");
 }
+// bytes % 16 == 0 bytes at a 16-byte aligned address into L2
+AFB_DEV void bulk_prefetch_l2(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
 AFB_DEV void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // at most N of this thread's bulk groups still read shared memory
 template <int N>
