@@ -392,22 +392,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             tmem_ld32(acc + BN / 2 + q * 32, w);
             tmem_ld_wait();
             if (q == 1) tell();
-            if (g.f32 && live) {
+            if (g.f32) {
+              with_act(g.act, [&](auto A) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                  float a0, d0, a1, d1;
+                  act_grad<A.value>(v[j], a0, d0);
+                  act_grad<A.value>(v[j + 1], a1, d1);
+                  h[q * 16 + j / 2] = pack2<F16>(a0 * w[j], a1 * w[j + 1]);
+                  w[j] *= d0, w[j + 1] *= d1;
+                  v[j] = a0, v[j + 1] = a1;
+                }
+              });
 #pragma unroll
               for (int j = 0; j < 32; j += 8) {
                 const int col = col0 + q * 32 + j;
-                if (col < g.N) {
-                  st_gu(g.f32 + at_gu(row, col, g.F, 0), v + j);
-                  st_gu(g.f32 + at_gu(row, col, g.F, 1), w + j);
+                if (live && col < g.N) {
+                  st_gu(g.f32 + at_gu(row, col, g.F, 0), w + j);
+                  st_gu(g.f32 + at_gu(row, col, g.F, 1), v + j);
                 }
               }
-            }
-            with_act(g.act, [&](auto A) {
+            } else {
+              with_act(g.act, [&](auto A) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                h[q * 16 + j] = pack2<F16>(act_only<A.value>(v[2 * j]) * w[2 * j],
-                                           act_only<A.value>(v[2 * j + 1]) * w[2 * j + 1]);
-            });
+                for (int j = 0; j < 16; ++j)
+                  h[q * 16 + j] = pack2<F16>(act_only<A.value>(v[2 * j]) * w[2 * j],
+                                             act_only<A.value>(v[2 * j + 1]) * w[2 * j + 1]);
+              });
+            }
           }
           begin_put();
           put_row(buf, lane, h);
@@ -426,16 +438,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           tmem_ld16(acc + c * 16, v);
           tmem_ld_wait();
           if (c == CH - 1) tell();
-          with_act(g.act, [&](auto A) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              float a0, d0, a1, d1;
-              act_grad<A.value>(gp[2 * j], a0, d0);
-              act_grad<A.value>(gp[2 * j + 1], a1, d1);
-              dgp[j] = pack2<F16>(v[2 * j] * up[2 * j] * d0, v[2 * j + 1] * up[2 * j + 1] * d1);
-              dup[j] = pack2<F16>(v[2 * j] * a0, v[2 * j + 1] * a1);
-            }
-          });
+          for (int j = 0; j < 8; ++j) {
+            dgp[j] = pack2<F16>(v[2 * j] * gp[2 * j], v[2 * j + 1] * gp[2 * j + 1]);
+            dup[j] = pack2<F16>(v[2 * j] * up[2 * j], v[2 * j + 1] * up[2 * j + 1]);
+          }
           load_gu(c + 2 < CH ? gu_now : gu_next, (c + 2) % CH, gp, up);
         };
 #pragma unroll 1
@@ -735,14 +742,18 @@ __global__ void __launch_bounds__(192) ffn_few_kernel(const __grid_constant__ CU
       float4 a = sum((r * 128 + f) * 4);
       if constexpr (DUAL_) {
         const float4 u = sum(((rows + r) * 128 + f) * 4);
-        if (g.gu) {
-          *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 0)) = a;
-          *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 1)) = u;
-        }
+        float4 d;
         with_act(g.act, [&](auto A) {
-          a = make_float4(act_only<A.value>(a.x) * u.x, act_only<A.value>(a.y) * u.y, act_only<A.value>(a.z) * u.z,
-                          act_only<A.value>(a.w) * u.w);
+          act_grad<A.value>(a.x, a.x, d.x);
+          act_grad<A.value>(a.y, a.y, d.y);
+          act_grad<A.value>(a.z, a.z, d.z);
+          act_grad<A.value>(a.w, a.w, d.w);
         });
+        if (g.gu) {
+          *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 0)) = make_float4(u.x * d.x, u.y * d.y, u.z * d.z, u.w * d.w);
+          *reinterpret_cast<float4*>(g.gu + at_gu(t, col, g.F, 1)) = a;
+        }
+        a = make_float4(a.x * u.x, a.y * u.y, a.z * u.z, a.w * u.w);
         const uint2 hi = make_uint2(pack2<F16>(a.x, a.y), pack2<F16>(a.z, a.w));
         const float2 r0 = unpack2<F16>(hi.x), r1 = unpack2<F16>(hi.y);
         const uint2 lo = make_uint2(
