@@ -29,7 +29,8 @@ constexpr uint32_t OP_BYTES = 128 * BK * 2;  // one operand of one CTA and stage
 constexpr int EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
 
 enum Epi { STORE = 0, PARTIAL = 1, DUAL = 2, DACT = 3 };
-enum Layout { NT = 0, NN = 1, TN = 2 };  // A K-major B K-major | A K-major B MN-major | both MN-major
+// A K-major B K-major | A K-major B MN-major | both MN-major | dx (NN) and the weight gradients (TN) in one launch
+enum Layout { NT = 0, NN = 1, TN = 2, GRADS = 3 };
 
 constexpr int STAGES = 6;
 constexpr uint32_t EPI_OFF = STAGES * 2 * OP_BYTES;
@@ -37,6 +38,17 @@ constexpr uint32_t EPI_BYTES = 4096;  // staging of an epilogue warp: 32 rows of
 constexpr uint32_t BAR_OFF = EPI_OFF + EPI_WARPS * EPI_BYTES;
 constexpr uint32_t SMEM = BAR_OFF + (2 * STAGES + 4) * 8 + 16 + 1024;
 
+// The backward products after DACT in one launch: dx [T, H] (2F / 64 K blocks a tile), dW13 [2F, H] and dW2 [N, F] (T / 64
+// K blocks a tile). Alone each of them ends in a wave that leaves pairs idle; together the tiles with fewer K blocks
+// fill in behind those with more: pair p of P takes long tiles p, p + P, ..., then x short ones where it had one long
+// tile more than the others, y otherwise (x <= y).
+struct Grads {
+  uint32_t tiles[3] = {}, mt[3] = {}, nt[3] = {}, kb[3] = {};  // dx, dW13, dW2
+  int M[3] = {}, N[3] = {};
+  uint32_t dx_long = 0;            // the long tiles are dx's (else the weight gradients')
+  uint32_t longs = 0, shorts = 0;  // tiles of the two kinds
+  uint32_t x = 0, y = 0;
+};
 struct Args {
   int64_t M = 0;  // rows of the result
   int N = 0;      // columns of the result (DUAL: F)
@@ -46,11 +58,13 @@ struct Args {
   int splits = 1;                  // PARTIAL
   const void* residual = nullptr;  // STORE, optional
   int64_t ldr = 0;
+  Grads grads;           // GRADS
   float* f32 = nullptr;  // PARTIAL: sums [splits, M in whole tiles, N]; DUAL: g and u (at_gu) or null; DACT: g and u
 };
-// tensor maps: operands; the 16-bit result (STORE, DUAL h, DACT dg), and DACT's du
+// tensor maps: operands; the 16-bit result (STORE, DUAL h, DACT dg), and DACT's du; GRADS: of each product
+template <int LAYOUT>
 struct Maps {
-  CUtensorMap a, b, out, out2;
+  CUtensorMap a[LAYOUT == GRADS ? 3 : 1], b[LAYOUT == GRADS ? 3 : 1], out[LAYOUT == GRADS ? 3 : 2];
 };
 
 // g and u are kept as the epilogue's threads hold them, 32 rows x 8 columns (32 bytes a row) at a time: a warp's access
@@ -106,7 +120,8 @@ AFB_DEV void with_act(int act, F&& f) {
 }
 
 struct Tile {
-  int m, n, split;  // row tile, column tile, K split
+  int m, n, split;  // row tile, column tile, K split (GRADS: product)
+  uint32_t kb0, kb1;
 };
 // tile order: bands of 8 row tiles, down the band first, so that the tiles in flight share both operands in L2.
 // 32-bit: the tile count is checked on the host, and a 64-bit division costs the producer some 200 cycles.
@@ -119,6 +134,29 @@ AFB_DEV Tile tile_at(uint32_t t, uint32_t mt, uint32_t nt) {
   r.m = band * 8u + in - n * rows;
   r.n = n;
   return r;
+}
+// the k-th tile of pair p of P; false behind its last one
+AFB_DEV bool grads_tile(const Grads& g, uint32_t k, uint32_t p, uint32_t P, Tile& r) {
+  const uint32_t more = g.longs % P, nl = g.longs / P + (p < more);
+  uint32_t i;
+  bool dx;
+  if (k < nl) {
+    i = k * P + p;
+    dx = g.dx_long;
+  } else {
+    const uint32_t j = k - nl;
+    if (j >= (p < more ? g.x : g.y)) return false;
+    i = j < g.x ? j * P + p : g.x * P + (j - g.x) * (P - more) + (p - more);
+    if (i >= g.shorts) return false;
+    dx = !g.dx_long;
+  }
+  const uint32_t q = dx ? 0 : i < g.tiles[1] ? 1 : 2;
+  if (q == 2) i -= g.tiles[1];
+  r = tile_at(i, g.mt[q], g.nt[q]);
+  r.split = q;
+  r.kb0 = 0;
+  r.kb1 = g.kb[q];
+  return true;
 }
 
 AFB_DEV void st32(void* p, const uint32_t* r) {
@@ -156,8 +194,8 @@ AFB_DEV void put_half_row(uint8_t* buf, int row, const uint32_t* w) {
 // epilogue is kept to whole 128-byte lines.
 template <int LAYOUT, int EPI, bool F16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-    ffn_gemm_kernel(const __grid_constant__ Maps maps, Args g, uint32_t* status) {
-  constexpr bool A_MN = LAYOUT == TN, B_MN = LAYOUT != NT;
+    ffn_gemm_kernel(const __grid_constant__ Maps<LAYOUT> maps, Args g, uint32_t* status) {
+  constexpr bool B_MN = LAYOUT != NT;
   constexpr int TN_COLS = EPI == DUAL ? BN / 2 : BN;  // result columns per tile
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -170,14 +208,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_cta_rank();
   const uint32_t mt = (uint32_t)((g.M + BM - 1) / BM), nt = (g.N + TN_COLS - 1) / TN_COLS, tiles = mt * nt * g.splits;
-  const uint32_t t0 = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const uint32_t kb_total = (uint32_t)((g.K + BK - 1) / BK);
-  // first K block of a split; at most 32 splits of 2^25 blocks
-  auto kb_lo = [&](uint32_t split) { return EPI == PARTIAL ? kb_total * split / (uint32_t)g.splits : split * kb_total; };
+  // the k-th tile of this pair
+  auto tile = [&](uint32_t k, Tile& r) {
+    if constexpr (LAYOUT == GRADS) return grads_tile(g.grads, k, pair, pairs, r);
+    const uint32_t t = pair + k * pairs;
+    if (t >= tiles) return false;
+    r = tile_at(t, mt, nt);
+    r.kb0 = 0;
+    r.kb1 = kb_total;
+    if constexpr (EPI == PARTIAL) {  // at most 32 splits of 2^25 blocks
+      r.kb0 = kb_total * r.split / (uint32_t)g.splits;
+      r.kb1 = kb_total * (r.split + 1) / (uint32_t)g.splits;
+    }
+    return true;
+  };
+  auto a_mn = [](const Tile& r) { return LAYOUT == TN || (LAYOUT == GRADS && r.split > 0); };
+  auto q_of = [](const Tile& r) { return LAYOUT == GRADS ? r.split : 0; };  // the product's maps
 
-  if (threadIdx.x == 32) {
-    prefetch_tmap(&maps.a);
-    prefetch_tmap(&maps.b);
+  if (threadIdx.x >= 32 && threadIdx.x < 32 + (LAYOUT == GRADS ? 3 : 1)) {
+    prefetch_tmap(&maps.a[threadIdx.x - 32]);
+    prefetch_tmap(&maps.b[threadIdx.x - 32]);
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -203,12 +255,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       uint32_t i = 0, s = 0, ph = 1;  // stages issued, the ring's next stage and its empty barrier's parity
       bool ok = true;
-      for (uint32_t t = t0; t < tiles && ok; t += step) {
-        const Tile tl = tile_at(t, mt, nt);
-        const uint32_t kb1 = kb_lo(tl.split + 1);
+      Tile tl;
+      for (uint32_t n = 0; ok && tile(n, tl); ++n) {
+        const CUtensorMap *tm_a = &maps.a[q_of(tl)], *tm_b = &maps.b[q_of(tl)];
         const int ma = tl.m * BM + (int)rank * 128;
         const int nb = EPI == DUAL ? (int)rank * g.F + tl.n * TN_COLS : tl.n * TN_COLS + (int)rank * 128;
-        for (uint32_t kb = kb_lo(tl.split); kb < kb1; ++kb, ++i) {
+        for (uint32_t kb = tl.kb0; kb < tl.kb1; ++kb, ++i) {
           if (!mbar_wait(&empty[s], ph, status)) {  // (passes at once in the ring's first round)
             ok = false;
             break;
@@ -218,17 +270,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           uint8_t* a = smem + s * 2 * OP_BYTES;
           uint8_t* b = a + OP_BYTES;
           const int k = (int)kb * BK;
-          if constexpr (A_MN) {
-            tma_load_2d_pair(a, &maps.a, bar, ma, k);
-            tma_load_2d_pair(a + 8192, &maps.a, bar, ma + 64, k);
+          if (a_mn(tl)) {
+            tma_load_2d_pair(a, tm_a, bar, ma, k);
+            tma_load_2d_pair(a + 8192, tm_a, bar, ma + 64, k);
           } else {
-            tma_load_2d_pair(a, &maps.a, bar, k, ma);
+            tma_load_2d_pair(a, tm_a, bar, k, ma);
           }
           if constexpr (B_MN) {
-            tma_load_2d_pair(b, &maps.b, bar, nb, k);
-            tma_load_2d_pair(b + 8192, &maps.b, bar, nb + 64, k);
+            tma_load_2d_pair(b, tm_b, bar, nb, k);
+            tma_load_2d_pair(b + 8192, tm_b, bar, nb + 64, k);
           } else {
-            tma_load_2d_pair(b, &maps.b, bar, k, nb);
+            tma_load_2d_pair(b, tm_b, bar, k, nb);
           }
           if (++s == STAGES) s = 0, ph ^= 1;
         }
@@ -239,12 +291,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc =
-          idesc_f16(BM, BN, F16 ? 0 : 1) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16);
       uint32_t n = 0, s = 0, ph = 0;  // tiles of this pair; ring stage and its full barrier's parity
       bool ok = true;
-      for (uint32_t t = t0; t < tiles && ok; t += step, ++n) {
-        const uint32_t split = EPI == PARTIAL ? t / (mt * nt) : 0, kb0 = kb_lo(split), kb1 = kb_lo(split + 1);
+      Tile tl;
+      for (; ok && tile(n, tl); ++n) {
+        const bool am = a_mn(tl);
+        const uint32_t idesc = idesc_f16(BM, BN, F16 ? 0 : 1) | ((uint32_t)am << 15) | ((uint32_t)B_MN << 16);
+        const uint32_t kb0 = tl.kb0, kb1 = tl.kb1;
         const uint32_t acc = tmem + (n & 1) * BN;
         if (!mbar_wait(&acc_empty[n & 1], ((n >> 1) & 1) ^ 1, status)) break;
         tc_fence_after();
@@ -257,7 +310,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           const uint32_t a = smem_u32(smem + s * 2 * OP_BYTES), b = a + OP_BYTES;
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk) {
-            const uint64_t da = A_MN ? sw128_desc_mn(a + kk * 2048, 8192, 1024) : sw128_desc(a) + 2 * kk;
+            const uint64_t da = am ? sw128_desc_mn(a + kk * 2048, 8192, 1024) : sw128_desc(a) + 2 * kk;
             const uint64_t db = B_MN ? sw128_desc_mn(b + kk * 2048, 8192, 1024) : sw128_desc(b) + 2 * kk;
             umma_f16_pair(acc, da, db, idesc, kb > kb0 || kk > 0);
           }
@@ -288,10 +341,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       const float *g, *u;  // this lane's first column of the tile, or null where its row is outside the result
       int col;
     };
-    auto gu_tile = [&](uint32_t t) {
+    auto gu_tile = [&](uint32_t k) {
       GuTile r{nullptr, nullptr, 0};
-      if (EPI != DACT || t >= tiles) return r;
-      const Tile tl = tile_at(t, mt, nt);
+      Tile tl;
+      if (EPI != DACT || !tile(k, tl)) return r;
       const int64_t row = (int64_t)tl.m * BM + warp_row + lane;
       r.col = tl.n * TN_COLS + lane_col;
       if (row < g.M) r.g = g.f32 + at_gu(row, r.col, g.F, 0), r.u = g.f32 + at_gu(row, r.col, g.F, 1);
@@ -306,17 +359,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           ld_gu(p.u + (c * 16 + j) * 32, up + j);
         }
     };
-    GuTile gu_now = gu_tile(t0);
+    GuTile gu_now = gu_tile(0);
     if constexpr (EPI == DACT) {
       load_gu(gu_now, 0, gq[0], uq[0]);
       load_gu(gu_now, 1, gq[1], uq[1]);
     }
     uint32_t n = 0;  // tiles of this pair
-    for (uint32_t t = t0; t < tiles; t += step, ++n) {
-      const Tile tl = tile_at(t, mt, nt);
+    Tile tl;
+    for (; tile(n, tl); ++n) {
       const int row0 = tl.m * BM + warp_row, col0 = tl.n * TN_COLS + lane_col;
-      const int64_t row = (int64_t)row0 + lane;
-      const bool live = row < g.M, any = row0 < g.M;  // this lane's row, one of the warp's
+      const int64_t row = (int64_t)row0 + lane, M = LAYOUT == GRADS ? g.grads.M[q_of(tl)] : g.M;
+      const int N = LAYOUT == GRADS ? g.grads.N[q_of(tl)] : g.N;
+      const bool live = row < M, any = row0 < M;  // this lane's row, one of the warp's
       // one answer for the warp
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[n & 1], (n >> 1) & 1, status))) break;
       tc_fence_after();
@@ -333,7 +387,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll 1
         for (int c = 0; c < HALF && any; c += 64) {
           const int col = col0 + c;
-          if (col >= g.N) break;
+          if (col >= N) break;
           float v[64];
           tmem_ld32(acc + c, v);
           tmem_ld32(acc + c + 32, v + 32);
@@ -343,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const uint16_t* rp = reinterpret_cast<const uint16_t*>(g.residual) + row * g.ldr + col;
 #pragma unroll
             for (int j = 0; j < 64; j += 8)
-              if (col + j < g.N) {
+              if (col + j < N) {
                 const uint4 q = *reinterpret_cast<const uint4*>(rp + j);
                 const uint32_t r[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -361,7 +415,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           put_row(buf, lane, w);
           end_put();
           if (lane == 0) {
-            tma_store_2d(&maps.out, buf, col, row0);
+            tma_store_2d(&maps.out[q_of(tl)], buf, col, row0);
             bulk_commit();
           }
         }
@@ -378,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           put_row(buf, lane, reinterpret_cast<const uint32_t*>(v));
           end_put();
           if (lane == 0) {
-            tma_store_2d(&maps.out, buf, col, tl.split * (int)mt * BM + row0);
+            tma_store_2d(&maps.out[0], buf, col, tl.split * (int)mt * BM + row0);
             bulk_commit();
           }
         }
@@ -425,13 +479,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           put_row(buf, lane, h);
           end_put();
           if (lane == 0) {
-            tma_store_2d(&maps.out, buf, col0, row0);
+            tma_store_2d(&maps.out[0], buf, col0, row0);
             bulk_commit();
           }
         }
       } else {  // DACT
         constexpr int CH = HALF / 16;
-        const GuTile gu_next = gu_tile(t + step);
+        const GuTile gu_next = gu_tile(n + 1);
         uint32_t dg[16], du[16];  // 32 columns
         auto chunk = [&](int c, float* gp, float* up, uint32_t* dgp, uint32_t* dup) {
           float v[16];
@@ -456,8 +510,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           put_half_row(buf + 2048, lane, du);
           end_put();
           if (lane == 0) {
-            tma_store_2d(&maps.out, buf, col, row0);
-            tma_store_2d(&maps.out2, buf + 2048, col, row0);
+            tma_store_2d(&maps.out[0], buf, col, row0);
+            tma_store_2d(&maps.out[1], buf + 2048, col, row0);
             bulk_commit();
           }
         }
@@ -495,19 +549,21 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict
       make_uint4(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7]));
 }
 
-// K splits of a product: those that minimise waves of tiles x K blocks of a tile (0.37 us each at the rate the products reach), plus
-// the fp32 partials written and read again (about 4 TB/s through L2) and the second launch (3 us)
-static int plan_splits(int64_t M, int N, int64_t K, int num_sms) {
+// K splits of a product: those that minimise waves of tiles x K blocks of a tile (0.37 us each at the rate the products
+// reach), plus the fp32 partials written and read again (about 4 TB/s through L2) and the second launch (3 us).
+// `us`: the estimate.
+constexpr double KB_US = 0.37;
+static int plan_splits(int64_t M, int N, int64_t K, int num_sms, double* us = nullptr) {
   const int64_t tiles = ((M + BM - 1) / BM) * ((N + BN - 1) / BN), kb = (K + BK - 1) / BK, pairs = num_sms / 2;
-  if (tiles < 1 || tiles >= pairs) return 1;
   int best = 1;
   double cost = 1e300;
-  for (int s = 1; s <= 32 && s * 4 <= std::max<int64_t>(kb, 4); ++s) {
+  for (int s = 1; s <= 32 && s * 4 <= std::max<int64_t>(kb, 4) && (s == 1 || tiles < pairs); ++s) {
     const double waves = (double)((tiles * s + pairs - 1) / pairs);
-    const double c = waves * (double)((kb + s - 1) / s) * 0.37 +
+    const double c = waves * (double)((kb + s - 1) / s) * KB_US +
                      (s > 1 ? 3. + 8. * s * (double)M * N / 4e6 : 0.);
     if (c < cost * 0.98) best = s, cost = c;
   }
+  if (us) *us = cost;
   return best;
 }
 
@@ -516,16 +572,21 @@ struct Ptr {  // a row-major matrix
   int64_t ld;
 };
 
-template <int LAYOUT, int EPI, bool F16>
-static int launch(Ptr A, Ptr B, int64_t b_rows, Maps& maps, const Args& g, int num_sms, uint32_t* status,
-                  cudaStream_t st) {
-  constexpr bool A_MN = LAYOUT == TN, B_MN = LAYOUT != NT;
-  int rc = A_MN ? make_tmap_2d(&maps.a, A.p, 2, g.M, g.K, A.ld * 2, 64, BK, 1)
-                : make_tmap_2d(&maps.a, A.p, 2, g.K, g.M, A.ld * 2, BK, 128, 1);
+// maps of A [M, K] and B [n, K] (K-major: K innermost) or of their transposes as they lie (MN-major)
+static int operand_maps(CUtensorMap* a, CUtensorMap* b, bool a_mn, bool b_mn, Ptr A, Ptr B, int64_t M, int64_t n,
+                        int64_t K) {
+  int rc = a_mn ? make_tmap_2d(a, A.p, 2, M, K, A.ld * 2, 64, BK, 1)
+                : make_tmap_2d(a, A.p, 2, K, M, A.ld * 2, BK, 128, 1);
   if (rc) return 1000 + rc;
-  rc = B_MN ? make_tmap_2d(&maps.b, B.p, 2, b_rows, g.K, B.ld * 2, 64, BK, 1)
-            : make_tmap_2d(&maps.b, B.p, 2, g.K, b_rows, B.ld * 2, BK, 128, 1);
-  if (rc) return 2000 + rc;
+  rc = b_mn ? make_tmap_2d(b, B.p, 2, n, K, B.ld * 2, 64, BK, 1) : make_tmap_2d(b, B.p, 2, K, n, B.ld * 2, BK, 128, 1);
+  return rc ? 2000 + rc : 0;
+}
+
+template <int LAYOUT, int EPI, bool F16>
+static int launch(Ptr A, Ptr B, int64_t b_rows, Maps<LAYOUT>& maps, const Args& g, int num_sms, uint32_t* status,
+                  cudaStream_t st) {
+  const int rc = operand_maps(&maps.a[0], &maps.b[0], LAYOUT == TN, LAYOUT != NT, A, B, g.M, b_rows, g.K);
+  if (rc) return rc;
   auto kern = ffn_gemm_kernel<LAYOUT, EPI, F16>;
   static std::atomic<uint64_t> devs{0};
   if (const int e = smem_attr_once(devs, (const void*)kern, SMEM)) return e;
@@ -546,13 +607,13 @@ static int row_map(CUtensorMap* m, const void* p, int bytes, int64_t cols, int64
 template <int LAYOUT, bool F16>
 static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr residual, float* scratch, int num_sms,
                    uint32_t* status, cudaStream_t st) {
-  Maps maps;
+  Maps<LAYOUT> maps;
   Args g;
   g.M = M, g.N = N, g.K = K, g.residual = residual.p, g.ldr = residual.ld;
   g.splits = residual.p ? 1 : plan_splits(M, N, K, num_sms);
   const int64_t rows = (M + BM - 1) / BM * BM;  // of a split's partial sums: whole tiles
-  int rc = g.splits == 1 ? row_map(&maps.out, out, 2, N, M, N, 128)
-                         : row_map(&maps.out, scratch, 4, N, rows * g.splits, N, 128);
+  int rc = g.splits == 1 ? row_map(&maps.out[0], out, 2, N, M, N, 128)
+                         : row_map(&maps.out[0], scratch, 4, N, rows * g.splits, N, 128);
   if (rc) return rc;
   if (g.splits == 1) return launch<LAYOUT, STORE, F16>(A, B, N, maps, g, num_sms, status, st);
   rc = launch<LAYOUT, PARTIAL, F16>(A, B, N, maps, g, num_sms, status, st);
@@ -877,13 +938,50 @@ static int fwd(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h,
     auto f = s.T <= 16 ? fwd_few<16, F16> : s.T <= 32 ? fwd_few<32, F16> : s.T <= 64 ? fwd_few<64, F16> : fwd_few<128, F16>;
     return f(s, x, w13, w2, residual, h, gu, y, status, st);
   }
-  Maps maps;
+  Maps<NT> maps;
   Args g;
   g.M = s.T, g.N = s.F, g.K = s.H, g.F = s.F, g.act = s.act, g.f32 = gu;
-  int rc = row_map(&maps.out, h, 2, s.F, s.T, s.F, 128);
+  int rc = row_map(&maps.out[0], h, 2, s.F, s.T, s.F, 128);
   if (!rc) rc = launch<NT, DUAL, F16>(x, w13, 2 * (int64_t)s.F, maps, g, num_sms, status, st);
   if (rc) return rc;
   return product<NT, F16>({h, s.F}, w2, s.T, s.N, s.F, y, residual, scratch, num_sms, status, st);
+}
+
+// Tiles of the products after DACT, and whether one launch of all of them is expected to take less time than a launch
+// (5 us beside its tiles) for each. A K block takes some 15% more there, for tiles of different products in flight
+// share less of L2. Measured, together against apart: 1,237 x 1,152 x 4,304 56 and 85 us, 16,384 x 2,048 x 512 114 and
+// 136; 4,100 x 2,048 x 6,144, whose tiles fill their waves, 383 and 362; and dx of few tiles and many K blocks has to
+// be split.
+static bool plan_grads(const FfnShape& s, bool dw13, bool dw2, int num_sms, Grads& g) {
+  const int64_t M[3] = {s.T, dw13 ? 2 * (int64_t)s.F : 0, dw2 ? s.N : 0}, K[3] = {2 * (int64_t)s.F, s.T, s.T};
+  const int N[3] = {s.H, s.H, s.F};
+  const int64_t P = num_sms / 2;
+  double apart = 0;
+  int64_t units = 0;
+  for (int q = 0; q < 3; ++q) {
+    if (!M[q]) continue;
+    const int64_t mt = (M[q] + BM - 1) / BM, nt = (N[q] + BN - 1) / BN;
+    if (mt * nt >= (1 << 28)) return false;
+    g.M[q] = (int)M[q], g.N[q] = N[q], g.mt[q] = (uint32_t)mt, g.nt[q] = (uint32_t)nt, g.tiles[q] = (uint32_t)(mt * nt);
+    g.kb[q] = (uint32_t)((K[q] + BK - 1) / BK);
+    units += (int64_t)g.tiles[q] * g.kb[q];
+    double us = 0;
+    plan_splits(M[q], N[q], K[q], num_sms, &us);
+    apart += us + 5.;
+  }
+  const int64_t kt = std::max(g.kb[1], g.kb[2]), weights = (int64_t)g.tiles[1] + g.tiles[2];
+  g.dx_long = g.kb[0] >= kt;
+  g.longs = (uint32_t)(g.dx_long ? g.tiles[0] : weights), g.shorts = (uint32_t)(g.dx_long ? weights : g.tiles[0]);
+  const int64_t kl = g.dx_long ? g.kb[0] : kt, ks = g.dx_long ? kt : g.kb[0];
+  const int64_t each = g.longs / P, more = g.longs % P;
+  // the least load of a pair that holds all short tiles
+  int64_t load = std::max((each + (more > 0)) * kl, (units + P - 1) / P);
+  for (;; ++load) {
+    g.x = more ? (uint32_t)((load - (each + 1) * kl) / ks) : 0;
+    g.y = (uint32_t)((load - each * kl) / ks);
+    if (more * g.x + (P - more) * (int64_t)g.y >= g.shorts) break;
+  }
+  return load * KB_US * 1.15 + 5. < apart;
 }
 
 template <bool F16>
@@ -891,16 +989,35 @@ static int bwd(const FfnShape& s, Ptr dy, Ptr x, Ptr w13, Ptr w2, const void* h,
                void* dw13, void* dw2, float* scratch, int num_sms, uint32_t* status, cudaStream_t st) {
   const Ptr none{nullptr, 0}, d{dgu, 2 * (int64_t)s.F};
   int rc = 0;
-  if (dw2 && (rc = product<TN, F16>(dy, {h, s.F}, s.N, s.F, s.T, dw2, none, scratch, num_sms, status, st))) return rc;
+  Args gr;
+  const bool together = dx && (dw13 || dw2) && plan_grads(s, dw13, dw2, num_sms, gr.grads);
+  if (dw2 && !together && (rc = product<TN, F16>(dy, {h, s.F}, s.N, s.F, s.T, dw2, none, scratch, num_sms, status, st)))
+    return rc;
   if (!dx && !dw13) return 0;
-  Maps maps;
+  Maps<NN> maps;
   Args g;
   g.M = s.T, g.N = s.F, g.K = s.N, g.F = s.F, g.act = s.act, g.f32 = const_cast<float*>(gu);
   uint16_t* o = reinterpret_cast<uint16_t*>(dgu);
-  rc = row_map(&maps.out, o, 2, s.F, s.T, d.ld, 64);
-  if (!rc) rc = row_map(&maps.out2, o + s.F, 2, s.F, s.T, d.ld, 64);
+  rc = row_map(&maps.out[0], o, 2, s.F, s.T, d.ld, 64);
+  if (!rc) rc = row_map(&maps.out[1], o + s.F, 2, s.F, s.T, d.ld, 64);
   if (!rc) rc = launch<NN, DACT, F16>(dy, w2, s.F, maps, g, num_sms, status, st);
   if (rc) return rc;
+  if (together) {
+    Maps<GRADS> m;
+    rc = operand_maps(&m.a[0], &m.b[0], false, true, d, w13, s.T, s.H, 2 * (int64_t)s.F);
+    if (!rc) rc = row_map(&m.out[0], dx, 2, s.H, s.T, s.H, 128);
+    if (!rc && dw13) rc = operand_maps(&m.a[1], &m.b[1], true, true, d, x, 2 * (int64_t)s.F, s.H, s.T);
+    if (!rc && dw13) rc = row_map(&m.out[1], dw13, 2, s.H, 2 * (int64_t)s.F, s.H, 128);
+    if (!rc && dw2) rc = operand_maps(&m.a[2], &m.b[2], true, true, dy, {h, s.F}, s.N, s.F, s.T);
+    if (!rc && dw2) rc = row_map(&m.out[2], dw2, 2, s.F, s.N, s.F, 128);
+    if (rc) return rc;
+    if (!dw13) m.a[1] = m.a[0], m.b[1] = m.b[0], m.out[1] = m.out[0];  // not read, but fetched ahead
+    if (!dw2) m.a[2] = m.a[0], m.b[2] = m.b[0], m.out[2] = m.out[0];
+    auto kern = ffn_gemm_kernel<GRADS, STORE, F16>;
+    static std::atomic<uint64_t> devs{0};
+    if ((rc = smem_attr_once(devs, (const void*)kern, SMEM))) return rc;
+    return launch_pdl(kern, dim3(2 * (num_sms / 2)), dim3(THREADS), SMEM, st, m, gr, status);
+  }
   if (dx && (rc = product<NN, F16>(d, w13, s.T, s.H, 2 * (int64_t)s.F, dx, none, scratch, num_sms, status, st)))
     return rc;
   if (dw13) rc = product<TN, F16>(d, x, 2 * (int64_t)s.F, s.H, s.T, dw13, none, scratch, num_sms, status, st);

@@ -96,7 +96,8 @@ def run_ffn(x, w13, w2, res, dy, act):
 
 # rows, hidden, intermediate, outputs: one element of everything, ragged tiles, one past a tile, K tails, wide and thin
 FFN_SIZES = [(1, 8, 8, 8), (3, 64, 40, 72), (5, 8, 264, 8), (17, 200, 24, 520), (128, 256, 128, 256),
-             (129, 136, 264, 200), (257, 512, 384, 512), (64, 640, 512, 64), (1001, 72, 136, 264), (300, 264, 1032, 16)]
+             (129, 136, 264, 200), (257, 512, 384, 512), (64, 640, 512, 64), (1001, 72, 136, 264), (300, 264, 1032, 16),
+             (70, 136, 3592, 72), (2500, 520, 72, 264)]
 
 
 @pytest.mark.parametrize("size", FFN_SIZES)
