@@ -71,9 +71,12 @@ at::Tensor scratch_of(size_t n, const at::Tensor& like) {
   return at::empty({(int64_t)n}, like.options().dtype(at::kFloat));
 }
 
-// (y, h, gu): h and gu are what ffn_bwd reads; gu is kept only when `save`
-std::tuple<at::Tensor, at::Tensor, OptT> gated_ffn_fwd(const at::Tensor& x_, const at::Tensor& w13_,
-                                                       const at::Tensor& w2_, OptT residual, int64_t act, bool save) {
+// (y, h, gu): h and gu are what ffn_bwd reads; gu is kept only when `save`. y has x's leading dimensions (made in that
+// shape: a view as the result of an autograd node could not be changed in place).
+std::tuple<at::Tensor, at::Tensor, OptT> gated_ffn_fwd(const at::Tensor& xn, const at::Tensor& w13_,
+                                                       const at::Tensor& w2_, const OptT& rn, int64_t act, bool save) {
+  const at::Tensor x_ = rows2d(xn);
+  const OptT residual = rn ? OptT(rows2d(*rn)) : OptT();
   const afb::FfnShape s = ffn_shape(x_, w13_, w2_, act);
   c10::cuda::CUDAGuard g(x_.device());
   const at::Tensor x = tma_rows(x_), w13 = tma_rows(w13_.contiguous()), w2 = tma_rows(w2_.contiguous());
@@ -84,7 +87,9 @@ std::tuple<at::Tensor, at::Tensor, OptT> gated_ffn_fwd(const at::Tensor& x_, con
                 "gated_ffn: residual is [T, N] in x's type on its device");
     r = tma_rows(*residual);
   }
-  at::Tensor y = at::empty({s.T, s.N}, x.options()), h = at::empty({afb::ffn_h_rows(s), s.F}, x.options());
+  auto shape = xn.sizes().vec();
+  shape.back() = s.N;
+  at::Tensor y = at::empty(shape, x.options()), h = at::empty({afb::ffn_h_rows(s), s.F}, x.options());
   OptT gu;
   if (save) gu = at::empty({(s.T + 31) / 32 * 32, 2 * (int64_t)s.F}, x.options().dtype(at::kFloat));
   const size_t n_scr = afb::ffn_fwd_scratch(s, num_sms());
@@ -150,9 +155,16 @@ afb::NormArgs norm_args(const at::Tensor& x, const at::Tensor& w, bool rms, doub
   return a;
 }
 
-// (y, mean, rstd); mean and rstd only when `save` (mean not for rms)
-std::tuple<at::Tensor, OptT, OptT> norm_train_fwd(const at::Tensor& x, const at::Tensor& w, OptT b, double eps,
+// x [..., width] as rows with unit inner stride
+at::Tensor norm_rows(const at::Tensor& x) {
+  const at::Tensor r = rows2d(x);
+  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+}
+
+// (y, mean, rstd); mean and rstd only when `save` (mean not for rms); y has x's shape
+std::tuple<at::Tensor, OptT, OptT> norm_train_fwd(const at::Tensor& xn, const at::Tensor& w, OptT b, double eps,
                                                   bool rms, bool save) {
+  const at::Tensor x = norm_rows(xn);
   afb::NormArgs a = norm_args(x, w, rms, eps);
   if (b.has_value()) {
     TORCH_CHECK(!rms, "norm: rms has no bias");
@@ -162,7 +174,7 @@ std::tuple<at::Tensor, OptT, OptT> norm_train_fwd(const at::Tensor& x, const at:
     a.b = b->data_ptr();
   }
   c10::cuda::CUDAGuard g(x.device());
-  at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor y = at::empty(xn.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
   OptT mean, rstd;
   if (save) {
     rstd = at::empty({a.rows}, x.options().dtype(at::kFloat));
@@ -242,13 +254,11 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2,
                             const OptT& residual, int64_t act) {
     const bool need_gu = wants_grad(x) || wants_grad(w13);
-    auto [y, h, gu] = gated_ffn_fwd(rows2d(x), w13, w2, residual ? OptT(rows2d(*residual)) : OptT(), act, need_gu);
+    auto [y, h, gu] = gated_ffn_fwd(x, w13, w2, residual, act, need_gu);
     ctx->save_for_backward({x, w13, w2, wants_grad(w2) ? h : at::Tensor(), val(gu)});
     ctx->saved_data["act"] = act;
     ctx->saved_data["residual"] = residual.has_value();
-    auto shape = x.sizes().vec();
-    shape.back() = w2.size(0);
-    return y.view(shape);
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     differentiable_once("gated_ffn");
@@ -288,29 +298,18 @@ OptT gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2,
   if (!x.is_cuda() || !half || x.size(-1) % 8 || w2.size(0) % 8 || w2.size(1) % 8) return OptT();
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w13) || wants_grad(w2) || wants_grad(residual)))
     return GatedFfn::apply(x, w13, w2, residual, act);
-  const at::Tensor y = std::get<0>(
-      gated_ffn_fwd(rows2d(x), w13, w2, residual ? OptT(rows2d(*residual)) : OptT(), act, false));
-  if (x.dim() == 2) return y;
-  auto shape = x.sizes().vec();
-  shape.back() = w2.size(0);
-  return y.view(shape);
-}
-
-// x [..., width] as rows with unit inner stride
-at::Tensor norm_rows(const at::Tensor& x) {
-  const at::Tensor r = rows2d(x);
-  return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
+  return std::get<0>(gated_ffn_fwd(x, w13, w2, residual, act, false));
 }
 
 struct TrainNorm : torch::autograd::Function<TrainNorm> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const OptT& b, double eps,
                             bool rms) {
     const at::Tensor wc = w.contiguous();
-    auto [y, mean, rstd] = norm_train_fwd(norm_rows(x), wc, b ? OptT(b->contiguous()) : OptT(), eps, rms, true);
+    auto [y, mean, rstd] = norm_train_fwd(x, wc, b ? OptT(b->contiguous()) : OptT(), eps, rms, true);
     ctx->save_for_backward({x, w, val(mean), val(rstd)});
     ctx->saved_data["rms"] = rms;
     ctx->saved_data["bias"] = b.has_value();
-    return y.view(x.sizes());
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     differentiable_once(ctx->saved_data["rms"].toBool() ? "rms_norm" : "layer_norm");
@@ -331,9 +330,7 @@ at::Tensor train_norm(const at::Tensor& x, const at::Tensor& w, const OptT& b, d
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "norm: x [..., width]");
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return TrainNorm::apply(x, w, b, eps, rms);
-  const at::Tensor y = std::get<0>(norm_train_fwd(norm_rows(x), w.contiguous(), b ? OptT(b->contiguous()) : OptT(), eps,
-                                                  rms, false));
-  return x.dim() == 2 ? y : y.view(x.sizes());
+  return std::get<0>(norm_train_fwd(x, w.contiguous(), b ? OptT(b->contiguous()) : OptT(), eps, rms, false));
 }
 
 struct Dropout : torch::autograd::Function<Dropout> {

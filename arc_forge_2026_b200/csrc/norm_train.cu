@@ -487,7 +487,7 @@ static Kernel kernel_of(int nv, bool vec, int wpr) {
   }
 }
 
-constexpr int RING_SMEM = 180 * 1024;  // of an SM; the kernels' static shared memory is below 16 KB a CTA
+constexpr int RING_SMEM = 160 * 1024;  // of an SM; four CTAs' static shared memory (13 KB each) fits beside it
 
 // Chunks a lane, warps a row, rows a CTA, CTAs, ring. Forward, the instructions a row takes decide the first two: some 8
 // an element and 75 a warp for its sums, so few warps with much each, as far as the lanes' last chunks are not left
@@ -521,7 +521,7 @@ static int plan(const NormArgs& a, int num_sms, Shape& s, Kernel& kern) {
     cudaError_t e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_SMEM);
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, warps * 32, 0);
     if (e != cudaSuccess) return (int)e;
-    per_sm = std::max(1, std::min(per_sm, 8));
+    per_sm = std::max(1, std::min(per_sm, BWD ? 4 : 8));
     r.store(per_sm, std::memory_order_relaxed);
   }
   const int64_t blocks = (a.rows + s.groups - 1) / s.groups;

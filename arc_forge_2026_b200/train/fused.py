@@ -119,7 +119,7 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
     """Zero-centred RMSNorm ``x / rms(x) * (1 + w)`` of ``models.reference.rms_norm``: a frozen w at the model's widths
     in bf16 on the student's kernel, a trainable w (gradient of w in w's type), any other width up to 16,384, fp16
     and fp32 on the trainable norm's."""
-    if kernels.use("rms_norm") and _norm_ok(x, w):
+    if kernels.use("rms_norm") and not w.requires_grad and _norm_ok(x, w):
         kernels.hit("rms_norm", True)
         return _RMSNorm.apply(x, w.float().contiguous(), eps, None)
     if kernels.use("rms_norm") and w.shape == x.shape[-1:] and _train_norm_ok(x, w):

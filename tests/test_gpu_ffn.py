@@ -540,3 +540,44 @@ def test_gpu_refusals():
     check(y, *norm_oracle(wide, torch.ones(16392, device=dev), None, wide, 1e-6, False)["y"], "wide")
     z = torch.randn(4, 16, dtype=torch.float64, device=dev)
     assert torch.equal(fused.dropout(z, 0.5, 3).cpu(), fused.dropout(z.cpu(), 0.5, 3))
+
+
+def test_results_can_be_changed_in_place_and_graphs_walked_twice():
+    x, w13, w2, res, dy = ffn_inputs(24, 32, 16, 32, BF, seed=20)
+    nw = torch.ones(32, device=dev, dtype=BF)
+    for f in (lambda t: gated_ffn(t, w13, w2), lambda t: fused.layer_norm(t, nw), lambda t: fused.rms_norm(t, nw, 1e-6),
+              lambda t: fused.dropout(t, 0.3, 4)):
+        for shape in ((24, 32), (2, 3, 4, 32)):
+            leaf = x.view(shape).clone().requires_grad_(True)
+            y = f(leaf)
+            y += 1
+            y.mul_(2)
+            (a,) = torch.autograd.grad(y, leaf, dy.view(y.shape), retain_graph=True)
+            (b,) = torch.autograd.grad(y, leaf, dy.view(y.shape))
+            assert torch.equal(a, b)
+            (c,) = torch.autograd.grad(f(leaf), leaf, 2 * dy.view(y.shape))
+            assert torch.equal(a, c)
+    # a saved input changed in place before the backward pass is refused
+    leaf = x.clone().requires_grad_(True)
+    z = leaf * 1
+    y = gated_ffn(z, w13, w2)
+    z.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_single_vectors_and_broadcast_rows():
+    """1-D inputs are one row; an expanded input (row stride 0) gives the gradient of the row it repeats."""
+    x, w13, w2, res, dy = ffn_inputs(9, 64, 24, 40, BF, seed=21)
+    w = (1 + 0.1 * torch.randn(64, generator=torch.Generator().manual_seed(1))).to(dev)
+    assert torch.equal(gated_ffn(x[0], w13, w2), gated_ffn(x[:1], w13, w2)[0])
+    assert torch.equal(fused.layer_norm(x[0], w), fused.layer_norm(x[:1], w)[0])
+    one = x[:1].clone().requires_grad_(True)
+    rows = one.expand(9, 64)
+    dn = torch.randn(9, 64, generator=torch.Generator().manual_seed(2)).to(BF).to(dev)
+    full = x[:1].repeat(9, 1).requires_grad_(True)
+    for f, d in ((lambda t: gated_ffn(t, w13, w2), dy), (lambda t: fused.layer_norm(t, w), dn)):
+        (a,) = torch.autograd.grad(f(rows), one, d, retain_graph=True)
+        (b,) = torch.autograd.grad(f(full), full, d)
+        assert torch.equal(a, b.sum(0, keepdim=True, dtype=BF))
+    check_status()
