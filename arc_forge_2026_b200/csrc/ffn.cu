@@ -3,16 +3,20 @@
 //   g = x Wg^T, u = x Wu^T, h = act(g) u      one kernel: a 256-column accumulator tile is 128 gate columns beside
 //                                             the same 128 up columns, so an epilogue thread holds both of a pair
 //   y = h W2^T (+ residual)
-//   dh = dy W2, dg = dh u act'(g), du = dh act(g)   one kernel, the activation's gradient in the epilogue
+//   dh = dy W2, dg = dh p, du = dh q          one kernel; p = u act'(g) and q = act(g) come from the forward epilogue
 //   dx = [dg | du] [Wg; Wu]
 //   dW13 = [dg | du]^T x, dW2 = dy^T h        both operands of these have the reduced index (the rows) outermost
 //
 // The five products share one kernel, templated on which operand has K contiguous (K-major) and which has M or N
 // contiguous (MN-major; read in place through the MN-major form of the shared-memory descriptor, so nothing is ever
 // transposed in memory), and on the epilogue. Sums are fp32 in TMEM. h and [dg | du] are rounded once to the element
-// type because the tensor cores take them as operands; g and u are kept in fp32 for the backward pass, since a
-// second rounding there would show in dx and dW13. Split-K partial sums are fp32 and added in a fixed order: every
-// result is bitwise reproducible.
+// type because the tensor cores take them as operands; p and q are kept in fp32 for the backward pass, since a second
+// rounding there would show in dx and dW13. Split-K partial sums are fp32 and added in a fixed order: every result is
+// bitwise reproducible. Up to 128 rows the forward pass has kernels of its own (below).
+//
+// Measured (one B200, kernels alone, TFLOP/s of 1,646 measured for a library GEMM): 4,100 x 2,048 x 6,144 forward DUAL
+// 155 us (1,330) and y 77 (1,340), backward DACT 93 (1,110), dx 145 (1,420), the weight gradients 230 (1,350); a product
+// of 8,192^3 735 (1,496). What is lost: the last wave of tiles (8 % on average there) and some 5 us a launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -59,7 +63,7 @@ struct Args {
   const void* residual = nullptr;  // STORE, optional
   int64_t ldr = 0;
   Grads grads;           // GRADS
-  float* f32 = nullptr;  // PARTIAL: sums [splits, M in whole tiles, N]; DUAL: g and u (at_gu) or null; DACT: g and u
+  float* f32 = nullptr;  // PARTIAL: sums [splits, M in whole tiles, N]; DUAL: p and q (at_gu) or null; DACT: p and q
 };
 // tensor maps: operands; the 16-bit result (STORE, DUAL h, DACT dg), and DACT's du; GRADS: of each product
 template <int LAYOUT>
@@ -67,7 +71,7 @@ struct Maps {
   CUtensorMap a[LAYOUT == GRADS ? 3 : 1], b[LAYOUT == GRADS ? 3 : 1], out[LAYOUT == GRADS ? 3 : 2];
 };
 
-// g and u are kept as the epilogue's threads hold them, 32 rows x 8 columns (32 bytes a row) at a time: a warp's access
+// p and q are kept as the epilogue's threads hold them, 32 rows x 8 columns (32 bytes a row) at a time: a warp's access
 // is 1 KB in one piece. (Row-major, a warp's 32-byte pieces of 32 rows cost four times the L1 cycles, which the MMAs'
 // operands need too: 187 against 152 us for the forward product at 4,100 x 2,048 x 6,144.)
 AFB_DEV int64_t at_gu(int64_t row, int col, int F, int half) {
@@ -335,7 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       fence_proxy_async_smem();
       __syncwarp();
     };
-    // DACT: g and u of 16 columns, two chunks ahead of their use
+    // DACT: p and q of 16 columns, two chunks ahead of their use
     float gq[2][EPI == DACT ? 16 : 1], uq[2][EPI == DACT ? 16 : 1];
     struct GuTile {
       const float *g, *u;  // this lane's first column of the tile, or null where its row is outside the result
@@ -645,7 +649,7 @@ struct FewArgs {
   int chunk = 0;     // rows of a CTA (gridDim.z chunks)
   int K = 0, F = 0, act = 0;
   void* out = nullptr;             // DUAL: h [2T, F]; else y [T, n]
-  float* gu = nullptr;             // DUAL: g and u (at_gu) or null
+  float* gu = nullptr;             // DUAL: p and q (at_gu) or null
   const void* residual = nullptr;  // else: [T, n] or null
   int64_t ldr = 0;
   const void* next = nullptr;      // DUAL: the down projection's weights, `next_bytes` of them (a multiple of 16)

@@ -5,6 +5,7 @@
     python -m arc_forge_2026_b200.utils.kbench gdn_scan # chunked-GDN inter-chunk scan at the QAD shape
     python -m arc_forge_2026_b200.utils.kbench gdn_train # chunked-GDN layer forward + backward at the QAD shape
     python -m arc_forge_2026_b200.utils.kbench qsa      # QSA selection + sparse verify attention (block 4 and 64)
+    python -m arc_forge_2026_b200.utils.kbench ffn      # gated feed-forward, trainable norms, dropout (both directions)
     python -m arc_forge_2026_b200.utils.kbench vision   # the 27-block vision tower beside the HF bf16 model
 
 Prints one JSON line per kernel: time, bytes, FLOPs and the fraction of MEASURED_PEAKS.json.
@@ -523,6 +524,43 @@ def bench_grouped(E=320, T=16384, k=10, H=2048, I=512, seed=0):
     return res
 
 
+def bench_ffn(seed=0):
+    """The trainers' feed-forward operators: the gated block at the drafter's and the shared expert's sizes (one token to
+    a packed 16k bin), the norms with trainable weights and dropout, forward and with gradients."""
+    from ..train import fused
+    from ..train.ffn import gated_ffn
+    peaks = load_peaks()
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def rn(*s, k=1.0, dtype=torch.bfloat16):
+        return (torch.randn(*s, generator=g, device="cuda") * k).to(dtype).requires_grad_(True)
+    res = []
+
+    def add(name, fn, leaves, byts, flops=0):
+        def both():
+            y = fn()
+            torch.autograd.grad(y, leaves, torch.ones_like(y))
+        with torch.no_grad():
+            ms = time_cuda(fn)
+        for kind, t, k in (("fwd", ms, 1), ("fwd_bwd", time_cuda(both), 3)):
+            r = {"kernel": f"{name}_{kind}", "ms": round(t, 4)}
+            if flops:
+                r |= {"tflops": round(k * flops / t / 1e9, 1),
+                      "frac_bf16_of_measured": round(k * flops / t / 1e9 / peaks["bf16_tflops"], 3)}
+            b = byts if k == 1 else 2 * byts
+            res.append(r | {"gbs": round(b / t / 1e6, 1), "frac_hbm_of_measured": round(b / t / 1e6 / peaks["hbm_gbs"], 3)})
+    for T, H, I in ((1, 2048, 6144), (4096, 2048, 6144), (16384, 2048, 512)):
+        x, w13, w2 = rn(T, H), rn(2 * I, H, k=H ** -0.5), rn(H, I, k=I ** -0.5)
+        add(f"gated_ffn_T{T}_H{H}_F{I}", lambda: gated_ffn(x, w13, w2), [x, w13, w2], 4 * T * H + 6 * H * I, 6 * T * H * I)
+    for rows, width, dt in ((5632, 1152, torch.bfloat16), (16384, 2048, torch.bfloat16), (16384, 2048, torch.float32)):
+        x, w, b = rn(rows, width, dtype=dt), rn(width, dtype=torch.float32), rn(width, dtype=torch.float32)
+        byts = 2 * x.numel() * x.element_size()
+        add(f"layer_norm_{rows}x{width}_{str(dt)[6:]}", lambda: fused.layer_norm(x, w, b), [x, w, b], byts)
+    x = rn(16384, 2560)
+    add("dropout_16384x2560", lambda: fused.dropout(x, 0.1, 1), [x], 4 * x.numel())
+    return res
+
+
 def bench_ple(T=16384, base=250_000, seed=0):
     """PLE lookup of one packed 16k-token row: 16 heads (2- and 3-grams x 8) of 160 e4m3 dims from a table of
     ~4M rows (a quarter-size stand-in of the 20M-bucket heads; the gather is random either way)."""
@@ -608,7 +646,7 @@ def bench_gdn_train(B=1, T=16384, Hk=16, Hv=32):
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["moe", "gemm", "gdn", "attn", "qsa", "train_attn", "ref_triton", "gdn_scan", "gdn_train", "grouped", "ple", "vision", "all"])
+    ap.add_argument("what", choices=["moe", "gemm", "gdn", "attn", "qsa", "train_attn", "ref_triton", "gdn_scan", "gdn_train", "grouped", "ple", "ffn", "vision", "all"])
     ap.add_argument("--T", type=int, default=640)
     ap.add_argument("--S", type=int, default=128, help="sessions of the attn case")
     ap.add_argument("--seq", type=int, default=16384, help="sequence length of the gdn_scan / gdn_train cases")
@@ -635,6 +673,8 @@ def main():
         res += bench_gdn_scan(n=(a.seq + 63) // 64)
     if a.what in ("ple", "all"):
         res += bench_ple()
+    if a.what in ("ffn", "all"):
+        res += bench_ffn()
     if a.what in ("grouped", "all"):
         res += bench_grouped()
     if a.what in ("gdn_train", "all"):

@@ -303,7 +303,7 @@ def run_norm(x, w, b, dy, eps, rms):
     return dict(zip(("y", "dx", "dw", "db"), (y.detach(), *gs)))
 
 
-@pytest.mark.parametrize("W", [1, 7, 8, 33, 128, 256, 264, 768, 1001, 1024, 1152, 1160, 2048, 2056, 2560, 4095, 4608,
+@pytest.mark.parametrize("W", [1, 7, 8, 33, 128, 256, 264, 768, 1001, 1002, 1024, 1152, 1160, 2048, 2056, 2560, 4095, 4606, 4608,
                                5000, 8192, 8200, 16384])
 @pytest.mark.parametrize("rms", [False, True])
 def test_trainable_norms(W, rms):
@@ -319,8 +319,8 @@ def test_trainable_norms(W, rms):
 def test_norm_strides_empty_frozen_and_constant_rows():
     x, w, b, dy = norm_inputs(50, 264, BF, FP, seed=11)
     ref = norm_oracle(x, w, b, dy, 1e-6, False)
-    wide = torch.zeros(50, 300, dtype=BF, device=dev)
-    for off in (8, 3):  # an aligned view and one that is not
+    wide = torch.zeros(50, 304, dtype=BF, device=dev)
+    for off in (8, 2, 3):  # views whose rows start on 16 bytes, on 4 and on 2
         wide[:, off:off + 264] = x
         got = run_norm(wide[:, off:off + 264], w, b, dy.t().contiguous().t(), 1e-6, False)
         for k in got:
