@@ -193,9 +193,10 @@ AFB_DEV void put_half_row(uint8_t* buf, int row, const uint32_t* w) {
 // Persistent: pair p of the grid takes tiles p, p + pairs, ... Each CTA: warp 0 loads its halves of the operands by
 // TMA into a STAGES-deep ring, one thread of the leader's warp 1 issues the MMAs of both CTAs into one of two TMEM
 // accumulators, and 8 epilogue warps drain the other one (two warps a lane quadrant, half of the columns each) through
-// swizzled staging rows and TMA stores, so the tensor cores work through the next tile meanwhile. What bounds the tiles
-// is shared memory's bandwidth (a K block moves 80 KB of it a CTA: 600 cycles, where its MMAs take 512), so the
-// epilogue is kept to whole 128-byte lines.
+// swizzled staging rows and TMA stores, so the tensor cores work through the next tile meanwhile. A K block takes 600
+// cycles where its MMAs take 512, more ring stages do not change that (5 and 6 are equal), and every line an epilogue
+// moves through L1 or shared memory adds to it: by all signs shared memory's bandwidth bounds the tiles (a K block moves
+// 80 KB of it a CTA). So the epilogue is kept to whole 128-byte lines.
 template <int LAYOUT, int EPI, bool F16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     ffn_gemm_kernel(const __grid_constant__ Maps<LAYOUT> maps, Args g, uint32_t* status) {
