@@ -2,6 +2,7 @@
 // allocation of results and scratch on the tensors' own device, launch on that device's current stream, and their
 // autograd nodes (in C++: a small call's time is the host's, and a Python node costs several times the kernels).
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 
 #include "binding_utils.h"
 #include "ffn.h"
@@ -22,6 +23,24 @@ OptT opt(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 at::Tensor rows2d(const at::Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
 void differentiable_once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " is differentiable once: create_graph=True is not supported");
+}
+
+// A leaf's gradient goes to its accumulator on the stream on which the leaf was first used by a graph that still lives.
+// Where that is the default stream, a capture on another one would have to be joined by it, which CUDA forbids (and the
+// error can end the process): refused here, before it comes to that.
+void capturable_backward(const char* what) {
+  const auto node = torch::autograd::get_current_node();
+  const auto st = at::cuda::getCurrentCUDAStream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (!node || st.stream() == nullptr || cudaStreamIsCapturing(st.stream(), &status) != cudaSuccess ||
+      status == cudaStreamCaptureStatusNone)
+    return;
+  for (const auto& e : node->next_edges())
+    if (auto* acc = dynamic_cast<torch::autograd::AccumulateGrad*>(e.function.get())) {
+      const auto s = acc->stream();
+      TORCH_CHECK(!s || s->id() != 0, what, ": its backward pass is captured while a graph of the same leaf that was made",
+                  " outside the capture, on the default stream, is alive; release that graph first");
+    }
 }
 
 int elem_type(const at::Tensor& t, const char* what) {
@@ -262,6 +281,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     differentiable_once("gated_ffn");
+    capturable_backward("gated_ffn");
     const variable_list v = ctx->get_saved_variables();
     const at::Tensor& dy = grads[0];
     const bool need_x = ctx->needs_input_grad(0), need_w13 = ctx->needs_input_grad(1),
@@ -309,16 +329,30 @@ struct TrainNorm : torch::autograd::Function<TrainNorm> {
     ctx->save_for_backward({x, w, val(mean), val(rstd)});
     ctx->saved_data["rms"] = rms;
     ctx->saved_data["bias"] = b.has_value();
+    ctx->saved_data["eps"] = eps;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    differentiable_once(ctx->saved_data["rms"].toBool() ? "rms_norm" : "layer_norm");
+    const bool rms = ctx->saved_data["rms"].toBool(), need_x = ctx->needs_input_grad(0),
+               need_w = ctx->needs_input_grad(1),
+               need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    capturable_backward(rms ? "rms_norm" : "layer_norm");
     const variable_list v = ctx->get_saved_variables();
-    auto [dx, dw, db] = norm_train_bwd(rows2d(grads[0]), norm_rows(v[0]), v[1].contiguous(), opt(v[2]), v[3],
-                                       ctx->saved_data["rms"].toBool(), ctx->needs_input_grad(0),
-                                       ctx->needs_input_grad(1),
-                                       ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2));
     variable_list out(5);
+    if (at::GradMode::is_enabled()) {  // create_graph: the formulas in operations that can be differentiated again
+      const at::Tensor x = v[0].to(at::kFloat), w = v[1].to(at::kFloat), dy = grads[0].to(at::kFloat);
+      const at::Tensor c = rms ? x : x - x.mean({-1}, true);
+      const at::Tensor rstd = at::rsqrt(c.square().mean({-1}, true) + ctx->saved_data["eps"].toDouble());
+      const at::Tensor xh = c * rstd, g = dy * (rms ? 1. + w : w);
+      at::Tensor d = g - xh * (g * xh).mean({-1}, true);
+      if (!rms) d = d - g.mean({-1}, true);
+      if (need_x) out[0] = (rstd * d).to(v[0].scalar_type());
+      if (need_w) out[1] = rows2d(dy * xh).sum(0).to(v[1].scalar_type());
+      if (need_b) out[2] = rows2d(dy).sum(0).to(v[1].scalar_type());
+      return out;
+    }
+    auto [dx, dw, db] = norm_train_bwd(rows2d(grads[0]), norm_rows(v[0]), v[1].contiguous(), opt(v[2]), v[3], rms,
+                                       need_x, need_w, need_b);
     if (dx) out[0] = dx->view(v[0].sizes());
     out[1] = val(dw);
     out[2] = val(db);
@@ -345,6 +379,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     differentiable_once("dropout");
+    capturable_backward("dropout");
     variable_list out(6);
     if (ctx->needs_input_grad(0))
       out[0] = dropout_op(grads[0], OptT(), ctx->saved_data["threshold"].toInt(), ctx->saved_data["seed"].toInt(),

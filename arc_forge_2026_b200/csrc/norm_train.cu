@@ -238,7 +238,8 @@ struct Ring {
   }
 };
 
-// a group's threads leave together: one that gave up waiting says so before the row's barrier
+// A group's threads leave together: one that gave up waiting says at which row before that row's barrier (a later row's
+// number does not stop a warp that has yet to look: it meets the others at that row's barrier)
 AFB_DEV void group_sync(const Group& g) {
   if (g.wpr > 1) named_bar_sync(1 + g.idx, g.lanes);
   else __syncwarp();
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(NormArgs a, int wpr, int
     for (int i = 0; i < rs.depth; ++i) mbar_init(&full_s[g.idx][i], 1);
     fence_mbar_init();
     fence_proxy_async_smem();
-    *bad = 0;
+    *bad = INT32_MAX;
   }
   __syncthreads();
   grid_dep_wait();
@@ -288,13 +289,13 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(NormArgs a, int wpr, int
   T* y = reinterpret_cast<T*>(a.y) + row0 * a.width;
   int k = 0;
   for (; k < n; ++k, ring.next(), y += stride * a.width) {
-    if (!ring.wait()) *bad = 1;
+    if (!ring.wait()) *bad = k;
     const T* x = reinterpret_cast<const T*>(ring.slot + (V == 8 ? 0 : reinterpret_cast<uintptr_t>(ring.x) & 15));
     float v[NV][8];
 #pragma unroll
     for (int p = 0; p < NV; ++p) unpack(load_chunk<V>(x, g, p, a.width), v[p]);
     group_sync(g);  // the slot has been read
-    if (*bad) break;
+    if (*bad <= k) break;
     if (g.t == 0 && k + rs.depth < n) ring.refill();
     float mean = 0.f;
     if (!a.rms) {
@@ -347,7 +348,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_bwd_kernel(NormArgs a, int wp
     for (int i = 0; i < rs.depth; ++i) mbar_init(&full_s[g.idx][i], 1);
     fence_mbar_init();
     fence_proxy_async_smem();
-    *bad = 0;
+    *bad = INT32_MAX;
   }
   __syncthreads();
   grid_dep_wait();
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_bwd_kernel(NormArgs a, int wp
       my_rstd = a.rstd[row0 + (k + lane) * stride];
       if (!a.rms) my_mean = a.mean[row0 + (k + lane) * stride];
     }
-    if (!ring.wait()) *bad = 1;
+    if (!ring.wait()) *bad = k;
     const T* x = reinterpret_cast<const T*>(ring.slot + (V == 8 ? 0 : reinterpret_cast<uintptr_t>(ring.x) & 15));
     const T* dy = reinterpret_cast<const T*>(ring.slot + rs.part + (V == 8 ? 0 : reinterpret_cast<uintptr_t>(ring.dy) & 15));
     float h[NV][8], v[NV][8];
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(MAXT, MINB) norm_bwd_kernel(NormArgs a, int wp
       unpack(load_chunk<V>(dy, g, p, a.width), v[p]);
     }
     group_sync(g);  // the slot has been read
-    if (*bad) break;
+    if (*bad <= k) break;
     if (g.t == 0 && k + rs.depth < n) ring.refill();
     const float r = __shfl_sync(0xffffffffu, my_rstd, k & 31), mu = __shfl_sync(0xffffffffu, my_mean, k & 31);
     float2 s = make_float2(0.f, 0.f);
@@ -515,9 +516,10 @@ constexpr int RING_SMEM = 160 * 1024;  // of an SM; four CTAs' static shared mem
 
 // Chunks a lane, warps a row, rows a CTA, CTAs, ring. Forward, the instructions a row takes decide the first two: some 8
 // an element and 75 a warp for its sums, so few warps with much each, as far as the lanes' last chunks are not left
-// idle (5,632 rows of 1,152 in bf16: three chunks 11 us, one 14, two 15, four 14). Backward, two chunks a lane (16,384 rows of 2,048 in bf16: 46 us; one chunk 61, for the sums of twice the warps;
-// three 70 and four 65, for want of registers), one where a row is 512 columns or less, four where it passes 8,192, and
-// three from 4,097 to 4,608, where two would leave an SM one CTA.
+// idle (5,632 rows of 1,152 in bf16: three chunks 11 us, one 14, two 15, four 14). Backward, two chunks a lane (16,384
+// rows of 2,048 in bf16: 46 us; one chunk 61, for the sums of twice the warps; three 70 and four 65, for want of
+// registers), one where a row is 512 columns or less, four where it passes 8,192, and three from 4,097 to 4,608, where
+// two would leave an SM one CTA.
 // CTAs: as many as are resident (a second wave would wait for the first). The ring takes what shared memory the SM's
 // CTAs leave each other, up to 8 rows.
 template <typename T, bool BWD>

@@ -140,8 +140,8 @@ def layer_norm_reference(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | Non
 
 
 def layer_norm(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
-    """LayerNorm ``(x - mean) / sqrt(var + eps) * w (+ b)`` over the last dim (1 to 16,384 wide), differentiable (once)
-    in x, w and b; x bf16, fp16 or fp32, w and b in x's type or fp32 (their gradients come in their own type).
+    """LayerNorm ``(x - mean) / sqrt(var + eps) * w (+ b)`` over the last dim (1 to 16,384 wide), differentiable in x, w
+    and b; x bf16, fp16 or fp32, w and b in x's type or fp32 (their gradients come in their own type).
     Statistics and sums are fp32 and of fixed order."""
     if x.dim() < 1 or w.shape != x.shape[-1:] or (b is not None and b.shape != w.shape):
         raise ValueError(f"layer_norm: x {tuple(x.shape)}, w {tuple(w.shape)}"

@@ -303,8 +303,8 @@ def run_norm(x, w, b, dy, eps, rms):
     return dict(zip(("y", "dx", "dw", "db"), (y.detach(), *gs)))
 
 
-@pytest.mark.parametrize("W", [1, 7, 8, 33, 128, 256, 264, 768, 1001, 1002, 1024, 1152, 1160, 2048, 2056, 2560, 4095, 4606, 4608,
-                               5000, 8192, 8200, 16384])
+@pytest.mark.parametrize("W", [1, 7, 8, 33, 128, 256, 264, 768, 1001, 1002, 1024, 1152, 1160, 2048, 2056, 2560, 4095,
+                               4606, 4608, 5000, 8192, 8200, 16384])
 @pytest.mark.parametrize("rms", [False, True])
 def test_trainable_norms(W, rms):
     for i, (dt, wdt, T) in enumerate([(BF, FP, 37), (BF, BF, 700), (HF, HF, 5), (HF, FP, 1), (FP, FP, 300)]):
@@ -492,7 +492,7 @@ def test_lora_dropout_on_the_native_products():
 
 def test_checkpointed_student_layer_and_second_derivatives():
     """Activation checkpointing recomputes the same values (dropout masks among them) through the C++ autograd nodes;
-    create_graph is refused instead of giving second derivatives that lack terms."""
+    create_graph is refused where it would give second derivatives that lack terms."""
     from arc_forge_2026_b200.config import preset
     from arc_forge_2026_b200.train import lora
     from arc_forge_2026_b200.train.student import random_student
@@ -511,8 +511,7 @@ def test_checkpointed_student_layer_and_second_derivatives():
     for u, v in zip(a, b):
         assert torch.equal(u, v)
     x, w13, w2, res, dy = ffn_inputs(8, 16, 8, 16, BF)
-    for f in (lambda t: gated_ffn(t, w13, w2), lambda t: fused.layer_norm(t, w2[0].new_ones(16), None),
-              lambda t: fused.dropout(t, 0.5, 1)):
+    for f in (lambda t: gated_ffn(t, w13, w2), lambda t: fused.dropout(t, 0.5, 1)):
         leaf = x.clone().requires_grad_(True)
         with pytest.raises(RuntimeError, match="differentiable once"):
             torch.autograd.grad(f(leaf).float().sum(), leaf, create_graph=True)
@@ -580,4 +579,83 @@ def test_single_vectors_and_broadcast_rows():
         (a,) = torch.autograd.grad(f(rows), one, d, retain_graph=True)
         (b,) = torch.autograd.grad(f(full), full, d)
         assert torch.equal(a, b.sum(0, keepdim=True, dtype=BF))
+    check_status()
+
+
+@pytest.mark.parametrize("rms", [False, True])
+def test_norm_second_derivatives(rms):
+    """create_graph through the norms: the second derivatives equal autograd's of the plain form in fp64."""
+    g = torch.Generator().manual_seed(21)
+    x, w, b, dy, k = (torch.randn(*s, generator=g).to(dev) for s in ((6, 40), (40,), (40,), (6, 40), (6, 40)))
+
+    def second(f, *ts):
+        ls = [t.clone().requires_grad_(True) for t in ts]
+        y = f(*ls)
+        first = torch.autograd.grad(y, ls, dy.to(y.dtype), create_graph=True)
+        return [*first, *torch.autograd.grad((first[0] * k.to(y.dtype)).sum() + first[1].square().sum(), ls[:2])]
+
+    def plain(x, w, *b):
+        c = x if rms else x - x.mean(-1, keepdim=True)
+        y = c * torch.rsqrt(c.square().mean(-1, keepdim=True) + 1e-5) * (1 + w if rms else w)
+        return y if rms else y + b[0]
+    ts = (x, w) if rms else (x, w, b)
+    got = second((lambda x, w: fused.rms_norm(x, w, 1e-5)) if rms else (lambda x, w, b: fused.layer_norm(x, w, b)), *ts)
+    want = second(plain, *(t.double() for t in ts))
+    for a, r in zip(got, want):
+        # sums of at most 40 x 6 terms, each the product of a few fp32 values; inputs and derivatives of order 1 to 100
+        assert (a.double() - r).abs().max() <= 2 * 240 * E * max(1.0, float(r.detach().abs().max())) * 4
+
+
+def test_backward_captured_while_an_eager_graph_of_the_leaves_lives_is_refused():
+    """The accumulators of the living graph are on the default stream, which may not join a capture."""
+    x, w13, w2, _, dy = ffn_inputs(40, 64, 32, 64, BF, seed=9)
+    w = torch.ones(64, device=dev)
+    calls = ((lambda x, a, b, w: gated_ffn(x, a, b)), (lambda x, a, b, w: fused.layer_norm(x, w)),
+             (lambda x, a, b, w: fused.dropout(x, 0.5, 1)))
+    for f in calls:
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w13, w2, w)]
+        alive = f(*leaves)  # noqa: F841
+        gr = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="release that graph first"):
+            with torch.cuda.graph(gr):
+                f(*leaves).backward(dy)
+        torch.cuda.synchronize()
+        del alive
+        for t in leaves:
+            assert t.grad is None
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            f(*leaves).backward(dy)
+        gr.replay()
+        ref = [t.detach().clone().requires_grad_(True) for t in leaves]
+        f(*ref).backward(dy)
+        for a, r in zip(leaves, ref):
+            assert (a.grad is None) == (r.grad is None) and (r.grad is None or torch.equal(a.grad, r.grad))
+    check_status()
+
+
+def test_calls_on_two_streams_at_once():
+    """Workspaces belong to a call: the same operators, run on two streams at the same time, give what they give alone."""
+    def work(t, w):
+        out = []
+        for i in range(4):
+            out += run_ffn(*t, "silu").values()
+            leaf = t[0].clone().requires_grad_(True)
+            y = fused.dropout(fused.rms_norm(leaf, w, 1e-6), 0.3, i)
+            out += [y, *torch.autograd.grad(y, leaf, t[0])]
+        return out
+    data = [(ffn_inputs(T, 256, 264, 256, BF, seed=T), torch.randn(256, device=dev).requires_grad_(True))
+            for T in (1500, 90)]
+    alone = [work(*d) for d in data]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in data]
+    both = []
+    for d, s in zip(data, streams):
+        with torch.cuda.stream(s):
+            both.append(work(*d))
+    torch.cuda.synchronize()
+    for a, b in zip(alone, both):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
     check_status()
