@@ -125,6 +125,23 @@ def test_gated_ffn_row_counts_of_serving(T):
     check(y, *ref["y"], T)
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("size", [(8, 8, 8), (264, 1032, 520), (1024, 2056, 1024), (2048, 1544, 2048)])
+def test_gated_ffn_single_tokens(size, T):
+    """One to five rows, on both sides of where the kernels change (rows and bytes of weights); fp16 and bf16, rows of
+    a wider tensor, with and without what the backward pass reads."""
+    for dt, act in ((BF, "silu"), (HF, "gelu")):
+        x, w13, w2, res, dy = ffn_inputs(T, size[0], size[1], size[2], dt, seed=T)
+        wide = torch.full((T, size[0] + 8), float("nan"), dtype=dt, device=dev)
+        wide[:, :size[0]] = x
+        got = run_ffn(x, w13, w2, res, dy, act)
+        for k, (want, bound) in ffn_oracle(x, w13, w2, res, dy, act).items():
+            check(got[k], want, bound, k)
+        with torch.no_grad():
+            assert torch.equal(gated_ffn(wide[:, :size[0]], w13, w2, act=act, residual=res), got["y"])
+    check_status()
+
+
 def test_gated_ffn_gradient_against_differences():
     """<gradient, direction> of the kernels against the central difference of the fp64 block along the direction."""
     x, w13, w2, res, dy = ffn_inputs(96, 128, 200, 64, BF, seed=3)
