@@ -12,7 +12,7 @@
 // transposed in memory), and on the epilogue. Sums are fp32 in TMEM. h and [dg | du] are rounded once to the element
 // type because the tensor cores take them as operands; p and q are kept in fp32 for the backward pass, since a second
 // rounding there would show in dx and dW13. Split-K partial sums are fp32 and added in a fixed order: every result is
-// bitwise reproducible. Up to 128 rows the forward pass has kernels of its own (below), and others for one to four.
+// bitwise reproducible. Up to 128 rows the forward pass has kernels of its own (below), and others for one to sixteen.
 //
 // Measured (one B200, kernels alone, TFLOP/s of 1,646 measured for a library GEMM): 4,100 x 2,048 x 6,144 forward DUAL
 // 155 us (1,330) and y 77 (1,340), backward DACT 93 (1,110), dx 145 (1,420), the weight gradients 230 (1,350); a product
@@ -931,21 +931,30 @@ static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void
   return few_rows<false, NT, F16>(w2, s.N, {h, s.F}, 2 * s.T, g, status, st);
 }
 
-// ------------------------------------------------------------------------------------------ one to four rows
-// One or two rows are dot products on the CUDA cores: the FMAs of a row keep pace with HBM (2,048 x 6,144: some 3 us of
-// them beside 11.5 us of loads), and a CTA has no ring to fill and no TMEM or cluster to wait for. A CTA takes two columns
-// of h (four weight rows) or two of y; its four warps share K in chunks of 256, so that a row's values are loaded once for
-// all weight rows and every weight load is 512 bytes in one piece. Small CTAs, many an SM, keep enough loads on the way
-// (eight warps and four columns a CTA: 18.5 us where this takes 15.4). h goes from one kernel to the other in fp32.
-// Measured, here and as the tensor cores' kernels for few rows (us): one row 2,048 x 6,144 15.4 and 20.6, 5,120 x 17,408
-// 82 and 93 (6.5 TB/s and 5.7), 2,048 x 512 4.5 and 8.7; two rows 17.5 and 20.8, 96 and 93, 5.1 and 8.7. Four rows lack
-// registers for loads enough: 27.5 and 21 at 2,048 x 6,144 and 15.4 and 14.2 at 1,152 x 4,304 (30 MB of weights), but 6.4
-// and 8.7 at 2,048 x 512 and 7.6 and 10.1 at 2,560 x 640 (10 MB), where latency counts: three and four rows come here up
-// to DOT_BYTES of weights.
-constexpr int DOT = 4, DOT_COLS = 2, DOT_WARPS = 4;
-constexpr int64_t DOT_BYTES = 16 << 20;
-static bool dots(const FfnShape& s) {
-  return s.T <= 2 || (s.T <= DOT && (2 * (int64_t)s.H + s.N) * s.F * 2 <= DOT_BYTES);
+// ------------------------------------------------------------------------------------------ one to sixteen rows
+// Here a launch's latency counts beside the weights' bytes, and the kernels above have a ring to fill, TMEM to allocate
+// and read and two cluster barriers. These read the weights straight into registers and add a CTA's partial sums, one
+// share of K a warp, through shared memory. h goes from the first to the second in two terms, as above.
+//
+// One row: dot products on the CUDA cores, whose FMAs keep pace with HBM (2,048 x 6,144: some 3 us of them beside 11.5 us
+// of loads). A CTA takes two columns of h (four weight rows) or two of y; its four warps take chunks of 256 elements, so
+// every load is 512 bytes of a row in one piece. Small CTAs, many an SM, keep enough loads on the way (eight warps and
+// four columns a CTA: 18.5 us where this takes 14.8).
+//
+// More rows: mma.sync, for a lane can load 16 bytes of "its" weight row as they lie and hand them on as fragments. K may
+// come in any order if weights and rows agree, so lane 4 r + c takes elements 8 c .. 8 c + 7 of a block of 32 of row r:
+// two MMAs' worth. A CTA takes 8 columns of h (its MMA's 16 weight rows are the 8 gate and the 8 up rows, so a
+// thread ends with both of a pair) or 16 of y. FMAs instead, with the rows' values in registers: 2 rows 18.4 us at
+// 2,048 x 6,144 and 14.3 at 1,152 x 4,304, 4 rows 27 and 15; this 18.3 and 10.7, 18.8 and 11.0.
+//
+// Measured, us here and in the kernels above: one row 2,048 x 6,144 15 and 20.6, 5,120 x 17,408 86 and 93 (6.2 TB/s and
+// 5.7), 2,048 x 512 4.7 and 8.7. Eight rows 2,048 x 512 5.5 and 9.0, 2,048 x 2,048 7.4 and 12.3, 2,048 x 6,144 (75 MB of
+// weights) 19.5 and 20.9, 5,120 x 17,408 (535 MB) 120 and 89, for a row's 64 bytes at a time are less than HBM wants.
+// Sixteen rows 2,048 x 512 5.2 and 9.3, 2,048 x 2,048 (25 MB) 10.6 and 12.6, 1,152 x 4,304 (30 MB) 16.2 and 14.7. 24 rows:
+// 2,048 x 512 7.8 and 9.9, 2,560 x 640 11.4 and 11.1.
+static bool tokens(const FfnShape& s) {
+  const int64_t bytes = (2 * (int64_t)s.H + s.N) * s.F * 2;
+  return s.T == 1 || (s.T <= 8 && bytes <= 96 << 20) || (s.T <= 16 && bytes <= 24 << 20);
 }
 
 // not by way of L1, which another kernel on the SM may have filled before the weights were written
@@ -957,22 +966,42 @@ AFB_DEV uint4 ld_weights(const void* p) {
                : "memory");
   return v;
 }
-// eight elements as pairs, and the multiply-add of pairs (two a lane and instruction)
-AFB_DEV uint64_t pair_of(float2 v) { return *reinterpret_cast<uint64_t*>(&v); }
-AFB_DEV float2 of_pair(uint64_t v) { return *reinterpret_cast<float2*>(&v); }
-template <bool F16>
-AFB_DEV void unpack8(const uint4& q, uint64_t* f) {
-  const uint32_t r[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = pair_of(unpack2<F16>(r[i]));
+AFB_DEV void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+struct TokenArgs {
+  int T = 0, n = 0, K = 0, act = 0;  // rows; columns of the result (DUAL: F)
+  const void* w = nullptr;           // [n or 2 n, K]
+  const void* x = nullptr;           // DUAL: [T, K]; else h [2T, K]
+  int64_t ldx = 0;
+  void* out = nullptr;             // DUAL: h [2T, F]; else y [T, n]
+  float* gu = nullptr;             // DUAL: p and q (at_gu) or null
+  const void* residual = nullptr;  // else: [T, n] or null
+  int64_t ldr = 0;
+};
+// from the sums of one element (DUAL: gate a and up u; else a) to what is stored
+template <bool DUAL_, bool F16>
+AFB_DEV void finish(const TokenArgs& g, int t, int col, float a, float u) {
+  uint16_t* out = reinterpret_cast<uint16_t*>(g.out) + (int64_t)t * g.n + col;
+  if constexpr (DUAL_) {
+    float d;
+    with_act(g.act, [&](auto A) { act_grad<A.value>(a, a, d); });
+    if (g.gu) {
+      g.gu[at_gu(t, col, g.n, 0)] = u * d;
+      g.gu[at_gu(t, col, g.n, 1)] = a;
+    }
+    const float h = a * u;
+    const uint32_t hi = pack2<F16>(h, 0.f);
+    const float f = unpack2<F16>(hi).x;
+    out[0] = (uint16_t)hi;
+    out[(int64_t)g.T * g.n] = (uint16_t)pack2<F16>(isfinite(f) ? h - f : 0.f, 0.f);
+  } else {
+    if (g.residual) a += unpack2<F16>(reinterpret_cast<const uint16_t*>(g.residual)[t * g.ldr + col]).x;
+    out[0] = (uint16_t)pack2<F16>(a, 0.f);
+  }
 }
-AFB_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
+
 // Sums of V values over a warp's lanes, each left in the lanes whose top bits are its index: a step exchanges half of
-// the values that are left, so 32 values take 31 shuffles
+// the values that are left
 template <int V>
 AFB_DEV float warp_sums(float* v) {
   const int lane = threadIdx.x & 31;
@@ -986,130 +1015,202 @@ AFB_DEV float warp_sums(float* v) {
       v[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
     }
   }
+#pragma unroll
   for (; bit > 0; bit >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);
   return v[0];
 }
+template <bool F16>
+AFB_DEV void unpack8(const uint4& q, float* f) {
+  const uint32_t r[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = unpack2<F16>(r[i]);
+    f[2 * i] = v.x, f[2 * i + 1] = v.y;
+  }
+}
 
-struct DotArgs {
-  int T = 0, n = 0, K = 0, act = 0;  // rows; columns of the result (DUAL: F)
-  const void* w = nullptr;           // [n or 2 n, K]
-  const void* x = nullptr;           // DUAL: [T, K]; else h in fp32 [T, K]
-  int64_t ldx = 0;
-  void* out = nullptr;             // DUAL: h [T, F]; else y [T, n]
-  float* h32 = nullptr;            // DUAL: h in fp32 [T, F]
-  float* gu = nullptr;             // DUAL: p and q (at_gu) or null
-  const void* residual = nullptr;  // else: [T, n] or null
-  int64_t ldr = 0;
-};
+constexpr int ROW_WARPS = 4, ROW_COLS = 2;
 
-// TT: rows (1, 2 or 4; a row past the last is computed as the last and left out)
-template <bool DUAL_, int TT, bool F16>
-__global__ void __launch_bounds__(32 * DOT_WARPS) ffn_dot_kernel(DotArgs g) {
-  // result columns, weight rows, chunks at a time, sums
-  constexpr int R = DOT_COLS, WR = DUAL_ ? 2 * R : R, U = DUAL_ ? 1 : 2, V = WR * TT;
-  __shared__ float red[DOT_WARPS][V];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * R;
+template <bool DUAL_, bool F16>
+__global__ void __launch_bounds__(32 * ROW_WARPS) ffn_row_kernel(TokenArgs g) {
+  // weight rows; chunks a warp has on the way at a time (half of them: 17.0 us at 2,048 x 6,144 and 12.3 at 1,152 x 4,304,
+  // where these take 14.8 and 9.0)
+  constexpr int WR = DUAL_ ? 2 * ROW_COLS : ROW_COLS, U = DUAL_ ? 2 : 4, STEP = ROW_WARPS * 256;
+  __shared__ float red[ROW_WARPS][WR];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n0 = blockIdx.x * ROW_COLS, first = warp * 256 + lane * 8;
   const uint16_t* w = reinterpret_cast<const uint16_t*>(g.w) + (int64_t)n0 * g.K;
-  auto row_of = [&](int r) { return w + (int64_t)(r < R ? r : g.n + r - R) * g.K; };
+  auto row_of = [&](int r) { return w + (int64_t)(r < ROW_COLS ? r : g.n + r - ROW_COLS) * g.K; };
   uint4 q[U][WR];
   auto load = [&](int k0) {  // this lane's 8 elements of a weight row and chunk
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * DOT_WARPS * 256;
-      if (k < g.K) {
+    for (int u = 0; u < U; ++u)
+      if (k0 + u * STEP < g.K) {
 #pragma unroll
-        for (int r = 0; r < WR; ++r) q[u][r] = ld_weights(row_of(r) + k);
+        for (int r = 0; r < WR; ++r) q[u][r] = ld_weights(row_of(r) + k0 + u * STEP);
       }
-    }
   };
-  const int first = warp * 256 + lane * 8;
-  // as in the kernels for few rows: W2 may be read before the wait, W13 only brought nearer
+  // as above: W2 may be read before the wait, W13 only brought nearer
   if constexpr (!DUAL_) {
     load(first);
   } else if ((lane & 7) == 0) {
 #pragma unroll
-    for (int r = 0; r < WR; ++r)
-      if (first < g.K) asm volatile("prefetch.global.L2 [%0];" ::"l"(row_of(r) + first));
+    for (int u = 0; u < U; ++u)
+      if (first + u * STEP < g.K) {
+#pragma unroll
+        for (int r = 0; r < WR; ++r) prefetch_l2(row_of(r) + first + u * STEP);
+      }
   }
   grid_dep_wait();
   grid_dep_trigger();
-  uint64_t acc[V] = {};
-  for (int k0 = first; k0 < g.K; k0 += U * DOT_WARPS * 256) {
+  float acc[WR] = {};
+  for (int k0 = first; k0 < g.K; k0 += U * STEP) {
     if (DUAL_ || k0 != first) load(k0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * DOT_WARPS * 256;
+      const int k = k0 + u * STEP;
       if (k < g.K) {
-        uint64_t x[TT][4];
+        const uint16_t* xp = reinterpret_cast<const uint16_t*>(g.x) + k;
+        float x[8], f[8];
+        unpack8<F16>(*reinterpret_cast<const uint4*>(xp), x);
+        if constexpr (!DUAL_) {  // h in two terms
+          unpack8<F16>(*reinterpret_cast<const uint4*>(xp + g.ldx), f);
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          const int64_t at = min(t, g.T - 1) * g.ldx + k;
-          if constexpr (DUAL_) {
-            unpack8<F16>(*reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(g.x) + at), x[t]);
-          } else {
-            const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(g.x) + at);
-            const float4 a = p[0], b = p[1];
-            x[t][0] = pair_of({a.x, a.y}), x[t][1] = pair_of({a.z, a.w});
-            x[t][2] = pair_of({b.x, b.y}), x[t][3] = pair_of({b.z, b.w});
-          }
+          for (int i = 0; i < 8; ++i) x[i] += f[i];
         }
 #pragma unroll
         for (int r = 0; r < WR; ++r) {
-          uint64_t f[4];
           unpack8<F16>(q[u][r], f);
 #pragma unroll
-          for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t * WR + r] = fma2(f[i], x[t][i], acc[t * WR + r]);
+          for (int i = 0; i < 8; ++i) acc[r] += f[i] * x[i];
         }
       }
     }
   }
-  float sums[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) sums[v] = of_pair(acc[v]).x + of_pair(acc[v]).y;
-  const float s = warp_sums<V>(sums);
-  if (lane % (32 / V) == 0) red[warp][lane / (32 / V)] = s;
+  const float s = warp_sums<WR>(acc);
+  if (lane % (32 / WR) == 0) red[warp][lane / (32 / WR)] = s;
   __syncthreads();
-  const int t = threadIdx.x / R, r = threadIdx.x % R, col = n0 + r;
-  if (t >= g.T) return;
-  auto total = [&](int v) {
-    float f = 0.f;
+  const int r = threadIdx.x;
+  if (r >= ROW_COLS) return;
+  float a = 0.f, u = 0.f;
 #pragma unroll
-    for (int i = 0; i < DOT_WARPS; ++i) f += red[i][v];
-    return f;
-  };
-  uint16_t* out = reinterpret_cast<uint16_t*>(g.out) + (int64_t)t * g.n + col;
-  float a = total(t * WR + r);
-  if constexpr (DUAL_) {
-    const float u = total(t * WR + R + r);
-    float d;
-    with_act(g.act, [&](auto A) { act_grad<A.value>(a, a, d); });
-    if (g.gu) {
-      g.gu[at_gu(t, col, g.n, 0)] = u * d;
-      g.gu[at_gu(t, col, g.n, 1)] = a;
-    }
-    g.h32[(int64_t)t * g.n + col] = a * u;
-    out[0] = (uint16_t)pack2<F16>(a * u, 0.f);
-  } else {
-    if (g.residual)
-      a += unpack2<F16>(reinterpret_cast<const uint16_t*>(g.residual)[t * g.ldr + col]).x;
-    out[0] = (uint16_t)pack2<F16>(a, 0.f);
+  for (int i = 0; i < ROW_WARPS; ++i) {
+    a += red[i][r];
+    if (DUAL_) u += red[i][WR - ROW_COLS + r];
   }
+  finish<DUAL_, F16>(g, 0, n0 + r, a, u);
 }
 
-template <int TT, bool F16>
-static int fwd_dot(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, cudaStream_t st) {
-  DotArgs g;
+template <bool F16>
+AFB_DEV void mma_rows(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (F16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    mma_bf16(c, a0, a1, a2, a3, b0, b1);
+}
+
+constexpr int TOK_WARPS = 16;
+
+// NG: groups of 8 rows (one past the last is computed as the last and left out)
+template <bool DUAL_, int NG, bool F16>
+__global__ void __launch_bounds__(32 * TOK_WARPS) ffn_tokens_kernel(TokenArgs g) {
+  // terms of the rows' values, blocks of 64 elements at a time, columns of the result
+  constexpr int TERMS = DUAL_ ? 1 : 2, U = DUAL_ ? 2 : 4, STEP = TOK_WARPS * 64, COLS = DUAL_ ? 8 : 16;
+  __shared__ float red[TOK_WARPS][8 * NG][16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, gc = (lane & 3) * 8, first = warp * 64;
+  const int n0 = blockIdx.x * COLS;
+  const uint16_t* wp[2];  // rows gr and gr + 8 of the MMA
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    wp[i] = reinterpret_cast<const uint16_t*>(g.w) +
+            (int64_t)(DUAL_ ? i * g.n + n0 + gr : min(n0 + i * 8 + gr, g.n - 1)) * g.K;
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 q[U][2][2];
+  auto load = [&](int kb) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int k = kb + u * STEP + j * 32 + gc;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q[u][i][j] = k < g.K ? ld_weights(wp[i] + k) : zero;
+      }
+  };
+  if constexpr (!DUAL_) {
+    load(first);
+  } else if (gc == 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (first + u * STEP < g.K) prefetch_l2(wp[0] + first + u * STEP), prefetch_l2(wp[1] + first + u * STEP);
+  }
+  grid_dep_wait();
+  grid_dep_trigger();
+  float acc[NG][4] = {};
+  const uint16_t* xp[NG];
+#pragma unroll
+  for (int i = 0; i < NG; ++i) xp[i] = reinterpret_cast<const uint16_t*>(g.x) + min(i * 8 + gr, g.T - 1) * g.ldx;
+  for (int kb = first; kb < g.K; kb += U * STEP) {
+    if (DUAL_ || kb != first) load(kb);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (kb + u * STEP < g.K) {
+        uint4 x[2][NG][TERMS];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int k = kb + u * STEP + j * 32 + gc;
+#pragma unroll
+          for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t)
+              x[j][i][t] = k < g.K ? *reinterpret_cast<const uint4*>(xp[i] + t * g.T * g.ldx + k) : zero;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int t = 0; t < TERMS; ++t) {
+              const uint4 &a = q[u][0][j], &b = q[u][1][j], &v = x[j][i][t];
+              mma_rows<F16>(acc[i], a.x, b.x, a.y, b.y, v.x, v.y);
+              mma_rows<F16>(acc[i], a.z, b.z, a.w, b.w, v.z, v.w);
+            }
+      }
+  }
+  // of the MMA's result a lane holds weight rows gr and gr + 8 of rows 2 (lane % 4) and the next
+#pragma unroll
+  for (int i = 0; i < NG; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[warp][i * 8 + (lane & 3) * 2 + (e & 1)][gr + (e >> 1) * 8] = acc[i][e];
+  __syncthreads();
+  const int t = threadIdx.x / COLS, r = threadIdx.x % COLS;
+  static_assert(8 * NG * COLS <= 32 * TOK_WARPS, "a thread has one element at most");
+  if (t >= g.T || n0 + r >= g.n) return;
+  float a = 0.f, u = 0.f;
+#pragma unroll
+  for (int i = 0; i < TOK_WARPS; ++i) {
+    a += red[i][t][r];
+    if (DUAL_) u += red[i][t][r + 8];
+  }
+  finish<DUAL_, F16>(g, t, n0 + r, a, u);
+}
+
+template <bool F16>
+static int fwd_tokens(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y,
+                      cudaStream_t st) {
+  auto run = [&](auto* row, auto* one, auto* two, int cols, const TokenArgs& g) {
+    if (s.T == 1) return launch_pdl(row, dim3(g.n / ROW_COLS), dim3(32 * ROW_WARPS), 0, st, g);
+    return launch_pdl(s.T <= 8 ? one : two, dim3((g.n + cols - 1) / cols), dim3(32 * TOK_WARPS), 0, st, g);
+  };
+  TokenArgs g;
   g.T = (int)s.T, g.n = s.F, g.K = s.H, g.act = s.act, g.w = w13.p, g.x = x.p, g.ldx = x.ld, g.out = h, g.gu = gu;
-  g.h32 = reinterpret_cast<float*>(reinterpret_cast<uint16_t*>(h) + s.T * s.F);
-  const int rc = launch_pdl(ffn_dot_kernel<true, TT, F16>, dim3(s.F / DOT_COLS), dim3(32 * DOT_WARPS), 0, st, g);
+  const int rc = run(ffn_row_kernel<true, F16>, ffn_tokens_kernel<true, 1, F16>, ffn_tokens_kernel<true, 2, F16>, 8, g);
   if (rc) return rc;
-  const float* h32 = g.h32;
-  g = DotArgs();
-  g.T = (int)s.T, g.n = s.N, g.K = s.F, g.w = w2.p, g.x = h32, g.ldx = s.F, g.out = y, g.residual = residual.p;
+  g = TokenArgs();
+  g.T = (int)s.T, g.n = s.N, g.K = s.F, g.w = w2.p, g.x = h, g.ldx = s.F, g.out = y, g.residual = residual.p;
   g.ldr = residual.ld;
-  return launch_pdl(ffn_dot_kernel<false, TT, F16>, dim3(s.N / DOT_COLS), dim3(32 * DOT_WARPS), 0, st, g);
+  return run(ffn_row_kernel<false, F16>, ffn_tokens_kernel<false, 1, F16>, ffn_tokens_kernel<false, 2, F16>, 16, g);
 }
 
 static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {
@@ -1120,10 +1221,7 @@ static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {
 template <bool F16>
 static int fwd(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, float* scratch,
                int num_sms, uint32_t* status, cudaStream_t st) {
-  if (dots(s)) {
-    auto f = s.T == 1 ? fwd_dot<1, F16> : s.T == 2 ? fwd_dot<2, F16> : fwd_dot<4, F16>;
-    return f(s, x, w13, w2, residual, h, gu, y, st);
-  }
+  if (tokens(s)) return fwd_tokens<F16>(s, x, w13, w2, residual, h, gu, y, st);
   if (s.T <= FEW) {
     auto f = s.T <= 16 ? fwd_few<16, F16> : s.T <= 32 ? fwd_few<32, F16> : s.T <= 64 ? fwd_few<64, F16> : fwd_few<128, F16>;
     return f(s, x, w13, w2, residual, h, gu, y, status, st);
@@ -1224,7 +1322,7 @@ static bool valid(const FfnShape& s) {
 size_t ffn_fwd_scratch(const FfnShape& s, int num_sms) {
   return s.T <= ffn::FEW ? 0 : ffn::product_scratch(s.T, s.N, s.F, num_sms);
 }
-int64_t ffn_h_rows(const FfnShape& s) { return ffn::dots(s) ? 3 * s.T : s.T <= ffn::FEW ? 2 * s.T : s.T; }
+int64_t ffn_h_rows(const FfnShape& s) { return s.T <= ffn::FEW ? 2 * s.T : s.T; }
 size_t ffn_bwd_scratch(const FfnShape& s, int num_sms) {
   return std::max({ffn::product_scratch(s.N, s.F, s.T, num_sms), ffn::product_scratch(s.T, s.H, 2 * s.F, num_sms),
                    ffn::product_scratch(2 * s.F, s.H, s.T, num_sms)});

@@ -18,8 +18,7 @@ struct FfnShape {
 // fp32 elements of scratch the calls below need (one buffer per call in flight)
 size_t ffn_fwd_scratch(const FfnShape& s, int num_sms);
 size_t ffn_bwd_scratch(const FfnShape& s, int num_sms);
-int64_t ffn_h_rows(const FfnShape& s);  // rows of the buffer for h: T, and T or 2T more where the forward
-                                         // pass keeps a second term or fp32 values
+int64_t ffn_h_rows(const FfnShape& s);  // rows of the buffer for h: T, or 2T where a second term is kept
 // h [ffn_h_rows, F], h itself in the first T rows; gu [T rounded up to 32, 2F] fp32 (u act'(g) and act(g) in the
 // kernels' own order, for the backward pass), 32-byte aligned, or null; y [T, N]
 int ffn_fwd(const FfnShape& s, const void* x, int64_t ldx, const void* w13, const void* w2, const void* residual,
