@@ -12,7 +12,7 @@
 // transposed in memory), and on the epilogue. Sums are fp32 in TMEM. h and [dg | du] are rounded once to the element
 // type because the tensor cores take them as operands; p and q are kept in fp32 for the backward pass, since a second
 // rounding there would show in dx and dW13. Split-K partial sums are fp32 and added in a fixed order: every result is
-// bitwise reproducible. Up to 128 rows the forward pass has kernels of its own (below), and others for one to sixteen.
+// bitwise reproducible. Few rows have forward kernels of their own (below).
 //
 // Measured (one B200, kernels alone, TFLOP/s of 1,646 measured for a library GEMM): 4,100 x 2,048 x 6,144 forward DUAL
 // 155 us (1,330) and y 77 (1,340), backward DACT 93 (1,110), dx 145 (1,420), the weight gradients 230 (1,350); a product
@@ -628,13 +628,26 @@ static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr res
 }
 
 // ------------------------------------------------------------------------------------------ few rows
-// Up to FEW rows the weights' bytes are the time. The weights take the M side of the MMA (128 weight rows a CTA, gate
+// With few rows the weights' bytes are the time. The weights take the M side of the MMA (128 weight rows a CTA, gate
 // and up tiles side by side in TMEM for DUAL) and the rows the N side, padded to NT; the C CTAs of a cluster take a
 // share of K each and add their partial sums through distributed shared memory, so no partial goes through HBM and
 // there is one launch a product. h is kept as two terms (value and rounding error, rows 0.. and T.. of a [2T, F]
 // buffer): the second MMA column block costs nothing here and leaves the result with its own rounding only.
-constexpr int FEW = 128;
 constexpr int64_t PREFETCH = 48 << 20;  // of the down projection's weights, into the 126 MB of L2
+
+static int64_t weight_bytes(const FfnShape& s) { return (2 * (int64_t)s.H + s.N) * s.F * 2; }
+// Up to 32 rows an SM holds two CTAs, with more one, and clusters of a power of two leave SMs without one where there are
+// many weight tiles: so the limits. Measured, us here and as large tiles: 2,048 x 6,144 (75 MB of weights) 33 rows 27.6
+// and 31, 128 rows 33.7 and 31.5; 2,560 x 10,240 (157 MB) 33 rows 48 and 53, 65 rows 66 and 53; 4,096 x 8,192 (201 MB) 64
+// rows 54 and 54; 5,120 x 17,408 (535 MB) 32 rows 97 and 109, 33 rows 135 and 109. (Two CTAs an SM up to 64 rows as well:
+// 100 us for the last, but 2,048 x 2,048 14.6 -> 16.8.) Of few weights, where large tiles would be few and deep, 129 rows
+// of 2,048 x 1,024 (13 MB) 16 and 23, 384 rows 22.9 and 23.4, 512 23.6 and 23.5; 256 rows of 2,048 x 2,048 (25 MB) 23.6 and
+// 26.0, 257 27.3 and 26.5; 256 rows of 1,152 x 4,304 (30 MB) 28 and 23.
+static bool few(const FfnShape& s) {
+  const int64_t b = weight_bytes(s);
+  return s.T <= 32 || (s.T <= 64 && b <= 200'000'000) || (s.T <= 128 && b <= 80'000'000) ||
+         (s.T <= 256 && b <= 26'000'000) || (s.T <= 384 && b <= 13'000'000);
+}
 
 template <bool DUAL_, int NT>
 struct Few {
@@ -888,6 +901,7 @@ static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, FewArgs g, i
   if (!rc) rc = make_tmap_2d(&tx, x.p, 2, g.K, x_rows, x.ld * 2, BK, NT, 1);
   if (rc) return 5000 + rc;
   g.chunk = (g.T + chunks - 1) / chunks;
+  if (g.chunk > NT) return 6;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(C, (g.n + 127) / 128, chunks);
   cfg.blockDim = dim3(192);
@@ -904,18 +918,19 @@ static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, FewArgs g, i
   return e == cudaSuccess ? (int)cudaGetLastError() : (int)e;
 }
 
-// The rows go as one chunk, or as two where that costs the clusters no CTA: the partial sums that a cluster exchanges
-// are halved (80 rows at 2,560 x 640: 16.5 us in one chunk, 15.1 in two)
+// The rows go as chunks of NT, or of NT / 2 where that costs the clusters no CTA: the partial sums that a cluster
+// exchanges are halved (80 rows at 2,560 x 640: 16.5 us in one chunk, 15.1 in two)
 template <bool DUAL_, int NT, bool F16>
 static int few_rows(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArgs& g, uint32_t* status, cudaStream_t st) {
-  const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK, C = few_cluster<DUAL_, NT, F16>(tiles, kb);
+  const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK, chunks = (g.T + NT - 1) / NT;
+  const int C = few_cluster<DUAL_, NT, F16>(chunks * tiles, kb);
   if (C < 0) return -C;
   if constexpr (NT > 32) {
-    const int C2 = few_cluster<DUAL_, NT / 2, F16>(2 * tiles, kb);
+    const int chunks2 = (g.T + NT / 2 - 1) / (NT / 2), C2 = few_cluster<DUAL_, NT / 2, F16>(chunks2 * tiles, kb);
     if (C2 < 0) return -C2;
-    if (C2 >= C) return launch_few<DUAL_, NT / 2, F16>(w, w_rows, x, x_rows, g, 2, C2, status, st);
+    if (C2 >= C) return launch_few<DUAL_, NT / 2, F16>(w, w_rows, x, x_rows, g, chunks2, C2, status, st);
   }
-  return launch_few<DUAL_, NT, F16>(w, w_rows, x, x_rows, g, 1, C, status, st);
+  return launch_few<DUAL_, NT, F16>(w, w_rows, x, x_rows, g, chunks, C, status, st);
 }
 
 template <int NT, bool F16>
@@ -953,8 +968,7 @@ static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void
 // Sixteen rows 2,048 x 512 5.2 and 9.3, 2,048 x 2,048 (25 MB) 10.6 and 12.6, 1,152 x 4,304 (30 MB) 16.2 and 14.7. 24 rows:
 // 2,048 x 512 7.8 and 9.9, 2,560 x 640 11.4 and 11.1.
 static bool tokens(const FfnShape& s) {
-  const int64_t bytes = (2 * (int64_t)s.H + s.N) * s.F * 2;
-  return s.T == 1 || (s.T <= 8 && bytes <= 96 << 20) || (s.T <= 16 && bytes <= 24 << 20);
+  return s.T == 1 || (s.T <= 8 && weight_bytes(s) <= 100'000'000) || (s.T <= 16 && weight_bytes(s) <= 26'000'000);
 }
 
 // not by way of L1, which another kernel on the SM may have filled before the weights were written
@@ -1222,7 +1236,7 @@ template <bool F16>
 static int fwd(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y, float* scratch,
                int num_sms, uint32_t* status, cudaStream_t st) {
   if (tokens(s)) return fwd_tokens<F16>(s, x, w13, w2, residual, h, gu, y, st);
-  if (s.T <= FEW) {
+  if (few(s)) {
     auto f = s.T <= 16 ? fwd_few<16, F16> : s.T <= 32 ? fwd_few<32, F16> : s.T <= 64 ? fwd_few<64, F16> : fwd_few<128, F16>;
     return f(s, x, w13, w2, residual, h, gu, y, status, st);
   }
@@ -1320,9 +1334,9 @@ static bool valid(const FfnShape& s) {
 }  // namespace ffn
 
 size_t ffn_fwd_scratch(const FfnShape& s, int num_sms) {
-  return s.T <= ffn::FEW ? 0 : ffn::product_scratch(s.T, s.N, s.F, num_sms);
+  return ffn::few(s) ? 0 : ffn::product_scratch(s.T, s.N, s.F, num_sms);
 }
-int64_t ffn_h_rows(const FfnShape& s) { return s.T <= ffn::FEW ? 2 * s.T : s.T; }
+int64_t ffn_h_rows(const FfnShape& s) { return ffn::few(s) ? 2 * s.T : s.T; }
 size_t ffn_bwd_scratch(const FfnShape& s, int num_sms) {
   return std::max({ffn::product_scratch(s.N, s.F, s.T, num_sms), ffn::product_scratch(s.T, s.H, 2 * s.F, num_sms),
                    ffn::product_scratch(2 * s.F, s.H, s.T, num_sms)});

@@ -8,7 +8,7 @@ lie (no transposed copies).
 
 Types: bf16 or fp16, weights in x's type. Sums are fp32; ``h`` and the gradients of the two pre-activations are
 rounded once to x's type (they are tensor-core operands); what the backward pass needs of the pre-activations is kept
-in fp32 (8 F bytes a row; nothing when neither x nor w13 asks for a gradient). Up to 128 rows the forward pass keeps h
+in fp32 (8 F bytes a row; nothing when neither x nor w13 asks for a gradient). With few rows the forward pass keeps h
 in two terms, so that only the result is rounded. Results do not depend on timing or on other work on the GPU: every
 sum has a fixed order.
 

@@ -142,6 +142,19 @@ def test_gated_ffn_single_tokens(size, T):
     check_status()
 
 
+@pytest.mark.parametrize("size", [(33, 4096, 4200), (64, 4096, 8200), (65, 4096, 4200), (128, 2048, 6512), (129, 1024, 1032),
+                                  (250, 1032, 4184), (256, 1024, 8464), (257, 1024, 1032), (384, 2056, 1048),
+                                  (385, 1024, 1032)])
+def test_gated_ffn_where_the_kernels_change(size):
+    """Both sides of where rows and bytes of weights choose another kernel."""
+    T, H, F = size
+    t = ffn_inputs(T, H, F, H, BF, seed=T)
+    got, ref = run_ffn(*t, "silu"), ffn_oracle(*t, "silu")
+    for k in got:
+        check(got[k], *ref[k], k)
+    check_status()
+
+
 def test_gated_ffn_gradient_against_differences():
     """<gradient, direction> of the kernels against the central difference of the fp64 block along the direction."""
     x, w13, w2, res, dy = ffn_inputs(96, 128, 200, 64, BF, seed=3)
