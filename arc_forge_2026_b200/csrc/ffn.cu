@@ -946,7 +946,7 @@ static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void
   return few_rows<false, NT, F16>(w2, s.N, {h, s.F}, 2 * s.T, g, status, st);
 }
 
-// ------------------------------------------------------------------------------------------ one to sixteen rows
+// ------------------------------------------------------------------------------------------ one to 32 rows
 // Here a launch's latency counts beside the weights' bytes, and the kernels above have a ring to fill, TMEM to allocate
 // and read and two cluster barriers. These read the weights straight into registers and add a CTA's partial sums, one
 // share of K a warp, through shared memory. h goes from the first to the second in two terms, as above.
@@ -965,10 +965,11 @@ static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void
 // Measured, us here and in the kernels above: one row 2,048 x 6,144 15 and 20.6, 5,120 x 17,408 86 and 93 (6.2 TB/s and
 // 5.7), 2,048 x 512 4.7 and 8.7. Eight rows 2,048 x 512 5.5 and 9.0, 2,048 x 2,048 7.4 and 12.3, 2,048 x 6,144 (75 MB of
 // weights) 19.5 and 20.9, 5,120 x 17,408 (535 MB) 120 and 89, for a row's 64 bytes at a time are less than HBM wants.
-// Sixteen rows 2,048 x 512 5.2 and 9.3, 2,048 x 2,048 (25 MB) 10.6 and 12.6, 1,152 x 4,304 (30 MB) 16.2 and 14.7. 24 rows:
-// 2,048 x 512 7.8 and 9.9, 2,560 x 640 11.4 and 11.1.
+// Sixteen rows 2,048 x 512 5.2 and 9.3, 2,048 x 2,048 (25 MB) 10.6 and 12.6, 1,152 x 4,304 (30 MB) 16.2 and 14.7. 32
+// rows 2,048 x 512 (6 MB) 9.2 and 10.2, 256 x 136 6.6 and 10, 2,560 x 640 (10 MB) 13.9 and 11.5.
 static bool tokens(const FfnShape& s) {
-  return s.T == 1 || (s.T <= 8 && weight_bytes(s) <= 100'000'000) || (s.T <= 16 && weight_bytes(s) <= 26'000'000);
+  return s.T == 1 || (s.T <= 8 && weight_bytes(s) <= 100'000'000) || (s.T <= 16 && weight_bytes(s) <= 26'000'000) ||
+         (s.T <= 32 && weight_bytes(s) <= 7'000'000);
 }
 
 // not by way of L1, which another kernel on the SM may have filled before the weights were written
@@ -1213,18 +1214,20 @@ __global__ void __launch_bounds__(32 * TOK_WARPS) ffn_tokens_kernel(TokenArgs g)
 template <bool F16>
 static int fwd_tokens(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void* h, float* gu, void* y,
                       cudaStream_t st) {
-  auto run = [&](auto* row, auto* one, auto* two, int cols, const TokenArgs& g) {
-    if (s.T == 1) return launch_pdl(row, dim3(g.n / ROW_COLS), dim3(32 * ROW_WARPS), 0, st, g);
-    return launch_pdl(s.T <= 8 ? one : two, dim3((g.n + cols - 1) / cols), dim3(32 * TOK_WARPS), 0, st, g);
+  auto run = [&](auto dual, const TokenArgs& g) {
+    constexpr bool D = decltype(dual)::value;
+    if (s.T == 1) return launch_pdl(ffn_row_kernel<D, F16>, dim3(g.n / ROW_COLS), dim3(32 * ROW_WARPS), 0, st, g);
+    auto kern = s.T <= 8 ? ffn_tokens_kernel<D, 1, F16> : s.T <= 16 ? ffn_tokens_kernel<D, 2, F16> : ffn_tokens_kernel<D, 4, F16>;
+    return launch_pdl(kern, dim3(D ? g.n / 8 : (g.n + 15) / 16), dim3(32 * TOK_WARPS), 0, st, g);
   };
   TokenArgs g;
   g.T = (int)s.T, g.n = s.F, g.K = s.H, g.act = s.act, g.w = w13.p, g.x = x.p, g.ldx = x.ld, g.out = h, g.gu = gu;
-  const int rc = run(ffn_row_kernel<true, F16>, ffn_tokens_kernel<true, 1, F16>, ffn_tokens_kernel<true, 2, F16>, 8, g);
+  const int rc = run(std::true_type(), g);
   if (rc) return rc;
   g = TokenArgs();
   g.T = (int)s.T, g.n = s.N, g.K = s.F, g.w = w2.p, g.x = h, g.ldx = s.F, g.out = y, g.residual = residual.p;
   g.ldr = residual.ld;
-  return run(ffn_row_kernel<false, F16>, ffn_tokens_kernel<false, 1, F16>, ffn_tokens_kernel<false, 2, F16>, 16, g);
+  return run(std::false_type(), g);
 }
 
 static size_t product_scratch(int64_t M, int N, int64_t K, int num_sms) {

@@ -125,7 +125,7 @@ def test_gated_ffn_row_counts_of_serving(T):
     check(y, *ref["y"], T)
 
 
-@pytest.mark.parametrize("T", [1, 2, 3, 7, 8, 9, 13, 16, 17])
+@pytest.mark.parametrize("T", [1, 2, 3, 7, 8, 9, 13, 16, 17, 25, 32])
 @pytest.mark.parametrize("size", [(8, 8, 8), (264, 1032, 520), (1024, 2056, 1032), (2048, 2056, 2048), (4104, 4200, 4104)])
 def test_gated_ffn_single_tokens(size, T):
     """Few rows, on both sides of where the kernels change (rows and bytes of weights); fp16 and bf16, rows of
