@@ -919,17 +919,21 @@ static int launch_few(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, FewArgs g, i
 }
 
 // The rows go as chunks of NT, or of half of that (and half again, to 32) where that costs the clusters no CTA: the partial
-// sums that a cluster exchanges are halved (80 rows at 2,560 x 640: 16.5 us in one chunk, 14.7 in three; 128 rows at
-// 256 x 136: 13.6 in two chunks, 10.1 in four. Chunks of 16: 64 rows at 2,048 x 512 11.6, of 32 10.9)
+// sums that a cluster exchanges are halved (80 rows at 2,560 x 640: 16.5 us in one chunk, 14.5 in two; 128 rows at
+// 256 x 136: 13.6 in two chunks, 10.1 in four). Chunks of 32 only if there are twice as many (80 rows at 2,560 x 640 in
+// three: 14.7; chunks of 16: 64 rows at 2,048 x 512 11.6, of 32 10.9).
 template <bool DUAL_, int NT, bool F16>
 static int few_rows(Ptr w, int64_t w_rows, Ptr x, int64_t x_rows, const FewArgs& g, uint32_t* status, cudaStream_t st) {
   const int tiles = (g.n + 127) / 128, kb = (g.K + BK - 1) / BK, chunks = (g.T + NT - 1) / NT;
   const int C = few_cluster<DUAL_, NT, F16>(chunks * tiles, kb);
   if (C < 0) return -C;
   if constexpr (NT > 32) {
-    const int C2 = few_cluster<DUAL_, NT / 2, F16>((g.T + NT / 2 - 1) / (NT / 2) * tiles, kb);
-    if (C2 < 0) return -C2;
-    if (C2 >= C) return few_rows<DUAL_, NT / 2, F16>(w, w_rows, x, x_rows, g, status, st);
+    const int chunks2 = (g.T + NT / 2 - 1) / (NT / 2);
+    if (NT > 64 || chunks2 == 2 * chunks) {
+      const int C2 = few_cluster<DUAL_, NT / 2, F16>(chunks2 * tiles, kb);
+      if (C2 < 0) return -C2;
+      if (C2 >= C) return few_rows<DUAL_, NT / 2, F16>(w, w_rows, x, x_rows, g, status, st);
+    }
   }
   return launch_few<DUAL_, NT, F16>(w, w_rows, x, x_rows, g, chunks, C, status, st);
 }
