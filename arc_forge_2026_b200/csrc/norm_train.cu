@@ -12,7 +12,7 @@
 // partial sums of dw and db and a second kernel adds those in a fixed order (no atomics: results are bitwise
 // reproducible).
 //
-// Measured (one B200, cold L2): 16,383 x 2,048 fp32 forward 49 us (5.4 TB/s), backward 73 (5.5) + 4 for the sums;
+// Measured (one B200): 16,383 x 2,048 fp32 forward 43 us (6.3 TB/s), backward 72 (5.6) + 4 for the sums;
 // 5,633 x 4,608 bf16 29 (3.6), 36 (4.3) + 4: 16-bit rows are bound by the instructions of their elements, some 11
 // forward and 17 backward, before memory. Rows of more than 8,192 columns leave an SM one CTA: 4,096 x 16,384 bf16 77 and
 // 265 us.
@@ -513,6 +513,7 @@ static Kernel kernel_of(int nv, int v, int wpr) {
 }
 
 constexpr int RING_SMEM = 160 * 1024;  // of an SM; four CTAs' static shared memory (13 KB each) fits beside it
+constexpr int RING_AHEAD = 96 * 1024;  // of that, what the CTAs of an SM keep on the way
 
 // Chunks a lane, warps a row, rows a CTA, CTAs, ring. Forward, the instructions a row takes decide the first two: some 8
 // an element and 75 a warp for its sums, so few warps with much each, as far as the lanes' last chunks are not left
@@ -520,8 +521,11 @@ constexpr int RING_SMEM = 160 * 1024;  // of an SM; four CTAs' static shared mem
 // rows of 2,048 in bf16: 46 us; one chunk 61, for the sums of twice the warps; three 70 and four 65, for want of
 // registers), one where a row is 512 columns or less, four where it passes 8,192, and three from 4,097 to 4,608, where
 // two would leave an SM one CTA.
-// CTAs: as many as are resident (a second wave would wait for the first). The ring takes what shared memory the SM's
-// CTAs leave each other, up to 8 rows.
+// CTAs: as many as are resident (a second wave would wait for the first). The rings of an SM's CTAs keep 96 KB on
+// the way: more makes the memory slower, not faster (96 and 160 KB: 16,383 rows of 2,048 in fp32 42.6 and 47.8 us forward,
+// 71.5 and 74.5 backward, 16,384 of 2,048 in bf16 24.8 and 26.4, 44.5 and 46.1; 64 KB: 24.7 and 44.0, but 5,633 of 4,608
+// backward 39.0 where this takes 35.7). A CTA alone on its SM has two slots at least (4,096 rows of 8,192 in fp32, backward:
+// 78 us with one, 70 with two).
 template <typename T, bool BWD>
 static int plan(const NormArgs& a, int num_sms, Shape& s, Kernel& kern) {
   const int chunks = (a.width + 7) / 8;
@@ -556,8 +560,12 @@ static int plan(const NormArgs& a, int num_sms, Shape& s, Kernel& kern) {
   const int slot = s.ring.part * (BWD ? 2 : 1) * s.groups;
   per_sm = std::max(1, std::min(per_sm, RING_SMEM / slot));
   s.grid = (int)std::max<int64_t>(1, std::min(blocks, (int64_t)num_sms * per_sm));
-  s.ring.depth = std::max(1, std::min(MAX_DEPTH, RING_SMEM / per_sm / slot));
-  s.smem = s.ring.depth * slot;
+  const int least = per_sm == 1 ? std::min(2, RING_SMEM / slot) : 1;
+  s.ring.depth = std::max(least, std::min(MAX_DEPTH, RING_AHEAD / per_sm / slot));
+  // all of a CTA's share is asked for: CTAs that start while the kernel before still holds SMs spread evenly only if an SM
+  // cannot take more of them than planned (16,383 rows of 2,048 in fp32, both ways in a stream: 159 us without this, 120
+  // with it)
+  s.smem = std::max(s.ring.depth * slot, RING_SMEM / per_sm / 128 * 128);
   return 0;
 }
 
