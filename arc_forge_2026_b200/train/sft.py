@@ -18,8 +18,9 @@ parallel run takes bins r, r + world, ... Each optimizer step runs ``--bins-per-
 token mean of -log p(label) over the step's trained tokens on all ranks; adapter gradients are averaged over ranks
 (replicated LoRA, one fp32 all-reduce), clipped by global norm, AdamW with bf16 moments. ``--offload-checkpoints``
 keeps the layer checkpoints in pinned host memory (``train/offload.py``). ``--lora-dropout`` drops elements of the
-adapters' inputs; the masks are a function of (seed, adapter, step, rank, bin), so a resumed run draws the same ones. At the end (and with ``--save-every``)
-the adapters and optimizer state are saved, and ``--export`` writes the merged model (``fn-lora-merged-v2``).
+adapters' inputs; the masks are a function of (seed, adapter, step, rank, bin), so a resumed run draws the same ones.
+At the end (and with ``--save-every``) the adapters and optimizer state are saved, and ``--export`` writes the merged
+model (``fn-lora-merged-v2``).
 """
 from __future__ import annotations
 
