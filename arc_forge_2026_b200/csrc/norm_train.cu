@@ -469,12 +469,13 @@ __global__ void __launch_bounds__(1024) norm_reduce_kernel(const float* __restri
 }
 
 static bool aligned(const void* p, int to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
-// elements accessed at a time (col_of)
+// elements accessed at a time (col_of): of the rows and of the weights, which are read the same way (fp32 weights by
+// pairs one by one) and may start at any element of a flat buffer
 static int access_of(const NormArgs& a) {
   auto rows = [&](int to) { return aligned(a.x, to) && aligned(a.y, to) && aligned(a.dy, to) && aligned(a.dx, to); };
-  if (a.width % 8 == 0 && a.ldx % 8 == 0 && rows(16) && aligned(a.w, 16) && aligned(a.b, 16) && aligned(a.partial, 16))
-    return 8;
-  return a.dtype != ELEM_FP32 && a.width % 2 == 0 && a.ldx % 2 == 0 && rows(4) ? 2 : 1;
+  auto weights = [&](int to) { return aligned(a.w, to) && aligned(a.b, to); };
+  if (a.width % 8 == 0 && a.ldx % 8 == 0 && rows(16) && weights(16) && aligned(a.partial, 16)) return 8;
+  return a.dtype != ELEM_FP32 && a.width % 2 == 0 && a.ldx % 2 == 0 && rows(4) && weights(4) ? 2 : 1;
 }
 
 struct Shape {

@@ -378,6 +378,25 @@ def test_norm_strides_empty_frozen_and_constant_rows():
     assert torch.equal(y, fused.rms_norm(xs, ws, 1e-6))
 
 
+@pytest.mark.parametrize("W", [2, 264, 1002, 1152, 4608, 8200])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_norm_weights_at_any_element_of_a_flat_buffer(W, dt):
+    """16-bit w and b as views that start 2, 4, 6 or 16 bytes into a buffer, w and b each for itself."""
+    x, w, b, dy = norm_inputs(40, W, dt, dt, seed=15)
+
+    def at(t, off):
+        buf = torch.zeros(W + 16, dtype=dt, device=dev)
+        buf[off:off + W] = t
+        return buf[off:off + W]
+    for rms in (False, True):
+        ref = norm_oracle(x, w, None if rms else b, dy, 1e-6, rms)
+        for ow, ob in ((1, 0), (0, 1), (2, 0), (0, 2), (3, 5), (8, 2), (8, 8)):
+            got = run_norm(x, at(w, ow), at(b, ob), dy, 1e-6, rms)
+            for k in got:
+                check(got[k], *ref[k], (k, rms, ow, ob))
+    check_status()
+
+
 def test_norm_repeats_bitwise():
     x, w, b, dy = norm_inputs(3001, 1152, BF, FP, seed=13)
     a, c = run_norm(x, w, b, dy, 1e-6, False), run_norm(x, w, b, dy, 1e-6, False)
