@@ -1,8 +1,11 @@
 // Bindings of the gated feed-forward block, the norms with trainable weights and dropout: argument checks,
 // allocation of results and scratch on the tensors' own device, launch on that device's current stream, and their
 // autograd nodes (in C++: a small call's time is the host's, and a Python node costs several times the kernels).
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "binding_utils.h"
 #include "ffn.h"
@@ -19,6 +22,33 @@ bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad(); 
 bool wants_grad(const OptT& t) { return t.has_value() && wants_grad(*t); }
 at::Tensor val(const OptT& t) { return t.has_value() ? *t : at::Tensor(); }
 OptT opt(const at::Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
+// Whether a tensor's memory holds its value. It does not where the tensor is a function transform's wrapper, dispatches
+// to Python (a fake tensor has no memory at all), or is negated, conjugated or zeroed only when it is read.
+bool in_memory(const at::Tensor& t) {
+  using K = c10::DispatchKey;
+  static const c10::DispatchKeySet lazy({K::Python, K::Negative, K::Conjugate, K::ZeroTensor, K::Functionalize,
+                                         K::FuncTorchBatched, K::FuncTorchGradWrapper, K::Batched});
+  return !t.key_set().has_any(lazy);
+}
+bool in_memory(const OptT& t) { return !t.has_value() || in_memory(*t); }
+// Whether operations have to go through the dispatcher: inside a function transform, under a dispatch mode or while a
+// trace is recorded, where a kernel launch would pass unseen. The callers then take their plain forms.
+bool dispatched() {
+  return c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing() ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+}
+template <class... Ts>
+bool launchable(const Ts&... ts) {
+  return (in_memory(ts) && ...) && !dispatched();
+}
+// an incoming gradient for a kernel
+at::Tensor gradient(const at::Tensor& t, const char* what) {
+  if (in_memory(t)) return t;
+  const at::Tensor r = t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg();
+  TORCH_CHECK_NOT_IMPLEMENTED(in_memory(r), what, ": its backward pass takes plain tensors only, not those of a function ",
+                              "transform (is_grads_batched and the like)");
+  return r;
+}
 // x with its leading dimensions as one
 at::Tensor rows2d(const at::Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
 void differentiable_once(const char* what) {
@@ -283,7 +313,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
     differentiable_once("gated_ffn");
     capturable_backward("gated_ffn");
     const variable_list v = ctx->get_saved_variables();
-    const at::Tensor& dy = grads[0];
+    const at::Tensor dy = gradient(grads[0], "gated_ffn");
     const bool need_x = ctx->needs_input_grad(0), need_w13 = ctx->needs_input_grad(1),
                need_w2 = ctx->needs_input_grad(2);
     variable_list out(5);
@@ -299,7 +329,7 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
   }
 };
 
-// The block, or None where the kernels do not cover the type or the sizes (the caller's plain form does)
+// The block, or None where the kernels do not cover the type, the sizes or the kind of tensor (the caller's plain form does)
 OptT gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2, const OptT& residual, int64_t act) {
   TORCH_CHECK_VALUE(x.dim() >= 1 && w13.dim() == 2 && w2.dim() == 2 && w13.size(1) == x.size(-1) &&
                         w13.size(0) == 2 * w2.size(1),
@@ -316,6 +346,7 @@ OptT gated_ffn(const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w2,
   }
   const bool half = x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf;
   if (!x.is_cuda() || !half || x.size(-1) % 8 || w2.size(0) % 8 || w2.size(1) % 8) return OptT();
+  if (!launchable(x, w13, w2, residual)) return OptT();
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w13) || wants_grad(w2) || wants_grad(residual)))
     return GatedFfn::apply(x, w13, w2, residual, act);
   return std::get<0>(gated_ffn_fwd(x, w13, w2, residual, act, false));
@@ -339,7 +370,8 @@ struct TrainNorm : torch::autograd::Function<TrainNorm> {
     capturable_backward(rms ? "rms_norm" : "layer_norm");
     const variable_list v = ctx->get_saved_variables();
     variable_list out(5);
-    if (at::GradMode::is_enabled()) {  // create_graph: the formulas in operations that can be differentiated again
+    // create_graph, or a function transform's gradients: the formulas in operations that can be differentiated again
+    if (at::GradMode::is_enabled() || !in_memory(grads[0])) {
       const at::Tensor x = v[0].to(at::kFloat), w = v[1].to(at::kFloat), dy = grads[0].to(at::kFloat);
       const at::Tensor c = rms ? x : x - x.mean({-1}, true);
       const at::Tensor rstd = at::rsqrt(c.square().mean({-1}, true) + ctx->saved_data["eps"].toDouble());
@@ -360,7 +392,9 @@ struct TrainNorm : torch::autograd::Function<TrainNorm> {
   }
 };
 
-at::Tensor train_norm(const at::Tensor& x, const at::Tensor& w, const OptT& b, double eps, bool rms) {
+// The norm, or None for tensors that the kernels cannot read (the caller's plain form does)
+OptT train_norm(const at::Tensor& x, const at::Tensor& w, const OptT& b, double eps, bool rms) {
+  if (!launchable(x, w, b)) return OptT();
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "norm: x [..., width]");
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return TrainNorm::apply(x, w, b, eps, rms);
@@ -382,15 +416,17 @@ struct Dropout : torch::autograd::Function<Dropout> {
     capturable_backward("dropout");
     variable_list out(6);
     if (ctx->needs_input_grad(0))
-      out[0] = dropout_op(grads[0], OptT(), ctx->saved_data["threshold"].toInt(), ctx->saved_data["seed"].toInt(),
+      out[0] = dropout_op(gradient(grads[0], "dropout"), OptT(), ctx->saved_data["threshold"].toInt(), ctx->saved_data["seed"].toInt(),
                           ctx->saved_data["offset"].toInt(), opt(ctx->get_saved_variables()[0]));
     if (ctx->saved_data["residual"].toBool()) out[1] = grads[0];
     return out;
   }
 };
 
-at::Tensor dropout(const at::Tensor& x, const OptT& residual, int64_t threshold, int64_t seed, int64_t offset,
-                   const OptT& rng) {
+// y, or None for tensors that the kernel cannot read
+OptT dropout(const at::Tensor& x, const OptT& residual, int64_t threshold, int64_t seed, int64_t offset,
+             const OptT& rng) {
+  if (!launchable(x, residual, rng)) return OptT();
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(residual)))
     return Dropout::apply(x, residual, rng, threshold, seed, offset);
   return dropout_op(x, residual, threshold, seed, offset, rng);

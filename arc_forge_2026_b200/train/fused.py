@@ -9,6 +9,8 @@ SwiGLU and token aggregation, ``fp8_moe.py`` _swiglu_backward / _routing_backwar
 
 Beside them, with trainable weights: :func:`layer_norm` and :func:`rms_norm` (``csrc/norm_train.cu``) and
 :func:`dropout` from a counter-based generator (``csrc/dropout.cu``); the gated feed-forward block is ``train/ffn.py``.
+These four take their plain forms inside function transforms (``torch.func``), under dispatch modes, while a trace is
+recorded, and for tensors whose memory is not their value (fake tensors, other subclasses, lazily negated views).
 """
 from __future__ import annotations
 
@@ -123,8 +125,10 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
         kernels.hit("rms_norm", True)
         return _RMSNorm.apply(x, w.float().contiguous(), eps, None)
     if kernels.use("rms_norm") and w.shape == x.shape[-1:] and _train_norm_ok(x, w):
-        kernels.hit("rms_norm", True)
-        return _ext().train_norm(x, w, None, eps, True)
+        y = _ext().train_norm(x, w, None, eps, True)
+        if y is not None:
+            kernels.hit("rms_norm", True)
+            return y
     if x.is_cuda:
         kernels.hit("rms_norm", False)
     return R.rms_norm(x, w, eps)
@@ -149,8 +153,10 @@ def layer_norm(x: torch.Tensor, w: torch.Tensor, b: torch.Tensor | None = None, 
     if w.device != x.device or (b is not None and (b.device != w.device or b.dtype != w.dtype)):
         raise ValueError("layer_norm: w and b on x's device, b in w's type")
     if kernels.use("layer_norm") and _train_norm_ok(x, w):
-        kernels.hit("layer_norm", True)
-        return _ext().train_norm(x, w, b, eps, False)
+        y = _ext().train_norm(x, w, b, eps, False)
+        if y is not None:
+            kernels.hit("layer_norm", True)
+            return y
     if x.is_cuda:
         kernels.hit("layer_norm", False)
     return layer_norm_reference(x, w, b, eps)
@@ -234,11 +240,13 @@ def dropout(x: torch.Tensor, p: float, seed, offset: int = 0, residual: torch.Te
         raise ValueError("dropout: residual has x's shape, type and device")
     if not x.is_floating_point():
         raise ValueError(f"dropout: x is {x.dtype}")
-    native = x.is_cuda and x.dtype in _FLOATS and kernels.use("dropout")
+    if x.is_cuda and x.dtype in _FLOATS and kernels.use("dropout"):
+        y = _ext().dropout(x, residual, dropout_threshold(p), _i64(int(seed)), _i64(int(offset)), rng)
+        kernels.hit("dropout", y is not None)
+        # what the kernel cannot read goes through operations that can be transformed and traced
+        return _dropout_plain(x, residual, float(p), int(seed), int(offset), rng) if y is None else y
     if x.is_cuda:
-        kernels.hit("dropout", native)
-    if native:
-        return _ext().dropout(x, residual, dropout_threshold(p), _i64(int(seed)), _i64(int(offset)), rng)
+        kernels.hit("dropout", False)
     return _DropoutPlain.apply(x, residual, float(p), int(seed), int(offset), rng)
 
 

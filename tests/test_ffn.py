@@ -160,3 +160,43 @@ def test_opt_in_feed_forward_leaves_cpu_runs_alone():
         assert torch.equal(st.hidden(ids), y)
     finally:
         kernels.enable(sorted(old))
+
+
+def test_tensors_without_memory_never_reach_the_kernels():
+    """A fake tensor says that it is on the GPU and has no memory; function-transform wrappers and lazily negated views
+    have memory that is not their value. The bindings leave them to the plain forms before they look at any pointer, and
+    so they do inside transforms, dispatch modes and traces."""
+    pytest.importorskip("arc_forge_2026_b200._C")
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from arc_forge_2026_b200.ops import C
+    ext = C()
+    for dt in (torch.float32, BF):
+        with FakeTensorMode():
+            x, w = torch.empty(6, 40, dtype=dt, device="cuda"), torch.empty(40, device="cuda")
+            w13, w2 = torch.empty(32, 40, dtype=dt, device="cuda"), torch.empty(24, 16, dtype=dt, device="cuda")
+            for t in (x, x.detach().requires_grad_(True)):
+                assert t.is_cuda and fused.rms_norm(t, w, 1e-6).shape == fused.layer_norm(t, w).shape == (6, 40)
+                assert fused.dropout(t, 0.5, 1).shape == (6, 40) and gated_ffn(t, w13, w2).shape == (6, 24)
+                assert fused.rms_norm(t, w, 1e-6).requires_grad == t.requires_grad
+        assert ext.train_norm(x, w, None, 1e-6, True) is None and ext.dropout(x, None, 9, 1, 1, None) is None
+        assert ext.gated_ffn(x, w13, w2, None, 0) is None and fused.layer_norm(x, w).shape == (6, 40)
+    a, w = torch.ones(6, 40), torch.ones(40)
+    neg = torch.ones(6, 40, dtype=torch.complex64).conj().imag
+    assert neg.is_neg() and ext.train_norm(neg, w, None, 1e-6, True) is None
+    assert ext.train_norm(a, neg[0], None, 1e-6, True) is None and ext.dropout(a, neg, 9, 1, 1, None) is None
+    assert ext.train_norm(torch._efficientzerotensor((3, 40)), w, None, 1e-6, True) is None
+    seen = []
+
+    def inside(t):  # t, or a tensor that the transform does not know of
+        seen.append(ext.train_norm(t, w, None, 1e-6, True) is None and ext.dropout(a, None, 9, 1, 1, None) is None)
+        return t.sum()
+    torch.func.vmap(inside)(a)
+    torch.func.grad(inside)(a)
+    torch.func.jvp(inside, (a,), (a,))
+    make_fx(inside)(a)
+    torch.jit.trace(inside, (a,), check_trace=False)
+    assert len(seen) == 5 and all(seen)
+    with pytest.raises(RuntimeError, match="CUDA"):  # and outside of all that they are refused where they are
+        ext.train_norm(a, w, None, 1e-6, True)

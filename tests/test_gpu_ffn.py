@@ -708,3 +708,96 @@ def test_calls_on_two_streams_at_once():
         for u, v in zip(a, b):
             assert torch.equal(u, v)
     check_status()
+
+
+def _transform_cases():
+    """name -> (function of x, inputs, their {name: (value, bound)} from the fp64 formulas, which takes (x, dy))."""
+    x, w, b, dy = norm_inputs(12, 264, FP, FP, seed=30)
+    keep = fused.dropout_keep_reference(12 * 264, 0.25, 5, 0, dev).view(12, 264).double() * (65536 / 49152)
+    fx, w13, w2, _, fdy = ffn_inputs(12, 64, 40, 72, BF, seed=31)
+
+    def drop64(x, dy):  # one rounded scale, one rounded product
+        return {n: (t.double() * keep, 4 * E * t.double().abs()) for n, t in (("y", x), ("dx", dy))}
+    return {"rms": (lambda t: fused.rms_norm(t, w, 1e-6), x, dy, lambda x, dy: norm_oracle(x, w, None, dy, 1e-6, True)),
+            "layer": (lambda t: fused.layer_norm(t, w, b, 1e-6), x, dy,
+                      lambda x, dy: norm_oracle(x, w, b, dy, 1e-6, False)),
+            "dropout": (lambda t: fused.dropout(t, 0.25, 5), x, dy, drop64),
+            "ffn": (lambda t: gated_ffn(t, w13, w2), fx, fdy, lambda x, dy: ffn_oracle(x, w13, w2, None, dy, "silu"))}
+
+
+def check_tangent(tangent, t, y, dy, dx):
+    """<dy, J t> = <J^T dy, t>: the tangent, off by at most as much as dx is (the same factors, in fp32) and one
+    rounding."""
+    a, b = (dy.double() * tangent.double()).sum(), (dx[0] * t.double()).sum()
+    bound = 2 * (dx[1] * t.double().abs()).sum() + 2 * u_of(y.dtype) * (dy.double() * tangent.double()).abs().sum()
+    assert tangent.dtype == y.dtype and (a - b).abs() <= bound
+
+
+@pytest.mark.parametrize("name", ["rms", "layer", "dropout", "ffn"])
+def test_function_transforms_and_traces(name):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x, dy, oracle = _transform_cases()[name]
+    ref = oracle(x, dy)
+    if name != "dropout":  # (a sample's mask there is that of a tensor of the sample's shape)
+        check(torch.func.vmap(f)(x.view(3, 4, -1)).view_as(dy), *ref["y"], "vmap")
+    else:
+        y = torch.func.vmap(f)(x.view(3, 4, -1))
+        assert all(torch.equal(y[i], f(x.view(3, 4, -1)[i])) for i in range(3))
+    check(torch.func.grad(lambda t: (f(t) * dy).sum(dtype=FP))(x), *ref["dx"], "grad")
+    y, tangent = torch.func.jvp(f, (x,), (x.flip(0),))
+    check(y, *ref["y"], "jvp")
+    check_tangent(tangent, x.flip(0), y, dy, ref["dx"])
+    other = x.flip(0) + 1
+    want = oracle(other, dy)["y"]
+    check(make_fx(f)(x)(other), *want, "make_fx")
+    check(torch.jit.trace(f, (x,), check_trace=False)(other), *want, "jit")
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        assert f(mode.from_tensor(x)).shape == dy.shape
+    kernels.reset()
+    check(f(x), *ref["y"], "kernel")
+    assert not kernels.counts()["fallback"]
+    check_status()
+
+
+@pytest.mark.parametrize("name", ["rms", "layer", "dropout", "ffn"])
+def test_batched_incoming_gradients(name):
+    """Several gradients at once go through the norms' formulas; the other two refuse them."""
+    f, x, dy, oracle = _transform_cases()[name]
+    leaf = x.clone().requires_grad_(True)
+    y = f(leaf)
+    many = torch.stack([dy, dy.flip(0), -2 * dy])
+    if name in ("dropout", "ffn"):
+        with pytest.raises(NotImplementedError, match="plain tensors"):
+            torch.autograd.grad(y, leaf, many, is_grads_batched=True)
+        return
+    (got,) = torch.autograd.grad(y, leaf, many, is_grads_batched=True)
+    for i in range(3):
+        check(got[i], *oracle(x, many[i])["dx"], i)
+
+
+def test_lazily_negated_views():
+    def lazy(t):  # t's values in a view whose memory holds -t
+        v = torch.complex(torch.zeros_like(t.float()), -t.float()).to(torch.complex32 if t.dtype == HF else torch.complex64)
+        v = v.conj().imag
+        assert v.is_neg() and torch.equal(v, t)
+        return v
+    x, w, b, dy = norm_inputs(9, 40, FP, FP, seed=32)
+    for rms in (True, False):
+        ref = norm_oracle(x, w, None if rms else b, dy, 1e-6, rms)
+        for k in range(4):
+            got = run_norm(*(lazy(t) if i == k else t for i, t in enumerate((x, w, b))), lazy(dy) if k == 3 else dy, 1e-6, rms)
+            for n in got:
+                check(got[n], *ref[n], (n, k))
+    assert torch.equal(fused.dropout(lazy(x), 0.3, 2, residual=dy), fused.dropout(x, 0.3, 2, residual=dy))
+    assert torch.equal(fused.dropout(x, 0.3, 2, residual=lazy(dy)), fused.dropout(x, 0.3, 2, residual=dy))
+    leaf = x.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(fused.dropout(leaf, 0.3, 2), leaf, lazy(dy))[0], fused.dropout(dy, 0.3, 2))
+    t = ffn_inputs(9, 64, 40, 72, HF, seed=33)
+    ref = ffn_oracle(*t, "silu")
+    for k in range(5):
+        x, w13, w2, res, dy = (lazy(v) if i == k else v for i, v in enumerate(t))
+        leaves = [v.detach().requires_grad_(True) for v in (x, w13, w2)]
+        y = gated_ffn(*leaves, residual=res)
+        for n, got in zip(("y", "dx", "dw13", "dw2"), (y.detach(), *torch.autograd.grad(y, leaves, dy))):
+            check(got, *ref[n], (n, k))
