@@ -33,8 +33,9 @@ def _ext():
     return C()
 
 
-def _gpu_bf16(*ts) -> bool:
-    return all(t.is_cuda and t.dtype == _BF and t.stride(-1) == 1 for t in ts)
+def _gpu_bf16(*ts) -> bool:  # (tensors that dispatch to Python, fake ones among them, have no memory to read)
+    return all(t.is_cuda and t.dtype == _BF and t.stride(-1) == 1
+               and type(t).__torch_dispatch__ is torch.Tensor.__torch_dispatch__ for t in ts)
 
 
 class _ConvSiLU(torch.autograd.Function):

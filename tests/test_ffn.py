@@ -200,3 +200,16 @@ def test_tensors_without_memory_never_reach_the_kernels():
     assert len(seen) == 5 and all(seen)
     with pytest.raises(RuntimeError, match="CUDA"):  # and outside of all that they are refused where they are
         ext.train_norm(a, w, None, 1e-6, True)
+
+
+def test_fake_tensors_take_the_plain_forms_of_the_student_kernels():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w = torch.empty(2, 6, 256, dtype=BF, device="cuda"), torch.empty(256, device="cuda")
+        cw, route = torch.empty(256, 4, device="cuda"), torch.empty(3, 4, dtype=torch.int64, device="cuda")
+        kernels.reset()
+        assert fused.rms_norm(x, w, 1e-6).shape == fused.gated_rms_norm(x, x, w, 1e-6).shape == x.shape
+        assert fused.conv_silu(x, cw).shape == x.shape and fused.swiglu(x).shape == (2, 6, 128)
+        assert fused.moe_combine(x.view(12, 256), route.view(-1), torch.empty(3, 4, device="cuda")).shape == (3, 256)
+        assert fused.moe_dispatch(x[0], route.view(-1), route.view(-1), 2) is None
+    assert not kernels.counts()["native"]
