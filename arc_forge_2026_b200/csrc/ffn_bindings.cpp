@@ -31,15 +31,19 @@ bool in_memory(const at::Tensor& t) {
   return !t.key_set().has_any(lazy);
 }
 bool in_memory(const OptT& t) { return !t.has_value() || in_memory(*t); }
+// a tensor that carries a tangent (forward-mode differentiation; it need not require a gradient)
+bool dual(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+bool dual(const OptT& t) { return t.has_value() && dual(*t); }
 // Whether operations have to go through the dispatcher: inside a function transform, under a dispatch mode or while a
-// trace is recorded, where a kernel launch would pass unseen. The callers then take their plain forms.
+// trace is recorded, where a kernel launch would pass unseen. There and for dual tensors, whose tangents the kernels do not
+// make, the callers take their plain forms.
 bool dispatched() {
   return c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing() ||
          c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
 }
 template <class... Ts>
 bool launchable(const Ts&... ts) {
-  return (in_memory(ts) && ...) && !dispatched();
+  return (in_memory(ts) && ...) && !(dual(ts) || ...) && !dispatched();
 }
 // an incoming gradient for a kernel
 at::Tensor gradient(const at::Tensor& t, const char* what) {

@@ -9,8 +9,9 @@ SwiGLU and token aggregation, ``fp8_moe.py`` _swiglu_backward / _routing_backwar
 
 Beside them, with trainable weights: :func:`layer_norm` and :func:`rms_norm` (``csrc/norm_train.cu``) and
 :func:`dropout` from a counter-based generator (``csrc/dropout.cu``); the gated feed-forward block is ``train/ffn.py``.
-These four take their plain forms inside function transforms (``torch.func``), under dispatch modes, while a trace is
-recorded, and for tensors whose memory is not their value (fake tensors, other subclasses, lazily negated views).
+These four take their plain forms inside function transforms (``torch.func``), in forward-mode differentiation, under
+dispatch modes, while a trace is recorded, and for tensors whose memory is not their value (fake tensors, other
+subclasses, lazily negated views).
 """
 from __future__ import annotations
 

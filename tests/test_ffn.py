@@ -213,3 +213,18 @@ def test_fake_tensors_take_the_plain_forms_of_the_student_kernels():
         assert fused.moe_combine(x.view(12, 256), route.view(-1), torch.empty(3, 4, device="cuda")).shape == (3, 256)
         assert fused.moe_dispatch(x[0], route.view(-1), route.view(-1), 2) is None
     assert not kernels.counts()["native"]
+
+
+def test_dual_tensors_never_reach_the_kernels():
+    """A tangent would be dropped without an error: a dual tensor does not require a gradient."""
+    pytest.importorskip("arc_forge_2026_b200._C")
+    import torch.autograd.forward_ad as fwad
+
+    from arc_forge_2026_b200.ops import C
+    x, w = torch.ones(6, 40), torch.ones(40)
+    with fwad.dual_level():
+        xd, wd = fwad.make_dual(x, x), fwad.make_dual(w, w)
+        for args in ((xd, w, None), (x, wd, None), (x, w, wd)):
+            assert C().train_norm(*args, 1e-6, False) is None
+        assert C().dropout(xd, None, 9, 1, 1, None) is None
+        assert C().dropout(x, xd, 9, 1, 1, None) is None

@@ -801,3 +801,28 @@ def test_lazily_negated_views():
         y = gated_ffn(*leaves, residual=res)
         for n, got in zip(("y", "dx", "dw13", "dw2"), (y.detach(), *torch.autograd.grad(y, leaves, dy))):
             check(got, *ref[n], (n, k))
+
+
+@pytest.mark.parametrize("name", ["rms", "layer", "dropout", "ffn"])
+def test_forward_mode_tangents(name):
+    """In a sum with x, where a dropped tangent would leave that of x; and tangents of the weights alone."""
+    import torch.autograd.forward_ad as fwad
+    f, x, dy, oracle = _transform_cases()[name]
+    ref, t = oracle(x, dy), x.flip(0)
+    with fwad.dual_level():
+        xd = fwad.make_dual(x, t)
+        kernels.reset()
+        y, tangent = fwad.unpack_dual(f(xd))
+        check(y, *ref["y"], "y")
+        check_tangent(tangent, t, y, dy, ref["dx"])
+        if name != "ffn":
+            total = fwad.unpack_dual(xd + f(xd)).tangent
+            assert torch.equal(total, t + tangent)
+        assert not any(kernels.counts()["native"].values())
+        if name in ("rms", "layer"):
+            w, b = norm_inputs(12, 264, FP, FP, seed=30)[1:3]
+            wd = fwad.make_dual(w, w.flip(0))
+            y = fused.rms_norm(x, wd, 1e-6) if name == "rms" else fused.layer_norm(x, wd, b, 1e-6)
+            check_tangent(fwad.unpack_dual(y).tangent, w.flip(0), x, dy, ref["dw"])
+        f(x)  # an open level without tangents changes nothing
+        assert kernels.counts()["native"] or name == "ffn"
