@@ -12,9 +12,10 @@ in fp32 (8 F bytes a row; nothing when neither x nor w13 asks for a gradient). W
 in two terms, so that only the result is rounded. Results do not depend on timing or on other work on the GPU: every
 sum has a fixed order.
 
-Off the GPU, in fp32, or when H, F or N is no multiple of 8 the plain-torch form runs. The student's shared experts
-and the drafter trainer's feed-forward use it when the registry name ``gated_ffn`` is enabled
-(``--fast-kernels all`` leaves it off, so their results stay what they were).
+Off the GPU, in fp32, or when H, F or N is no multiple of 8 the plain-torch form runs, and so it does everywhere when
+the kernel registry is ``none``. The student's shared experts and the drafter trainer's feed-forward use the block when
+the registry name ``gated_ffn`` is enabled (``--fast-kernels all`` leaves it off, so their results stay what they were);
+a call of :func:`gated_ffn` itself needs no name.
 """
 from __future__ import annotations
 
@@ -22,6 +23,8 @@ import functools
 
 import torch
 import torch.nn.functional as F
+
+from . import kernels
 
 ACTS = {"silu": 0, "gelu_tanh": 1, "gelu": 2}
 
@@ -46,11 +49,6 @@ def gated_ffn_reference(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, ac
     return y.to(x.dtype)
 
 
-def native_ok(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor) -> bool:
-    return (x.is_cuda and x.dtype in (torch.bfloat16, torch.float16) and w13.dtype == x.dtype and w2.dtype == x.dtype
-            and x.shape[-1] % 8 == 0 and w2.shape[0] % 8 == 0 and w2.shape[1] % 8 == 0)
-
-
 def _check(x, w13, w2, residual):
     if w13.dim() != 2 or w2.dim() != 2 or x.dim() < 1 or w13.shape[1] != x.shape[-1] \
             or w13.shape[0] != 2 * w2.shape[1]:
@@ -73,8 +71,10 @@ def gated_ffn(x: torch.Tensor, w13: torch.Tensor, w2: torch.Tensor, act: str = "
     code = ACTS.get(act)
     if code is None:
         raise ValueError(f"gated_ffn: unknown act {act!r}; known: {', '.join(ACTS)}")
-    if x.is_cuda:  # the binding checks the arguments and returns None for what the kernels do not cover
+    if x.is_cuda and kernels.any_enabled():
+        # the binding checks the arguments and returns None for what the kernels do not cover
         y = _ext().gated_ffn(x, w13, w2, residual, code)
+        kernels.hit("gated_ffn", y is not None)
         if y is not None:
             return y
     _check(x, w13, w2, residual)

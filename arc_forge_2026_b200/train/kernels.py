@@ -61,6 +61,11 @@ def use(name: str) -> bool:
     return name in _enabled
 
 
+def any_enabled() -> bool:
+    """False under ``none``: PyTorch everywhere, also for an opt-in op that is called by its own name."""
+    return bool(_enabled)
+
+
 def hit(name: str, native: bool):
     with _lock:
         (_calls if native else _fallbacks)[name] += 1

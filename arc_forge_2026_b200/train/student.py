@@ -24,7 +24,7 @@ from ..models.ple import PLELayer
 from ..quant.int3_tiles import codes_to_tiles
 from . import fused, kernels
 from .fakequant import fp8_weight, int3_weight
-from .ffn import gated_ffn, native_ok
+from .ffn import gated_ffn
 from .hc import hc_inject, hc_read
 from .gdn_chunk import chunk_gated_delta_rule
 
@@ -144,7 +144,6 @@ class StudentMoE(nn.Module):
         out = fused.moe_combine(y, inv, w)
         w13, w2 = self.shared_w13.to(x.dtype), self.shared_down.to(x.dtype)
         if x.is_cuda and kernels.use("gated_ffn"):  # opt-in: one kernel per direction for both input projections
-            kernels.hit("gated_ffn", native_ok(x, w13, w2))
             sh = gated_ffn(x, w13, w2)
         else:
             sh = fused.swiglu(x @ w13.t()) @ w2.t()

@@ -826,3 +826,23 @@ def test_forward_mode_tangents(name):
             check_tangent(fwad.unpack_dual(y).tangent, w.flip(0), x, dy, ref["dw"])
         f(x)  # an open level without tangents changes nothing
         assert kernels.counts()["native"] or name == "ffn"
+
+
+def test_registry_none_is_plain_torch_everywhere():
+    """``none`` holds for the block as well, whose name is opt-in; any list leaves a call of the block itself native."""
+    x, w13, w2, res, dy = ffn_inputs(20, 64, 40, 72, BF, seed=34)
+    ref = ffn_oracle(x, w13, w2, res, dy, "silu")
+    old = {n for n in kernels.NAMES if kernels.enabled(n)}
+    try:
+        for spec, native in (("none", 0), ("rms_norm", 1), ("all", 1), ("gated_ffn", 1)):
+            kernels.enable(spec)
+            kernels.reset()
+            check(gated_ffn(x, w13, w2, residual=res), *ref["y"], spec)
+            assert kernels.counts()["native"].get("gated_ffn", 0) == native
+            with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+                gated_ffn(x, w13, w2)
+                torch.cuda.synchronize()
+            names = [e.key for e in prof.key_averages()]
+            assert names and any("afb::ffn::" in n for n in names) == bool(native), names
+    finally:
+        kernels.enable(sorted(old))
