@@ -637,16 +637,16 @@ constexpr int64_t PREFETCH = 48 << 20;  // of the down projection's weights, int
 
 static int64_t weight_bytes(const FfnShape& s) { return (2 * (int64_t)s.H + s.N) * s.F * 2; }
 // Up to 32 rows an SM holds two CTAs, with more one, and clusters of a power of two leave SMs without one where there are
-// many weight tiles: so the limits. Measured, us here and as large tiles: 2,048 x 6,144 (75 MB of weights) 33 rows 27.6
-// and 31, 128 rows 33.7 and 31.5; 2,560 x 10,240 (157 MB) 33 rows 48 and 53, 65 rows 66 and 53; 4,096 x 8,192 (201 MB) 64
-// rows 54 and 54; 5,120 x 17,408 (535 MB) 32 rows 97 and 109, 33 rows 135 and 109. (Two CTAs an SM up to 64 rows as well:
-// 100 us for the last, but 2,048 x 2,048 14.6 -> 16.8.) Of few weights, where large tiles would be few and deep, 129 rows
-// of 2,048 x 1,024 (13 MB) 16 and 23, 384 rows 22.9 and 23.4, 512 23.6 and 23.5; 256 rows of 2,048 x 2,048 (25 MB) 23.6 and
-// 26.0, 257 27.3 and 26.5; 256 rows of 1,152 x 4,304 (30 MB) 28 and 23.
+// many weight tiles: so the limits, each between two measured sizes. Measured with cold weights, us here and as large
+// tiles. 64 rows: 2,560 x 10,240 (157 MB of weights) 51.5 and 52.0, 4,096 x 8,192 (201 MB) 52.5 and 49.7. 128 rows:
+// 2,560 x 4,096 (63 MB) 29.7 and 31.1, 2,048 x 6,144 (75 MB) 34.1 and 31.9 (80 rows 31.6 and 30.7); 4,096 x 5,120
+// (126 MB), whose tiles happen to fill the clusters, 43.3 and 44.8, 2,560 x 10,240 75 and 54. 256 rows: 2,048 x 2,048
+// (25 MB) 23.5 and 25.8, 1,152 x 4,304 (30 MB) 28.2 and 22.9. 384 rows: 2,048 x 1,536 (19 MB) 25.2 and 25.7,
+// 2,048 x 2,048 30.2 and 28.3; 512 rows of 2,048 x 1,024 23.6 and 23.5. 32 rows: 5,120 x 17,408 (535 MB) 96 and 104.
 static bool few(const FfnShape& s) {
   const int64_t b = weight_bytes(s);
-  return s.T <= 32 || (s.T <= 64 && b <= 200'000'000) || (s.T <= 128 && b <= 80'000'000) ||
-         (s.T <= 256 && b <= 26'000'000) || (s.T <= 384 && b <= 13'000'000);
+  return s.T <= 32 || (s.T <= 64 && b <= 180'000'000) || (s.T <= 128 && b <= 70'000'000) ||
+         (s.T <= 256 && b <= 27'000'000) || (s.T <= 384 && b <= 22'000'000);
 }
 
 template <bool DUAL_, int NT>
@@ -967,13 +967,15 @@ static int fwd_few(const FfnShape& s, Ptr x, Ptr w13, Ptr w2, Ptr residual, void
 // thread ends with both of a pair) or 16 of y. FMAs instead, with the rows' values in registers: 2 rows 18.4 us at
 // 2,048 x 6,144 and 14.3 at 1,152 x 4,304, 4 rows 27 and 15; this 18.3 and 10.7, 18.8 and 11.0.
 //
-// Measured, us here and in the kernels above: one row 2,048 x 6,144 15 and 20.6, 5,120 x 17,408 86 and 93 (6.2 TB/s and
-// 5.7), 2,048 x 512 4.7 and 8.7. Eight rows 2,048 x 512 5.5 and 9.0, 2,048 x 2,048 7.4 and 12.3, 2,048 x 6,144 (75 MB of
-// weights) 19.5 and 20.9, 5,120 x 17,408 (535 MB) 120 and 89, for a row's 64 bytes at a time are less than HBM wants.
-// Sixteen rows 2,048 x 512 5.2 and 9.3, 2,048 x 2,048 (25 MB) 10.6 and 12.6, 1,152 x 4,304 (30 MB) 16.2 and 14.7. 32
-// rows 2,048 x 512 (6 MB) 9.2 and 10.2, 256 x 136 6.6 and 10, 2,560 x 640 (10 MB) 13.9 and 11.5.
+// Measured with cold weights, us here and in the kernels above; the limits lie between two measured sizes. One row:
+// 2,048 x 6,144 15 and 20.6, 5,120 x 17,408 86 and 93 (6.2 TB/s and 5.7), 2,048 x 512 4.7 and 8.7. Eight rows:
+// 2,048 x 512 5.5 and 8.8, 2,048 x 2,048 7.8 and 11.9, 2,048 x 6,144 (75 MB of weights) 21.0 and 22.2, 2,560 x 6,144
+// (94 MB) 29.9 and 24.6 (rows of 2,560 take a second round of the warps' blocks for a quarter of it: 2,560 x 2,560 16.7
+// and 15.1), 5,120 x 17,408 (535 MB) 129 and 92, for a row's 64 bytes at a time are less than HBM wants. Sixteen rows:
+// 2,048 x 512 5.4 and 8.9, 2,048 x 2,048 (25 MB) 11.0 and 12.4, 1,152 x 4,304 (30 MB) 16.4 and 14.1. 32 rows:
+// 2,048 x 512 (6 MB) 8.2 and 9.9, 256 x 136 6.6 and 10, 2,560 x 640 (10 MB) 13.9 and 11.5.
 static bool tokens(const FfnShape& s) {
-  return s.T == 1 || (s.T <= 8 && weight_bytes(s) <= 100'000'000) || (s.T <= 16 && weight_bytes(s) <= 26'000'000) ||
+  return s.T == 1 || (s.T <= 8 && weight_bytes(s) <= 85'000'000) || (s.T <= 16 && weight_bytes(s) <= 27'000'000) ||
          (s.T <= 32 && weight_bytes(s) <= 7'000'000);
 }
 

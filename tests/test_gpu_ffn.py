@@ -155,6 +155,21 @@ def test_gated_ffn_where_the_kernels_change(size):
     check_status()
 
 
+@pytest.mark.parametrize("size", [(64, 4096, 7320), (64, 4096, 7328), (65, 2048, 5688), (128, 2048, 5704), (256, 1024, 4392),
+                                  (129, 1024, 4400), (257, 2048, 1784), (384, 2048, 1792), (8, 2048, 6912), (2, 2048, 6920),
+                                  (9, 2048, 2192), (16, 2048, 2200)])
+def test_gated_ffn_at_the_limits_of_rows_and_bytes(size):
+    """One size below and one above each limit of the weights' bytes; without gradients as well."""
+    T, H, F = size
+    t = ffn_inputs(T, H, F, H, BF, seed=T)
+    got, ref = run_ffn(*t, "silu"), ffn_oracle(*t, "silu")
+    for k in got:
+        check(got[k], *ref[k], k)
+    with torch.no_grad():
+        assert torch.equal(gated_ffn(*t[:3], residual=t[3]), got["y"])
+    check_status()
+
+
 def test_gated_ffn_gradient_against_differences():
     """<gradient, direction> of the kernels against the central difference of the fp64 block along the direction."""
     x, w13, w2, res, dy = ffn_inputs(96, 128, 200, 64, BF, seed=3)
