@@ -535,10 +535,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   }
 }
 
-// Fixed-order sum of the split-K partials [splits, rows, N] -> out [M, N]
+// Fixed-order sum of the split-K partials [splits, rows, N] (+ residual, rows ldr apart) -> out [M, N]
 template <bool F16>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ part, int splits, int64_t rows,
-                                                         int64_t M, int N, void* __restrict__ out) {
+                                                         int64_t M, int N, void* __restrict__ out,
+                                                         const uint16_t* __restrict__ residual, int64_t ldr) {
   grid_dep_wait();
   grid_dep_trigger();
   const int64_t idx = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
@@ -549,6 +550,16 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict
     const float4 b = *reinterpret_cast<const float4*>(part + s * rows * N + idx + 4);
     v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
     v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+  if (residual) {  // (N is a multiple of 8: the eight elements are of one row)
+    const uint4 q = *reinterpret_cast<const uint4*>(residual + idx / N * ldr + idx % N);
+    const uint32_t r[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<F16>(r[i]);
+      v[2 * i] += f.x;
+      v[2 * i + 1] += f.y;
+    }
   }
   *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + idx) =
       make_uint4(pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3]), pack2<F16>(v[4], v[5]), pack2<F16>(v[6], v[7]));
@@ -615,7 +626,7 @@ static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr res
   Maps<LAYOUT> maps;
   Args g;
   g.M = M, g.N = N, g.K = K, g.residual = residual.p, g.ldr = residual.ld;
-  g.splits = residual.p ? 1 : plan_splits(M, N, K, num_sms);
+  g.splits = plan_splits(M, N, K, num_sms);
   const int64_t rows = (M + BM - 1) / BM * BM;  // of a split's partial sums: whole tiles
   int rc = g.splits == 1 ? row_map(&maps.out[0], out, 2, N, M, N, 128)
                          : row_map(&maps.out[0], scratch, 4, N, rows * g.splits, N, 128);
@@ -624,7 +635,7 @@ static int product(Ptr A, Ptr B, int64_t M, int N, int64_t K, void* out, Ptr res
   rc = launch<LAYOUT, PARTIAL, F16>(A, B, N, maps, g, num_sms, status, st);
   if (rc) return rc;
   return launch_pdl(ffn_reduce_kernel<F16>, dim3((unsigned)((M * N / 8 + 255) / 256)), dim3(256), 0, st,
-                    (const float*)scratch, g.splits, rows, M, N, out);
+                    (const float*)scratch, g.splits, rows, M, N, out, (const uint16_t*)residual.p, residual.ld);
 }
 
 // ------------------------------------------------------------------------------------------ few rows

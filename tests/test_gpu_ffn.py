@@ -170,6 +170,26 @@ def test_gated_ffn_at_the_limits_of_rows_and_bytes(size):
     check_status()
 
 
+@pytest.mark.parametrize("size", [(385, 64, 8192, 1024), (400, 64, 4104, 264), (520, 64, 16392, 8)])
+def test_gated_ffn_residual_of_a_split_product(size):
+    """Few row tiles and a deep down projection: its K is split, and the residual is added where the parts are; rows of
+    a wider tensor, and the second kernel runs with it as without it."""
+    T, H, F, N = size
+    for dt in (BF, HF):
+        x, w13, w2, res, dy = ffn_inputs(T, H, F, N, dt, seed=T)
+        wide = torch.full((T, N + 24), float("nan"), dtype=dt, device=dev)
+        wide[:, 8:8 + N] = res
+        ref = ffn_oracle(x, w13, w2, res, dy, "silu")["y"]
+        with torch.no_grad():
+            for r in (res, wide[:, 8:8 + N]):
+                with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+                    y = gated_ffn(x, w13, w2, residual=r)
+                    torch.cuda.synchronize()
+                assert any("ffn_reduce_kernel" in e.key for e in prof.key_averages())
+                check(y, *ref, (dt, r.stride()))
+    check_status()
+
+
 def test_gated_ffn_gradient_against_differences():
     """<gradient, direction> of the kernels against the central difference of the fp64 block along the direction."""
     x, w13, w2, res, dy = ffn_inputs(96, 128, 200, 64, BF, seed=3)
