@@ -190,6 +190,43 @@ def test_gated_ffn_residual_of_a_split_product(size):
     check_status()
 
 
+# every kernel for few rows: one row, mma.sync with one, two and four groups of rows, clusters by weights and by rows
+TWO_TERMS = [(1, 72, 512), (2, 72, 512), (8, 72, 512), (16, 72, 512), (32, 72, 512), (4, 72, 600000), (16, 72, 192000),
+             (32, 72, 49152), (48, 72, 512), (100, 72, 512), (200, 72, 512), (384, 72, 520)]
+
+
+def two_term_bound(x, w13, w2):
+    """y of the block without gradients for few rows, its bound, and y as it would be if h were rounded once. h goes on
+    as two terms, so it is off by u^2 |h| (fp16: or half of its smallest step) beside the fp32 errors of ffn_oracle."""
+    u, H, F = u_of(x.dtype), x.shape[1], w2.shape[1]
+    a64, b64, c64 = x.double(), w13.double(), w2.double()
+    gu, gua = a64 @ b64.T, a64.abs() @ b64.abs().T
+    g, up, eg, eu = gu[:, :F], gu[:, F:], H * E * gua[:, :F], H * E * gua[:, F:]
+    a, _ = act64("silu", g)
+    ea = 1.2 * eg + 16 * E * (a.abs() + g.abs())
+    h = a * up
+    half_step = torch.finfo(HF).smallest_normal * torch.finfo(HF).eps / 2 if x.dtype == HF else 0.0
+    eh = u * u * h.abs() + half_step + (ea * (up.abs() + eu) + (a.abs() + ea) * eu) + 4 * E * h.abs()
+    y = h @ c64.T
+    e = eh @ c64.abs().T + F * E * ((h.abs() + eh) @ c64.abs().T)
+    tiny = torch.finfo(HF).tiny if x.dtype == HF else 0.0
+    return y, e + u * (y.abs() + e) + tiny, (h.to(x.dtype).double() @ c64.T).to(x.dtype)
+
+
+@pytest.mark.parametrize("size", TWO_TERMS)
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_gated_ffn_keeps_both_terms_of_h_for_few_rows(size, dt):
+    T, F, N = size
+    x, w13, w2, _, _ = ffn_inputs(T, 8, F, N, dt, seed=T, residual=False)
+    y, bound, once = two_term_bound(x, w13, w2)
+    assert ((once.double() - y).abs() > bound).any()  # the bound tells the two apart
+    with torch.no_grad():
+        check(gated_ffn(x, w13, w2), y, bound, size)
+    leaves = [t.requires_grad_(True) for t in (x, w13, w2)]
+    check(gated_ffn(*leaves).detach(), y, bound, "with gradients")
+    check_status()
+
+
 def test_gated_ffn_gradient_against_differences():
     """<gradient, direction> of the kernels against the central difference of the fp64 block along the direction."""
     x, w13, w2, res, dy = ffn_inputs(96, 128, 200, 64, BF, seed=3)
