@@ -9,7 +9,9 @@ lie (no transposed copies).
 Types: bf16 or fp16, weights in x's type. Sums are fp32; ``h`` and the gradients of the two pre-activations are
 rounded once to x's type (they are tensor-core operands); what the backward pass needs of the pre-activations is kept
 in fp32 (8 F bytes a row; nothing when neither x nor w13 asks for a gradient). With few rows the forward pass keeps h
-in two terms, so that only the result is rounded. Results do not depend on timing or on other work on the GPU: every
+in two terms, so that only the result is rounded (dw2 is made from the first of them). In fp16 the rounded values have
+fp16's range: an h, dg or du past 65,504 becomes infinite, and with it its row of y or dx and the weight gradients, where
+the plain form, which rounds nothing before its result, may still be finite. Results do not depend on timing or on other work on the GPU: every
 sum has a fixed order.
 
 Off the GPU, in fp32, or when H, F or N is no multiple of 8 the plain-torch form runs, and so it does everywhere when

@@ -298,6 +298,29 @@ def test_gated_ffn_no_rows_and_bad_values():
     check_status()
 
 
+@pytest.mark.parametrize("T", [1, 4, 30, 100, 500])
+def test_gated_ffn_fp16_range_of_the_intermediate_row(T):
+    """An h past fp16's largest number is infinite, in its own row alone; just below it everything is finite. bf16 has
+    the range of fp32."""
+    for dt, scale, finite in ((HF, 1.01, False), (HF, 0.99, True), (BF, 100.0, True)):
+        x, w13, w2 = (torch.zeros(*s, dtype=dt, device=dev) for s in ((T, 8), (16, 8), (16, 8)))
+        x[:, 0], x[:, 1] = 16, 16
+        w13[0, 0] = w13[8, 1] = 8  # g = u = 128: h = 16,384, silu(128) being 128
+        w2[:, 0] = 2.0 ** -6       # y = 256
+        big = (T - 1) // 2
+        x[big, 1] = 64 * scale     # h = 65,536 x scale, and 65,504 is the largest
+        with torch.no_grad():
+            y = gated_ffn(x, w13, w2)
+        rest = [i for i in range(T) if i != big]
+        assert (y[rest] == 256).all()
+        if finite:
+            h = float(x[big, 1]) * 8 * 128
+            assert ((y[big].double() - h / 64).abs() <= 3 * u_of(dt) * h / 64).all()
+        else:
+            assert not torch.isfinite(y[big]).any()
+    check_status()
+
+
 def test_gated_ffn_repeats_bitwise_and_on_other_streams():
     t = ffn_inputs(333, 256, 136, 256, BF, seed=6)
     a = run_ffn(*t, "silu")
