@@ -519,9 +519,12 @@ constexpr int RING_AHEAD = 96 * 1024;  // of that, what the CTAs of an SM keep o
 // Chunks a lane, warps a row, rows a CTA, CTAs, ring. Forward, the instructions a row takes decide the first two: some 8
 // an element and 75 a warp for its sums, so few warps with much each, as far as the lanes' last chunks are not left
 // idle (5,632 rows of 1,152 in bf16: three chunks 11 us, one 14, two 15, four 14). Backward, two chunks a lane (16,384
-// rows of 2,048 in bf16: 46 us; one chunk 61, for the sums of twice the warps; three 70 and four 65, for want of
-// registers), one where a row is 512 columns or less, four where it passes 8,192, and three from 4,097 to 4,608, where
-// two would leave an SM one CTA.
+// rows of 2,048 in bf16: 46 us; one chunk 61, for the sums of twice the warps; three 49 and four 65, for want of
+// registers), one where a row is 512 columns or less, and four where it passes 8,192. Where two would take more than six
+// warps they leave an SM one CTA, and three, up to the six warps of which two CTAs fit, are better in 16 bits and alike in
+// fp32 (10,485 rows of 3,200 in bf16 58 us, two 72; 8,192 of 4,096 49 and 59; 7,281 of 4,608 45 and 66; in fp32 4,096 of
+// 4,096 42 and 43). From 4,609 columns the backward pass has one CTA an SM (7,269 of 4,616 in bf16 67 us, 4,096 of 8,192
+// 50), the forward pass from 8,193.
 // CTAs: as many as are resident (a second wave would wait for the first). The rings of an SM's CTAs keep 96 KB on
 // the way: more makes the memory slower, not faster (96 and 160 KB: 16,383 rows of 2,048 in fp32 42.6 and 47.8 us forward,
 // 71.5 and 74.5 backward, 16,384 of 2,048 in bf16 24.8 and 26.4, 44.5 and 46.1; 64 KB: 24.7 and 44.0, but 5,633 of 4,608
@@ -532,7 +535,7 @@ static int plan(const NormArgs& a, int num_sms, Shape& s, Kernel& kern) {
   const int chunks = (a.width + 7) / 8;
   auto warps_of = [&](int nv) { return (chunks + 32 * nv - 1) / (32 * nv); };
   if (BWD) {
-    s.nv = chunks <= 64 ? 1 : warps_of(2) > 8 && warps_of(3) <= 6 ? 3 : warps_of(2) <= 16 ? 2 : 4;
+    s.nv = chunks <= 64 ? 1 : warps_of(2) > 6 && warps_of(3) <= 6 ? 3 : warps_of(2) <= 16 ? 2 : 4;
   } else {
     int best = INT32_MAX;
     for (int nv = warps_of(4) > 8 ? 4 : 1; nv <= 4; ++nv) {  // (four past 8,192 columns, where a CTA has 512 threads)

@@ -441,6 +441,18 @@ def test_trainable_norms(W, rms):
             check(got[k], *ref[k], (k, dt, wdt, T))
 
 
+@pytest.mark.parametrize("W", [2816, 3201, 3202, 3208, 3848, 4088, 4096, 4104, 4616])
+def test_trainable_norms_where_the_chunks_of_a_lane_change(W):
+    """Two and three chunks a lane in the backward pass; rows by eight, by pairs and one by one."""
+    for i, (dt, wdt, T, rms) in enumerate([(BF, FP, 37, False), (BF, BF, 700, True), (HF, FP, 1, False), (FP, FP, 300, False)]):
+        x, w, b, dy = norm_inputs(T, W, dt, wdt, seed=i)
+        got = run_norm(x, w, b, dy, 1e-6, rms)
+        ref = norm_oracle(x, w, None if rms else b, dy, 1e-6, rms)
+        for k in got:
+            check(got[k], *ref[k], (k, dt, wdt, T))
+    check_status()
+
+
 def test_norm_strides_empty_frozen_and_constant_rows():
     x, w, b, dy = norm_inputs(50, 264, BF, FP, seed=11)
     ref = norm_oracle(x, w, b, dy, 1e-6, False)
