@@ -13,9 +13,11 @@
 // reproducible).
 //
 // Measured (one B200): 16,383 x 2,048 fp32 forward 43 us (6.3 TB/s), backward 72 (5.6) + 4 for the sums;
-// 5,633 x 4,608 bf16 29 (3.6), 36 (4.3) + 4: 16-bit rows are bound by the instructions of their elements, some 11
-// forward and 17 backward, before memory. Rows of more than 8,192 columns leave an SM one CTA: 4,096 x 16,384 bf16 77 and
-// 265 us.
+// 5,633 x 4,608 bf16 29 (3.6), 36 (4.3) + 4. 16-bit rows have twice the elements a byte, some 11 instructions each
+// forward and 17 backward: neither memory (24 % and 42 % busy with reads and writes of DRAM) nor the issue slots (44 % and
+// 53 %) bound them, but the twelve warps an SM that the registers leave, which wait for their own shuffles and results.
+// Rows that leave an SM one CTA (past 4,608 columns backward, 8,192 forward) are slower: 4,096 x 8,192 bf16 40 and 50 us,
+// 2,048 x 16,384 40 and 144.
 #include <algorithm>
 #include <type_traits>
 
