@@ -627,6 +627,30 @@ def test_student_and_drafter_take_the_block_when_asked():
     check_status()
 
 
+def test_drafter_with_a_shared_feed_forward_takes_the_block_twice():
+    """Dense and shared feed-forward of a dense_shared drafter, bf16 operands against fp32 products: each part and each
+    weight gradient of a linear loss is off by three rounded factors a product, as above."""
+    from arc_forge_2026_b200.config import drafter_preset
+    from arc_forge_2026_b200.train.drafter_train import DrafterTrain
+    cfg = drafter_preset("tiny", ffn="dense_shared", shared_intermediate_size=64)
+    dt = DrafterTrain(cfg, 256, 512, torch.arange(128), device=dev)
+    m = dt.layers[0]
+    g = torch.Generator(device=dev).manual_seed(4)
+    y, v = (torch.randn(6, cfg.k, cfg.hidden_size, device=dev, generator=g) for _ in range(2))
+
+    def step():
+        o = dt._ffn(m, y, 0, None)
+        return [o.detach(), *torch.autograd.grad((o * v).sum(), [m.w13, m.w2, m.sw13, m.sw2])]
+    base = step()
+    dense, shared = dt._gated(y, m.w13, m.w2), torch.sigmoid(y @ m.shared_gate.t()) * dt._gated(y, m.sw13, m.sw2)
+    got, counts = _with_opt_in(step)
+    assert counts["native"]["gated_ffn"] == 2 and not counts["fallback"].get("gated_ffn")
+    assert (got[0] - base[0]).norm() <= 6 * u_of(BF) * (dense.norm() + shared.norm())
+    for a, b in zip(got[1:], base[1:]):
+        assert a.dtype == FP and (a - b).norm() <= 6 * u_of(BF) * b.norm()
+    check_status()
+
+
 def test_lora_dropout_on_the_native_products():
     """An adapter's output and gradients with dropout equal those of the adapter without it on the dropped input."""
     from arc_forge_2026_b200.train.lora import LoRAAdapter
