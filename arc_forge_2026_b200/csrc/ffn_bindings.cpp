@@ -36,7 +36,7 @@ bool dual(const at::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
 bool dual(const OptT& t) { return t.has_value() && dual(*t); }
 // Whether operations have to go through the dispatcher: inside a function transform, under a dispatch mode or while a
 // trace is recorded, where a kernel launch would pass unseen. There and for dual tensors, whose tangents the kernels do not
-// make, the callers take their plain forms.
+// make, the callers take their plain forms, and backward passes the formulas in ordinary operations.
 bool dispatched() {
   return c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing() ||
          c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
@@ -44,14 +44,6 @@ bool dispatched() {
 template <class... Ts>
 bool launchable(const Ts&... ts) {
   return (in_memory(ts) && ...) && !(dual(ts) || ...) && !dispatched();
-}
-// an incoming gradient for a kernel
-at::Tensor gradient(const at::Tensor& t, const char* what) {
-  if (in_memory(t)) return t;
-  const at::Tensor r = t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg();
-  TORCH_CHECK_NOT_IMPLEMENTED(in_memory(r), what, ": its backward pass takes plain tensors only, not those of a function ",
-                              "transform (is_grads_batched and the like)");
-  return r;
 }
 // x with its leading dimensions as one
 at::Tensor rows2d(const at::Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
@@ -317,11 +309,23 @@ struct GatedFfn : torch::autograd::Function<GatedFfn> {
     differentiable_once("gated_ffn");
     capturable_backward("gated_ffn");
     const variable_list v = ctx->get_saved_variables();
-    const at::Tensor dy = gradient(grads[0], "gated_ffn");
+    const at::Tensor& dy = grads[0];
     const bool need_x = ctx->needs_input_grad(0), need_w13 = ctx->needs_input_grad(1),
                need_w2 = ctx->needs_input_grad(2);
     variable_list out(5);
-    if (need_x || need_w13 || need_w2) {
+    if (!launchable(dy)) {
+      const int64_t act = ctx->saved_data["act"].toInt(), F = v[2].size(1);
+      const at::Tensor x = v[0].to(at::kFloat), w13 = v[1].to(at::kFloat), w2 = v[2].to(at::kFloat), d = dy.to(at::kFloat);
+      const at::Tensor gu = at::matmul(x, w13.t()), g = gu.narrow(-1, 0, F), u = gu.narrow(-1, F, F), one = at::ones_like(g);
+      const char* kind = act == 1 ? "tanh" : "none";
+      const at::Tensor a = act == 0 ? at::silu(g) : at::gelu(g, kind);
+      const at::Tensor da = act == 0 ? at::silu_backward(one, g) : at::gelu_backward(one, g, kind);
+      const at::Tensor dh = at::matmul(d, w2), dgu = at::cat({dh * u * da, dh * a}, -1);
+      const auto type = v[0].scalar_type();
+      if (need_x) out[0] = at::matmul(dgu, w13).to(type);
+      if (need_w13) out[1] = at::matmul(rows2d(dgu).t(), rows2d(x)).to(type);
+      if (need_w2) out[2] = at::matmul(rows2d(d).t(), rows2d(a * u)).to(type);
+    } else if (need_x || need_w13 || need_w2) {
       auto [dx, dw13, dw2] = gated_ffn_bwd(rows2d(dy), rows2d(v[0]), v[1], v[2], opt(v[3]), opt(v[4]),
                                            ctx->saved_data["act"].toInt(), need_x, need_w13, need_w2);
       if (dx) out[0] = dx->view(v[0].sizes());
@@ -374,8 +378,8 @@ struct TrainNorm : torch::autograd::Function<TrainNorm> {
     capturable_backward(rms ? "rms_norm" : "layer_norm");
     const variable_list v = ctx->get_saved_variables();
     variable_list out(5);
-    // create_graph, or a function transform's gradients: the formulas in operations that can be differentiated again
-    if (at::GradMode::is_enabled() || !in_memory(grads[0])) {
+    // create_graph, or gradients that no kernel can take: the formulas in operations that can be differentiated again
+    if (at::GradMode::is_enabled() || !launchable(grads[0])) {
       const at::Tensor x = v[0].to(at::kFloat), w = v[1].to(at::kFloat), dy = grads[0].to(at::kFloat);
       const at::Tensor c = rms ? x : x - x.mean({-1}, true);
       const at::Tensor rstd = at::rsqrt(c.square().mean({-1}, true) + ctx->saved_data["eps"].toDouble());
@@ -419,9 +423,29 @@ struct Dropout : torch::autograd::Function<Dropout> {
     differentiable_once("dropout");
     capturable_backward("dropout");
     variable_list out(6);
-    if (ctx->needs_input_grad(0))
-      out[0] = dropout_op(gradient(grads[0], "dropout"), OptT(), ctx->saved_data["threshold"].toInt(), ctx->saved_data["seed"].toInt(),
-                          ctx->saved_data["offset"].toInt(), opt(ctx->get_saved_variables()[0]));
+    if (ctx->needs_input_grad(0)) {
+      const int64_t threshold = ctx->saved_data["threshold"].toInt();
+      auto masked = [&](const at::Tensor& t) {
+        return dropout_op(t, OptT(), threshold, ctx->saved_data["seed"].toInt(), ctx->saved_data["offset"].toInt(),
+                          opt(ctx->get_saved_variables()[0]));
+      };
+      const at::Tensor& dy = grads[0];
+      if (launchable(dy)) {
+        out[0] = masked(dy);
+      } else {  // the mask from a tensor that no transform and no mode knows of
+        at::Tensor keep;
+        {
+          c10::impl::ExcludeDispatchKeyGuard unseen(
+              c10::DispatchKeySet({c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::Tracer,
+                                   c10::DispatchKey::FuncTorchDynamicLayerFrontMode,
+                                   c10::DispatchKey::FuncTorchDynamicLayerBackMode}));
+          const auto device = at::TensorOptions().dtype(at::kFloat).device(dy.device());
+          keep = masked(at::ones(dy.sizes(), device)).ne(0.);
+        }
+        const at::Tensor y = dy.to(at::kFloat) * (threshold ? 65536. / threshold : 0.);
+        out[0] = at::where(keep, y, at::zeros({}, y.options())).to(dy.scalar_type());
+      }
+    }
     if (ctx->saved_data["residual"].toBool()) out[1] = grads[0];
     return out;
   }

@@ -892,19 +892,42 @@ def test_function_transforms_and_traces(name):
 
 
 @pytest.mark.parametrize("name", ["rms", "layer", "dropout", "ffn"])
-def test_batched_incoming_gradients(name):
-    """Several gradients at once go through the norms' formulas; the other two refuse them."""
+def test_incoming_gradients_that_no_kernel_can_take(name):
+    """Several gradients at once, gradients with a tangent, and a recorded backward pass: x itself is an ordinary tensor,
+    so the forward pass ran the kernels; the backward pass goes through the formulas."""
+    import torch.autograd.forward_ad as fwad
+    from torch.fx.experimental.proxy_tensor import make_fx
     f, x, dy, oracle = _transform_cases()[name]
     leaf = x.clone().requires_grad_(True)
     y = f(leaf)
+
+    def grad(d, **kw):
+        return torch.autograd.grad(y, leaf, d, retain_graph=True, **kw)[0]
     many = torch.stack([dy, dy.flip(0), -2 * dy])
-    if name in ("dropout", "ffn"):
-        with pytest.raises(NotImplementedError, match="plain tensors"):
-            torch.autograd.grad(y, leaf, many, is_grads_batched=True)
-        return
-    (got,) = torch.autograd.grad(y, leaf, many, is_grads_batched=True)
+    got = grad(many, is_grads_batched=True)
     for i in range(3):
         check(got[i], *oracle(x, many[i])["dx"], i)
+    with fwad.dual_level():  # the backward pass is linear in dy: its tangent is that of dy, sent through it
+        dx, tangent = fwad.unpack_dual(grad(fwad.make_dual(dy, many[1])))
+        check(dx, *oracle(x, dy)["dx"], "dual")
+        check(tangent, *oracle(x, many[1])["dx"], "tangent")
+    check(make_fx(grad)(dy)(many[2]), *oracle(x, many[2])["dx"], "make_fx")
+    check(grad(dy), *oracle(x, dy)["dx"], "kernel")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh", "gelu"])
+def test_gated_ffn_gradients_from_the_formulas(act):
+    """All gradients of a backward pass that no kernel can take, with leading dimensions and a residual."""
+    x, w13, w2, res, dy = ffn_inputs(24, 64, 40, 72, BF, seed=35)
+    leaves = [t.clone().requires_grad_(True) for t in (x.view(2, 3, 4, 64), w13, w2, res.view(2, 3, 4, 72))]
+    y = gated_ffn(*leaves[:3], act=act, residual=leaves[3])
+    many = torch.stack([dy, dy.flip(0)])
+    got = torch.autograd.grad(y, leaves, many.view(2, 2, 3, 4, 72), is_grads_batched=True)
+    for i in range(2):
+        ref = ffn_oracle(x, w13, w2, res, many[i], act)
+        for k, t in zip(("dx", "dw13", "dw2"), got):
+            check(t[i].reshape(ref[k][0].shape), *ref[k], (k, i))
+    assert torch.equal(got[3].view_as(many), many)
 
 
 def test_lazily_negated_views():
